@@ -15,6 +15,7 @@ import numpy as np
 MODE_MX, MODE_DS = 0, 1
 FMT_FP8, FMT_FP4 = 0, 1
 SCORE_IDENTITY, SCORE_SOFTMAX, SCORE_SQRT_SOFTPLUS = 0, 1, 2
+KV_BF16, KV_E4M3 = 0, 1
 EPI_STORE, EPI_SWIGLU, EPI_SQRT_SOFTPLUS, EPI_ACCUMULATE = 0, 1, 2, 3   # dsuf_gemm_opts.epilogue
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -47,6 +48,15 @@ class GemmOpts(C.Structure):
 
 class SamplingOpts(C.Structure):
     _fields_ = [("records", C.c_uint64), ("temperature", C.c_float), ("valid_rows", C.c_int32), ("id_offset", C.c_int32)]
+
+
+class KvCacheStruct(C.Structure):
+    _fields_ = [("k", C.c_uint64), ("v", C.c_uint64), ("k_scale", C.c_uint64), ("v_scale", C.c_uint64), ("page_stride", C.c_int64),
+                ("dtype", C.c_int32), ("n_pages", C.c_int32), ("page_size", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32)]
+
+
+class RopeStruct(C.Structure):
+    _fields_ = [("cos", C.c_uint64), ("sin", C.c_uint64), ("positions", C.c_int32), ("rot", C.c_int32), ("off", C.c_int32), ("half", C.c_int32)]
 
 
 class TensorInfo(C.Structure):
@@ -130,6 +140,13 @@ ABI = {
                                        C.c_int32, C.c_int32, C.c_uint64, C.c_int32]),
     "dsuf_moe_unpermute_quant": (C.c_int32, [C.c_void_p, C.c_void_p, C.POINTER(PlanStruct), C.c_uint64, C.c_uint64, C.c_int32, C.c_int32,
                                              C.c_int32, C.c_uint64, C.c_int32, C.c_int32, C.c_uint64, C.c_uint64]),
+    "dsuf_kv_append": (C.c_int32, [C.c_void_p, C.c_void_p, C.POINTER(KvCacheStruct), C.c_uint64, C.c_int32, C.c_uint64, C.c_int32, C.c_int32,
+                                   C.c_uint64, C.c_uint64, C.c_uint64, C.c_int32, C.c_int32, C.POINTER(RopeStruct), C.c_uint64, C.c_int32,
+                                   C.c_int32, C.c_uint64, C.c_int32]),
+    "dsuf_attn_workspace_bytes": (C.c_size_t, [C.c_void_p]),
+    "dsuf_attn_workspace_init": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_size_t]),
+    "dsuf_attn_decode": (C.c_int32, [C.c_void_p, C.c_void_p, C.POINTER(KvCacheStruct), C.c_uint64, C.c_int32, C.c_int32, C.c_int32, C.c_uint64,
+                                     C.c_int32, C.c_uint64, C.c_float, C.c_int32, C.c_uint64, C.c_int32, C.c_uint64, C.c_uint64]),
 }
 
 
@@ -284,7 +301,16 @@ class Ctx:
         nbytes = lib().dsuf_gemm_workspace_bytes(self.h)
         self.workspace = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
         self.check(lib().dsuf_workspace_init(self.h, self.stream(), self.workspace.data_ptr(), nbytes))
+        self.attn_workspace = self.new_attn_workspace()
         self.sm_count = lib().dsuf_sm_count(self.h)
+
+    def new_attn_workspace(self):
+        """A workspace for attn_decode, ready for use: calls and captured graphs that may run at the same time need one each."""
+        t = self.torch
+        nbytes = lib().dsuf_attn_workspace_bytes(self.h)
+        w = t.empty(nbytes, dtype=t.uint8, device=self.device)
+        self.check(lib().dsuf_attn_workspace_init(self.h, self.stream(), w.data_ptr(), nbytes))
+        return w
 
     def set_decode_path(self, tcgen05):
         """True: tcgen05 streaming kernels for decode shapes; False: the mma.sync streaming kernels."""
@@ -575,6 +601,126 @@ def lm_head(ctx, w, x, alpha=1.0, out=None, temperature=None, valid_rows=0, id_o
     ctx.check(lib().dsuf_lm_head_bf16(ctx.h, ctx.stream(), w.data_ptr(), n, k, x.data_ptr(), x.stride(0), m, alpha, out.data_ptr(),
                                       out.stride(0), C.byref(sp) if sp is not None else None))
     return (out, records) if temperature is not None else out
+
+
+def _need(cond, msg):
+    if not cond:
+        raise DsufError(-1, msg)
+
+
+def _need_tensor(ctx, name, x, dtype, shape, rows=False):
+    """x is a tensor of this type and shape (None: any size) on the context's device; contiguous, or with ``rows`` a matrix
+    whose rows may lie apart."""
+    _need(isinstance(x, ctx.torch.Tensor) and x.device == ctx.device and x.dtype == dtype,
+          f"{name}: a {dtype} tensor on {ctx.device} is wanted")
+    _need(x.dim() == len(shape) and all(w is None or g == w for g, w in zip(x.shape, shape)), f"{name}: shape {tuple(x.shape)}, wanted {tuple(shape)}")
+    if rows:
+        _need(x.numel() == 0 or (x.stride(1) == 1 and (x.shape[0] < 2 or x.stride(0) >= x.shape[1])), f"{name}: rows must be contiguous and not overlap")
+    else:
+        _need(x.is_contiguous(), f"{name}: must be contiguous")
+
+
+def _ld(x):
+    """Row stride of a matrix; that of a single row is its length, whatever the tensor says."""
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+class KvCache:
+    """dsuf_kv_cache: one layer's paged cache over tensors k, v [n_pages][kv_heads][page_size][head_dim], bf16 or (uint8 codes)
+    e4m3 with optional f32 scales per kv head.  The pages may lie apart (a slice of a tensor that holds all layers)."""
+
+    def __init__(self, ctx, k, v, k_scale=None, v_scale=None):
+        t = ctx.torch
+        _need(isinstance(k, t.Tensor) and k.dim() == 4 and k.dtype in (t.bfloat16, t.uint8), "KvCache: k must be bf16 or uint8 [pages][kv_heads][page][head_dim]")
+        n, h, p, d = k.shape
+        for name, x in (("k", k), ("v", v)):
+            _need(isinstance(x, t.Tensor) and x.device == ctx.device and x.dtype == k.dtype and x.shape == k.shape, f"KvCache: {name}: type, shape or device")
+            _need(x.stride()[1:] == (p * d, d, 1) and x.stride(0) == k.stride(0), f"KvCache: {name}: the heads of a page must be contiguous, k's and v's pages equally far apart")
+        for name, x in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if x is not None:
+                _need_tensor(ctx, "KvCache: " + name, x, t.float32, (h,))
+        self.ctx, self.k, self.v, self.k_scale, self.v_scale = ctx, k, v, k_scale, v_scale   # (keeps the tensors alive)
+        self.n_pages, self.kv_heads, self.page_size, self.head_dim = n, h, p, d
+        self.c = KvCacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if k_scale is not None else 0,
+                               v_scale.data_ptr() if v_scale is not None else 0, max(k.stride(0), h * p * d) if n > 1 else h * p * d,
+                               KV_BF16 if k.dtype == t.bfloat16 else KV_E4M3, n, p, h, d)
+
+    @staticmethod
+    def empty(ctx, n_pages, page_size, kv_heads, head_dim, fp8=False, k_scale=None, v_scale=None):
+        """A cache of its own memory (zeros)."""
+        t = ctx.torch
+        shape = (n_pages, kv_heads, page_size, head_dim)
+        k, v = (t.zeros(shape, dtype=t.uint8 if fp8 else t.bfloat16, device=ctx.device) for _ in range(2))
+        return KvCache(ctx, k, v, k_scale, v_scale)
+
+
+def kv_append(ctx, cache, k, v, pos, block_table, seq=None, rope=None, rope_half=False, q=None, q_out=None):
+    """dsuf_kv_append: writes the tokens' keys (rotated) and values bf16 [t][kv_heads * head_dim] into the cache at positions
+    ``pos`` i32 [t] of sequences ``seq`` i32 [t] (None: token i is sequence i), pages from ``block_table`` i32 [seqs][pages]; a
+    negative pos or seq is padding.  ``rope`` = (cos f32 [positions][rot/2], sin, off): columns [off, off + rot) of every head, in
+    (even, odd) pairs or with ``rope_half`` in pairs rot/2 apart.  ``q`` bf16 [t][q_heads * head_dim]: rotated as well, into
+    ``q_out`` (None: a new tensor; q itself: in place).  Returns q_out."""
+    t = ctx.torch
+    _need(cache.ctx is ctx, "kv_append: the cache belongs to another context")
+    d = cache.head_dim
+    _need_tensor(ctx, "kv_append: k", k, t.bfloat16, (None, cache.kv_heads * d), rows=True)
+    n = k.shape[0]
+    _need_tensor(ctx, "kv_append: v", v, t.bfloat16, (n, cache.kv_heads * d), rows=True)
+    _need_tensor(ctx, "kv_append: pos", pos, t.int32, (n,))
+    _need_tensor(ctx, "kv_append: block_table", block_table, t.int32, (None, None))
+    if seq is not None:
+        _need_tensor(ctx, "kv_append: seq", seq, t.int32, (n,))
+    r = None
+    if rope is not None:
+        cos, sin, off = rope
+        _need_tensor(ctx, "kv_append: cos", cos, t.float32, (None, None))
+        _need_tensor(ctx, "kv_append: sin", sin, t.float32, cos.shape)
+        r = RopeStruct(cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1], int(off), int(bool(rope_half)))
+    heads = 0
+    if q is not None:
+        _need_tensor(ctx, "kv_append: q", q, t.bfloat16, (n, None), rows=True)
+        _need(q.shape[1] % d == 0 and q.shape[1] > 0, "kv_append: q's rows must hold whole heads")
+        heads = q.shape[1] // d
+        if q_out is None:
+            q_out = t.empty((n, heads * d), dtype=t.bfloat16, device=ctx.device)
+        else:
+            _need_tensor(ctx, "kv_append: q_out", q_out, t.bfloat16, q.shape, rows=True)
+    ctx.check(lib().dsuf_kv_append(ctx.h, ctx.stream(), C.byref(cache.c), k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), n, pos.data_ptr(),
+                                   seq.data_ptr() if seq is not None else 0, block_table.data_ptr(), block_table.shape[0], block_table.shape[1],
+                                   C.byref(r) if r is not None else None, q.data_ptr() if heads else 0, _ld(q) if heads else 0, heads,
+                                   q_out.data_ptr() if heads else 0, _ld(q_out) if heads else 0))
+    return q_out
+
+
+def attn_decode(ctx, cache, q, block_table, seq_lens, scale=None, window=0, out=None, lse=None, return_lse=False, workspace=None):
+    """dsuf_attn_decode: attention of one new token per sequence, q bf16 [b][q_heads * head_dim], over the cached positions
+    [max(0, len - window), len) with len = ``seq_lens`` i32 [b] (the new token included, its key already appended); ``scale`` None:
+    head_dim ** -0.5.  Returns out bf16 [b][q_heads * head_dim], or (out, lse f32 [b][q_heads]) with ``return_lse``.
+    ``workspace``: one of ctx.new_attn_workspace() for calls that may overlap others of this context."""
+    t = ctx.torch
+    _need(cache.ctx is ctx, "attn_decode: the cache belongs to another context")
+    d = cache.head_dim
+    _need_tensor(ctx, "attn_decode: q", q, t.bfloat16, (None, None), rows=True)
+    b, width = q.shape
+    _need(width > 0 and width % (d * cache.kv_heads) == 0, "attn_decode: q's rows must hold a multiple of kv_heads heads")
+    _need_tensor(ctx, "attn_decode: block_table", block_table, t.int32, (b, None))
+    _need_tensor(ctx, "attn_decode: seq_lens", seq_lens, t.int32, (b,))
+    if out is None:
+        out = t.empty((b, width), dtype=t.bfloat16, device=ctx.device)
+    else:
+        _need_tensor(ctx, "attn_decode: out", out, t.bfloat16, (b, width), rows=True)
+    if lse is not None:
+        _need_tensor(ctx, "attn_decode: lse", lse, t.float32, (b, width // d))
+    elif return_lse:
+        lse = t.empty((b, width // d), dtype=t.float32, device=ctx.device)
+    if workspace is None:
+        workspace = ctx.attn_workspace
+    else:
+        _need_tensor(ctx, "attn_decode: workspace", workspace, t.uint8, (ctx.attn_workspace.numel(),))
+    ctx.check(lib().dsuf_attn_decode(ctx.h, ctx.stream(), C.byref(cache.c), q.data_ptr(), _ld(q), width // d, b, block_table.data_ptr(),
+                                     block_table.shape[1], seq_lens.data_ptr(), d ** -0.5 if scale is None else scale, window, out.data_ptr(), _ld(out),
+                                     lse.data_ptr() if lse is not None else 0, workspace.data_ptr()))
+    return (out, lse) if return_lse else out
 
 
 def probe_tensor_rate(ctx, n_cols=128, a_is_e2m1=False, iters=20000, reps=5):

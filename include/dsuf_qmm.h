@@ -388,6 +388,54 @@ typedef struct {
 int32_t dsuf_lm_head_bf16(dsuf_ctx* ctx, void* stream, uint64_t w, int32_t n, int32_t k, uint64_t x, int32_t ldx, int32_t m,
                           float alpha, uint64_t out, int32_t ldo, const dsuf_sampling_opts* sp);
 
+/* ---- paged key/value cache and attention ----
+ * The reference's attention (crates/kernels/cu/attn.cu) is specific to its model (compressed shared keys and values); these
+ * entries are the general grouped-head form, so that the projections and experts of this library compose into whole layers.
+ * One dsuf_kv_cache describes one layer's cache: page p, kv head h, slot s, column d lies at element
+ * p * page_stride + (h * page_size + s) * head_dim + d of k and of v.  A block table i32 [n_seqs][max_pages] (device) names the
+ * page of every page_size consecutive positions of a sequence.
+ *   dtype        DSUF_KV_BF16, or DSUF_KV_E4M3: stored code = e4m3(x / scale[h]) (IEEE division, saturating at 448), read back
+ *                as code * scale[h]
+ *   page_size    a power of two, 16..1024;  head_dim 64 or 128
+ *   page_stride  elements, at least kv_heads * page_size * head_dim and a multiple of 16 (layers may be interleaved)
+ *   k_scale/v_scale  f32 [kv_heads] on the device, E4M3 only; 0 = all ones
+ * Device-side indexes are checked on the device: a page id outside [0, n_pages), a position outside the block table's row or
+ * the rotation table, or a sequence outside [0, n_seqs) is never followed; it is reported as code 2 (inconsistent plan) by
+ * dsuf_status_poll, and the token (append) or the 16 keys (attention) concerned are skipped. */
+enum { DSUF_KV_BF16 = 0, DSUF_KV_E4M3 = 1 };
+typedef struct {
+    uint64_t k, v;
+    uint64_t k_scale, v_scale;
+    int64_t page_stride;
+    int32_t dtype, n_pages, page_size, kv_heads, head_dim;
+} dsuf_kv_cache;
+/* Rotary embedding of columns [off, off + rot) of every head: cos / sin f32 [positions][rot / 2] on the device (the tables of
+ * dsuf_gemm_opts.rope_cos / rope_sin); pair i is columns (off + 2i, off + 2i + 1), or with half != 0 (off + i, off + i + rot/2).
+ * (a, b) -> (a cos - b sin, b cos + a sin) in fp32.  rot % 16 == 0, off % 8 == 0. */
+typedef struct {
+    uint64_t cos, sin;
+    int32_t positions, rot, off, half;
+} dsuf_rope;
+/* Writes t tokens' keys (rotated to their positions when rope is given) and values into the cache and, with q_heads > 0, the
+ * rotated queries to q_out (q_out = q: in place).  k, v bf16 [t][kv_heads * head_dim] (row strides ldk, ldv), q / q_out bf16
+ * [t][q_heads * head_dim]; pos i32 [t], seq i32 [t] (0: token i belongs to sequence i, t <= n_seqs).  A token with a negative
+ * pos or seq is padding: nothing of it is written.  The (seq, pos) pairs of one call must be distinct, and distinct sequences must not
+ * share the pages that are written: which of two writes to one slot lands is undefined. */
+int32_t dsuf_kv_append(dsuf_ctx* ctx, void* stream, const dsuf_kv_cache* cache, uint64_t k, int32_t ldk, uint64_t v, int32_t ldv, int32_t t,
+                       uint64_t pos, uint64_t seq, uint64_t block_table, int32_t n_seqs, int32_t max_pages, const dsuf_rope* rope,
+                       uint64_t q, int32_t ldq, int32_t q_heads, uint64_t q_out, int32_t ldqo);
+/* Attention of one new token per sequence over the cache: out[b][h] = sum_j softmax_j(scale * <q[b][h], K_j>) V_j over positions
+ * j in [max(0, len - window), len) (window 0: all), kv head = h / (q_heads / kv_heads).  The new token's own key is in the cache
+ * already (dsuf_kv_append); seq_lens i32 [b] counts it.  A sequence of length <= 0 gives zeros and lse -inf.
+ * q / out bf16 [b][q_heads * head_dim]; lse f32 [b][q_heads] = log of the sum of exp(scale * <q, k>), or 0.
+ * q_heads a multiple of kv_heads.  workspace: dsuf_attn_workspace_bytes(ctx), zeroed once by dsuf_attn_workspace_init; the kernel
+ * leaves its counters zeroed.  Calls (and captured graphs) that share one workspace must be stream-ordered. */
+size_t dsuf_attn_workspace_bytes(dsuf_ctx* ctx);
+int32_t dsuf_attn_workspace_init(dsuf_ctx* ctx, void* stream, uint64_t workspace, size_t bytes);
+int32_t dsuf_attn_decode(dsuf_ctx* ctx, void* stream, const dsuf_kv_cache* cache, uint64_t q, int32_t ldq, int32_t q_heads, int32_t b,
+                         uint64_t block_table, int32_t max_pages, uint64_t seq_lens, float scale, int32_t window, uint64_t out,
+                         int32_t ldo, uint64_t lse, uint64_t workspace);
+
 #ifdef __cplusplus
 }
 #endif

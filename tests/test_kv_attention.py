@@ -1,0 +1,225 @@
+"""Paged cache, decode attention and prompt attention against their definitions in 64 bits.
+
+Tolerances count roundings: a bf16 output is off by at most half a step (2^-8 relative) plus what its inputs' roundings give.
+The softmax weights enter the second product rounded to bf16 (2^-8 each, at worst all in one direction), so an output is within
+2^-8 of its own magnitude plus 2^-8 of sum_j p_j |v_j|, the sum of its terms' magnitudes; fp32 sums and base-2 exponentials add
+less than 2^-12 of that sum (a score s has an absolute error of about d 2^-24 sum |q k| scale, below 2^-14 for these inputs)."""
+import math
+
+import pytest
+import torch
+
+gpu = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.fixture(scope="module")
+def actx(pkg):
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    c = pkg.Ctx(0)
+    yield c
+    c.close()
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def bf16(g, *shape, std=1.0):
+    return torch.empty(*shape, dtype=torch.bfloat16, device=DEV).normal_(0.0, std, generator=g)
+
+
+def tables(positions, rot):
+    angle = torch.arange(positions, dtype=torch.float64, device=DEV)[:, None] * 10000.0 ** (-torch.arange(rot // 2, dtype=torch.float64, device=DEV) * 2 / rot)
+    return angle.cos().float(), angle.sin().float()
+
+
+def turned64(x, cos, sin, off, half):
+    """x [t][h][d] with the pairs of columns [off, off + rot) turned, in 64 bits; cos, sin [t][rot / 2]."""
+    x = x.double().clone()
+    m = cos.shape[1]
+    for i in range(m):
+        a, b = (off + i, off + i + m) if half else (off + 2 * i, off + 2 * i + 1)
+        c, s = cos[:, i].double()[:, None], sin[:, i].double()[:, None]
+        u, w = x[..., a].clone(), x[..., b].clone()
+        x[..., a], x[..., b] = u * c - w * s, w * c + u * s
+    return x
+
+
+def within(got, want, size, rel=2 ** -8, terms=0.0):
+    """|got - want| <= rel |want| + terms size, elementwise; size: the magnitudes of what was added up."""
+    got, want = got.double(), want.double()
+    assert got.shape == want.shape
+    over = (got - want).abs() - (rel * want.abs() + terms * size + 1e-30)
+    assert not torch.isnan(got).any() and over.max().item() <= 0, f"off by {over.max().item()} more than allowed"
+
+
+def make_cache(pkg, ctx, g, pages, hkv, page, d, fp8, scales=True):
+    if fp8:
+        k, v = (torch.randn(pages, hkv, page, d, generator=g, device=DEV).mul_(60).clamp_(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8) for _ in range(2))
+        ks, vs = (torch.rand(hkv, generator=g, device=DEV) * 0.02 + 0.01 for _ in range(2)) if scales else (None, None)
+        return pkg.KvCache(ctx, k, v, ks, vs)
+    return pkg.KvCache(ctx, bf16(g, pages, hkv, page, d), bf16(g, pages, hkv, page, d))
+
+
+def cache64(cache, scaled=True):
+    out = []
+    for x, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
+        y = x.view(torch.float8_e4m3fn).double() if x.dtype == torch.uint8 else x.double()
+        out.append(y * s.double()[None, :, None, None] if scaled and s is not None else y)
+    return out
+
+
+# ------------------------------------------------------------------ append
+@gpu
+@pytest.mark.parametrize("d,hq,hkv,rot,off,half", [(128, 7, 1, 128, 0, False), (128, 56, 8, 64, 64, False), (64, 3, 3, 64, 0, True), (128, 6, 2, 32, 8, True),
+                                                   (64, 0, 5, 16, 40, False), (128, 4, 4, 0, 0, False), (128, 5, 1, 128, 0, True)])
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("t,page", [(1, 16), (37, 32), (700, 128)])
+def test_append(pkg, actx, d, hq, hkv, rot, off, half, fp8, t, page):
+    g = gen(t + d + hq + rot)
+    seqs, pages = 5, max(2, -(-t // 5 // page) + 2)
+    cache = make_cache(pkg, actx, g, seqs * pages + 2, hkv, page, d, fp8, scales=rot != 64)
+    k_before, v_before = cache.k.clone(), cache.v.clone()
+    rows = bf16(g, t, (hq + 2 * hkv) * d + 8)[:, : (hq + 2 * hkv) * d]
+    q, k, v = rows.split([hq * d, hkv * d, hkv * d], 1)
+    table = torch.randperm(seqs * pages + 2, generator=g, device=DEV)[: seqs * pages].reshape(seqs, pages).int()
+    at = torch.arange(t, device=DEV)
+    seq, pos = (at % seqs).int(), (at // seqs + page - 3).int()
+    pos[at % 11 == 4] = -1                                  # padding tokens
+    seq[at % 13 == 5] = -7
+    rope = tables(pages * page, rot) if rot else None
+    q_out = torch.full((t, hq * d), 7.0, dtype=torch.bfloat16, device=DEV) if hq else None
+    pkg.kv_append(actx, cache, k, v, pos, table, seq=seq, rope=(*rope, off) if rot else None, rope_half=half, q=q if hq else None, q_out=q_out)
+    torch.cuda.synchronize()
+    assert actx.status().code == 0
+    live = (pos >= 0) & (seq >= 0)
+    p, s = pos[live].long(), seq[live].long()
+    cs = [x[p] for x in rope] if rot else [torch.zeros(len(p), 0, device=DEV)] * 2
+    page_id = table[s, p // page].long()
+    if hq:
+        want = turned64(q[live].reshape(-1, hq, d), *cs, off, half)
+        size = torch.full_like(want, 0.0)
+        # fp32 rotation: three roundings of 2^-24 of the two products' magnitudes
+        size += q[live].double().abs().reshape(-1, hq, d).amax(-1, keepdim=True) * 2
+        within(q_out[live].reshape(-1, hq, d), want, size, terms=2 ** -22)
+        assert (q_out[~live] == 7.0).all()
+    for x, before, new, turn, scale in ((cache.k, k_before, k, True, cache.k_scale), (cache.v, v_before, v, False, cache.v_scale)):
+        want = new[live].reshape(-1, hkv, d).double()
+        size = new[live].double().abs().reshape(-1, hkv, d).amax(-1, keepdim=True).expand_as(want) * 2
+        want = turned64(new[live].reshape(-1, hkv, d), *cs, off, half) if turn else want
+        got = x[page_id, :, p % page]
+        if fp8:
+            s = scale.double()[:, None] if scale is not None else 1.0
+            got = got.view(torch.float8_e4m3fn)
+            # half a step of e4m3: 2^-4 relative, 2^-10 below its normal range; the fp32 value before it is off by 2^-22
+            within(got, (want / s).clamp(-448, 448), size / s + 2 ** -10 * 2 ** 22, rel=2 ** -4 * 1.0001, terms=2 ** -22)
+        else:
+            within(got, want, size, terms=2 ** -22)
+        touched = torch.zeros(x.shape[0], page, dtype=torch.bool, device=DEV)
+        touched[page_id, p % page] = True
+        same = (x.view(torch.uint8) == before.view(torch.uint8)).reshape(x.shape[0], hkv, page, -1).all(-1).all(1)
+        assert same[~touched].all()                         # nothing else of the cache is written
+
+
+@gpu
+def test_append_in_place_and_bad_indexes(pkg, actx):
+    g = gen(3)
+    d, hq, hkv, page = 128, 4, 2, 16
+    cache = make_cache(pkg, actx, g, 6, hkv, page, d, False)
+    q, k, v = bf16(g, 4, hq * d), bf16(g, 4, hkv * d), bf16(g, 4, hkv * d)
+    cos, sin = tables(40, 128)
+    table = torch.tensor([[0, 1], [2, 99], [3, -1]], dtype=torch.int32, device=DEV)
+    for half in (False, True):
+        fresh = pkg.kv_append(actx, cache, k, v, torch.tensor([0, 1, 2, 3], dtype=torch.int32, device=DEV), table,
+                              seq=torch.tensor([0, 1, 2, 0], dtype=torch.int32, device=DEV), rope=(cos, sin, 0), rope_half=half, q=q)
+        again = q.clone()
+        pkg.kv_append(actx, cache, k, v, torch.tensor([0, 1, 2, 3], dtype=torch.int32, device=DEV), table,
+                      seq=torch.tensor([0, 1, 2, 0], dtype=torch.int32, device=DEV), rope=(cos, sin, 0), rope_half=half, q=again, q_out=again)
+        assert torch.equal(fresh, again)
+    assert actx.status().code == 0
+    before = cache.k.clone()
+    # a page beyond the cache, a negative page, a sequence and a position beyond the table: each alone is reported and skipped
+    for seq, pos in ((1, 17), (2, 16), (3, 0), (0, 32)):
+        pkg.kv_append(actx, cache, k[:1], v[:1], torch.tensor([pos], dtype=torch.int32, device=DEV), table,
+                      seq=torch.tensor([seq], dtype=torch.int32, device=DEV), rope=(cos, sin, 0))
+        with pytest.raises(pkg.DsufError, match="status 2 from kernel 7"):
+            actx.status()
+    short = (cos[:10].contiguous(), sin[:10].contiguous(), 0)
+    pkg.kv_append(actx, cache, k[:1], v[:1], torch.tensor([12], dtype=torch.int32, device=DEV), table, rope=short)
+    with pytest.raises(pkg.DsufError):
+        actx.status()
+    assert torch.equal(before, cache.k) and actx.status().code == 0
+
+
+# ------------------------------------------------------------------ decode
+def decode64(cache, q, table, lens, window, scale, with_size=False):
+    b, hq, d = q.shape[0], q.shape[1] // cache.head_dim, cache.head_dim
+    k, v = cache64(cache)
+    out = torch.zeros(b, hq, d, dtype=torch.float64, device=DEV)
+    size = torch.zeros_like(out)
+    lse = torch.full((b, hq), -math.inf, dtype=torch.float64, device=DEV)
+    g = hq // cache.kv_heads
+    for i, n in enumerate(lens):
+        lo = max(0, n - window) if window else 0
+        if n <= 0:
+            continue
+        pg = table[i, : -(-n // cache.page_size)].long()
+        for h in range(hq):
+            kk, vv = (x[pg, h // g].reshape(-1, d)[lo:n] for x in (k, v))
+            s = (kk @ q[i].double().reshape(hq, d)[h]) * scale
+            lse[i, h] = torch.logsumexp(s, 0)
+            p = torch.softmax(s, 0)
+            out[i, h], size[i, h] = p @ vv, p @ vv.abs()
+    return out.reshape(b, -1), lse, size.reshape(b, -1)
+
+
+def decode_inputs(pkg, ctx, seed, lens, hq, hkv, d, page, fp8, poison=False):
+    g = gen(seed)
+    per = [max(1, -(-n // page)) for n in lens]
+    cache = make_cache(pkg, ctx, g, sum(per) + 3, hkv, page, d, fp8)
+    order = torch.randperm(sum(per) + 3, generator=g, device=DEV).int()
+    table = torch.full((len(lens), max(per) + 1), -1, dtype=torch.int32, device=DEV)   # behind a sequence: no page at all
+    if poison:   # every slot that no sequence sees holds NaN
+        nan = 0x7f if fp8 else 0x7fc0
+        seen = torch.zeros(sum(per) + 3, page, dtype=torch.bool, device=DEV)
+    e = 0
+    for i, n in enumerate(per):
+        table[i, :n] = order[e: e + n]
+        if poison:
+            for j in range(lens[i]):
+                seen[order[e + j // page].long(), j % page] = True
+        e += n
+    if poison:
+        for x in (cache.k, cache.v):
+            raw = x if fp8 else x.view(torch.int16)
+            raw[~seen[:, None, :, None].expand_as(x)] = nan
+    q = bf16(g, len(lens), hq * d + 16, std=1.5)[:, : hq * d]
+    return cache, q, table, torch.tensor(lens, dtype=torch.int32, device=DEV)
+
+
+@gpu
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (7, 1), (16, 2), (12, 1), (34, 2), (8, 8)])
+@pytest.mark.parametrize("lens,page,window", [([1], 16, 0), ([0, 5, 16, 17, 0, 64, 65, 300], 16, 0), ([1000, 1, 129], 32, 128), ([3001], 64, 0),
+                                              ([40, 500, 31], 128, 33), ([700, 2], 16, 1)])
+def test_decode(pkg, actx, fp8, d, hq, hkv, lens, page, window):
+    cache, q, table, n = decode_inputs(pkg, actx, 5 + len(lens) + hq, lens, hq, hkv, d, page, fp8, poison=True)
+    out, lse = pkg.attn_decode(actx, cache, q, table, n, window=window, return_lse=True)
+    torch.cuda.synchronize()
+    assert actx.status().code == 0
+    if fp8:   # (the 64-bit form multiplies what no sequence sees by nothing, but must not meet NaN in the pages it reads)
+        for x in (cache.k, cache.v):
+            x[x == 0x7f] = 0
+    else:
+        for x in (cache.k, cache.v):
+            x.nan_to_num_(0)
+    want, wl, size = decode64(cache, q, table, lens, window, d ** -0.5)
+    within(out, want, size, terms=2 ** -8 + 2 ** -12)
+    live = wl > -math.inf
+    assert torch.equal(live, lse > -math.inf)
+    assert ((lse.double() - wl)[live].abs() <= 2 ** -12 + 2 ** -22 * wl[live].abs()).all()
+    again = pkg.attn_decode(actx, cache, q, table, n, window=window)
+    assert torch.equal(out, again)                          # the join's order does not depend on timing
