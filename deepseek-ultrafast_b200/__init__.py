@@ -147,6 +147,9 @@ ABI = {
     "dsuf_attn_workspace_init": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_size_t]),
     "dsuf_attn_decode": (C.c_int32, [C.c_void_p, C.c_void_p, C.POINTER(KvCacheStruct), C.c_uint64, C.c_int32, C.c_int32, C.c_int32, C.c_uint64,
                                      C.c_int32, C.c_uint64, C.c_float, C.c_int32, C.c_uint64, C.c_int32, C.c_uint64, C.c_uint64]),
+    "dsuf_attn_prompt": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_int32, C.c_uint64, C.c_int32, C.c_uint64, C.c_int32, C.c_int32,
+                                     C.c_int32, C.c_int32, C.c_int32, C.c_uint64, C.c_int32, C.c_float, C.c_int32, C.c_uint64, C.c_int32,
+                                     C.c_uint64]),
 }
 
 
@@ -720,6 +723,34 @@ def attn_decode(ctx, cache, q, block_table, seq_lens, scale=None, window=0, out=
     ctx.check(lib().dsuf_attn_decode(ctx.h, ctx.stream(), C.byref(cache.c), q.data_ptr(), _ld(q), width // d, b, block_table.data_ptr(),
                                      block_table.shape[1], seq_lens.data_ptr(), d ** -0.5 if scale is None else scale, window, out.data_ptr(), _ld(out),
                                      lse.data_ptr() if lse is not None else 0, workspace.data_ptr()))
+    return (out, lse) if return_lse else out
+
+
+def attn_prompt(ctx, q, k, v, cu_seqlens, head_dim=128, scale=None, window=0, out=None, lse=None, return_lse=False):
+    """dsuf_attn_prompt: causal attention over packed prompts, q bf16 [t][q_heads * head_dim], k / v bf16 [t][kv_heads * head_dim] (their
+    rows may be parts of a merged projection's), ``cu_seqlens`` i32 [sequences + 1]; ``window`` > 0: a row sees that many rows, itself
+    included.  ``scale`` None: head_dim ** -0.5.  Rows behind the last sequence are not written.  Returns out bf16
+    [t][q_heads * head_dim], or (out, lse f32 [t][q_heads]) with ``return_lse``."""
+    t = ctx.torch
+    _need_tensor(ctx, "attn_prompt: q", q, t.bfloat16, (None, None), rows=True)
+    n, width = q.shape
+    _need_tensor(ctx, "attn_prompt: k", k, t.bfloat16, (n, None), rows=True)
+    _need_tensor(ctx, "attn_prompt: v", v, t.bfloat16, k.shape, rows=True)
+    _need(head_dim in (64, 128) and width % head_dim == 0 and k.shape[1] % head_dim == 0, "attn_prompt: head_dim is 64 or 128 and rows hold whole heads")
+    _need_tensor(ctx, "attn_prompt: cu_seqlens", cu_seqlens, t.int32, (None,))
+    _need(cu_seqlens.shape[0] >= 1, "attn_prompt: cu_seqlens holds at least one entry")
+    if out is None:
+        out = t.empty((n, width), dtype=t.bfloat16, device=ctx.device)
+    else:
+        _need_tensor(ctx, "attn_prompt: out", out, t.bfloat16, (n, width), rows=True)
+    if lse is not None:
+        _need_tensor(ctx, "attn_prompt: lse", lse, t.float32, (n, width // head_dim))
+    elif return_lse:
+        lse = t.empty((n, width // head_dim), dtype=t.float32, device=ctx.device)
+    ctx.check(lib().dsuf_attn_prompt(ctx.h, ctx.stream(), q.data_ptr(), _ld(q), k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), n, width // head_dim,
+                                     k.shape[1] // head_dim, head_dim, cu_seqlens.data_ptr(), cu_seqlens.shape[0] - 1,
+                                     head_dim ** -0.5 if scale is None else scale, window, out.data_ptr(), _ld(out),
+                                     lse.data_ptr() if lse is not None else 0))
     return (out, lse) if return_lse else out
 
 

@@ -1,0 +1,498 @@
+// Causal attention over packed prompts (dsuf_attn_prompt): grouped heads, ragged lengths, sliding window, bf16.
+//
+// out_i = sum_{j <= i} exp(scale <q_i, k_j> - top_i) v_j / sum: 4 D flops per visible pair against 2 D (2 hq + 2 hkv) bytes per
+// token, so it is bound by the tensor cores and, as tightly, by the exponential unit (a 128 x 128 tile of scores costs 2 x 512 tensor
+// cycles at D = 128 and 1024 cycles of 16 exponentials per clock and SM).
+//
+// One persistent CTA per SM works on two 128-row query tiles at a time that share their keys and values; the tiles of a (sequence,
+// kv head) are numbered block * group + head-in-group and paired in that order, so a pair is almost always two heads of the same block
+// and has one causal boundary (an odd group pairs the last head of a block with the first of the next).  Roles:
+//   warps 0-3, 4-7   softmax of tile 0 / 1: a thread owns a row; scores from tensor memory, p back to tensor memory
+//   warp 8           TMA: query tiles, and a ring of key / value tiles (K0 V0 K1 V1 ...)
+//   warp 9           tcgen05.mma: S_t = Q_t K^T (operands in shared memory), O_t += P_t V (P in tensor memory, V as it lies,
+//                    tokens by columns, through the MN-major operand form)
+// The issue order P0 V, S0, P1 V, S1 keeps the tensor core on one tile while the other tile's softmax runs; S of step j + 1 is issued
+// behind PV of step j, so its completion also says that the output may be rescaled.  The steps of successive pairs form one stream: the
+// next pair's first scores are issued before the last output is stored.
+//
+// Tensor memory (512 columns): S0 S1 (128 fp32 columns each; P_t overwrites the first 64 of S_t as packed bf16), O0 O1 (D each).
+// The reference point of a row only moves when a score exceeds it by 2^8 (exact: the sum and the output share it), which makes
+// rescaling rare after the first tile.  p is rounded once to bf16 as operand; sums, statistics and outputs are fp32.
+//
+// Pairs are ordered from the longest rows to the shortest inside a sequence and dealt to the CTAs back and forth, so that a CTA's
+// long and short pairs balance.  Values behind a sequence's end inside its last tile belong to another sequence (or nobody) and are
+// zeroed in shared memory before use: p is 0 there, but 0 x NaN is not.
+#include "internal.h"
+
+namespace dsuf {
+
+constexpr int KID_PROMPT = 9;
+constexpr int PA_THREADS = 320;
+constexpr int PA_BM = 128;
+constexpr float PA_UNSET = -1e30f;
+constexpr float PA_TRIGGER = 8.f;
+
+template <int D>
+struct PromptShape {
+    static constexpr int BOXES = D / 64;                       // 128-byte wide operand boxes of a tile
+    static constexpr int TILE = PA_BM * D * 2;                 // bytes of a query, key or value tile
+    static constexpr int STAGES = D == 128 ? 5 : 8;            // ring of key / value tiles
+    static constexpr int SMEM = 2 * TILE + STAGES * TILE + 1024;
+};
+
+struct PromptArgs {
+    CUtensorMap tm_q, tm_k, tm_v;
+    bf16* out;
+    float* lse;
+    int ldo, t, q_heads, kv_heads, group, n_seqs, window;
+    const int* cu;
+    float scale_log2;
+    DevStatus* status;
+};
+
+// kind::f16, fp32 accumulator, bf16 operands, M = 128; bit 16: B is MN-major.
+DSUF_DEV constexpr uint32_t pa_idesc(int n, bool b_mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n / 8) << 17) | ((uint32_t)(128 / 16) << 24);
+}
+DSUF_DEV void pa_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        "  .reg .pred keep_d;\n"
+        "  setp.ne.u32 keep_d, %4, 0;\n"
+        "  tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, keep_d;\n"
+        "}\n"
+        :
+        : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+DSUF_DEV void pa_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        "  .reg .pred keep_d;\n"
+        "  setp.ne.u32 keep_d, %4, 0;\n"
+        "  tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, keep_d;\n"
+        "}\n"
+        :
+        : "r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+#define PA_R4(v, i) "r"(v[i]), "r"(v[(i) + 1]), "r"(v[(i) + 2]), "r"(v[(i) + 3])
+#define PA_R16(v, i) PA_R4(v, i), PA_R4(v, (i) + 4), PA_R4(v, (i) + 8), PA_R4(v, (i) + 12)
+DSUF_DEV void tmem_st16(uint32_t taddr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+        :
+        : PA_R16(v, 0), "r"(taddr)
+        : "memory");
+}
+DSUF_DEV void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" : : : "memory"); }
+DSUF_DEV float pa_exp2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+DSUF_DEV uint32_t pa_pack(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// A pair of query tiles: tile t covers rows [qb[t] * 128, ..) of the sequence, query head head[t], key tiles [lo[t], hi[t]).
+struct PromptPair {
+    int start, len, kvh;
+    int qb[2], head[2], lo[2], hi[2];
+    int jlo, jhi;
+    bool ok;
+    DSUF_DEV bool active(int t, int j) const { return j >= lo[t] && j < hi[t]; }
+};
+
+// Walks the pairs of one CTA: row r of the deal takes index r * grid + c, or counted from the other end in odd rows.  A whole warp calls
+// next() together: its lanes look at 32 sequences at a time.
+struct PromptWalk {
+    const PromptArgs& a;
+    int row = 0, seq = 0;        // seq: first of the 32 sequences looked at
+    long long before = 0;        // pairs of the sequences below it
+    DSUF_DEV explicit PromptWalk(const PromptArgs& a_) : a(a_) {}
+    DSUF_DEV void bounds(int s, int& start, int& len) const {
+        start = len = 0;
+        if (s < a.n_seqs) {
+            start = min(max(__ldg(a.cu + s), 0), a.t);
+            len = max(min(max(__ldg(a.cu + s + 1), 0), a.t) - start, 0);
+        }
+    }
+    DSUF_DEV PromptPair next() {
+        const int lane = threadIdx.x & 31;
+        PromptPair p;
+        p.ok = false;
+        const long long x = (long long)row * gridDim.x + ((row & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        ++row;
+        for (; seq < a.n_seqs; seq += 32) {
+            int start, len;
+            bounds(seq + lane, start, len);
+            const long long mine = (long long)((((len + PA_BM - 1) / PA_BM) * a.group + 1) / 2) * a.kv_heads;
+            long long upto = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, before + upto > x);
+            if (past) {
+                const int owner = __ffs(past) - 1;
+                p.start = __shfl_sync(0xffffffffu, start, owner);
+                p.len = __shfl_sync(0xffffffffu, len, owner);
+                const int local = (int)(x - before - __shfl_sync(0xffffffffu, upto - mine, owner));
+                const int tiles = ((p.len + PA_BM - 1) / PA_BM) * a.group;
+                const int rank = local / a.kv_heads;
+                p.kvh = local % a.kv_heads;
+                const int pair = (tiles + 1) / 2 - 1 - rank;
+                p.jlo = 0x7fffffff;
+                p.jhi = 0;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int it = 2 * pair + t;
+                    p.qb[t] = it / a.group;
+                    p.head[t] = p.kvh * a.group + it % a.group;
+                    p.lo[t] = p.hi[t] = 0;
+                    if (it < tiles) {
+                        p.hi[t] = p.qb[t] + 1;
+                        p.lo[t] = a.window > 0 ? max(0, p.qb[t] * PA_BM - a.window + 1) / PA_BM : 0;
+                        p.jlo = min(p.jlo, p.lo[t]);
+                        p.jhi = max(p.jhi, p.hi[t]);
+                    }
+                }
+                p.ok = true;
+                return p;
+            }
+            before += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        return p;
+    }
+};
+
+template <int D>
+__global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid_constant__ PromptArgs a) {
+    using S = PromptShape<D>;
+    constexpr int BOX = PA_BM * 128;                 // bytes of one box
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t* ring = base + 2 * S::TILE;
+    __shared__ __align__(8) uint64_t q_full[2], q_empty[2], kv_full[S::STAGES], kv_empty[S::STAGES], s_full[2], p_full[2], o_full[2];
+    __shared__ uint32_t s_tmem;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    bool dead = false;
+
+    if (warp == 9) {
+        tmem_alloc(&s_tmem, 512);
+        tmem_relinquish();
+    }
+    if (tid == 0) {
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&q_full[t], 1);
+            mbar_init(&q_empty[t], 1);
+            mbar_init(&s_full[t], 1);
+            mbar_init(&p_full[t], 4);
+            mbar_init(&o_full[t], 1);
+        }
+        for (int s = 0; s < S::STAGES; ++s) {
+            mbar_init(&kv_full[s], 1);
+            mbar_init(&kv_empty[s], 1);
+        }
+        mbar_fence_init();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tm = s_tmem;
+    pdl_wait();
+    pdl_launch_dependents();
+    PromptWalk walk(a);
+
+    if (warp == 8) {
+        // ---------------- producer ----------------
+        if (lane == 0) {
+            prefetch_tmap(&a.tm_q);
+            prefetch_tmap(&a.tm_k);
+            prefetch_tmap(&a.tm_v);
+        }
+        int st = 0;
+        uint32_t ph = 0, qn[2] = {0, 0};
+        long long n = 0;
+        auto kv = [&](const PromptPair& p, const CUtensorMap* map, int j) {
+            if (n >= S::STAGES && !dead && !mbar_wait(&kv_empty[st], ph ^ 1, a.status, KID_PROMPT, 1)) dead = true;
+            if (warp_elect()) {
+                mbar_expect_tx(&kv_full[st], S::TILE);
+#pragma unroll
+                for (int b = 0; b < S::BOXES; ++b)
+                    tma_2d_nh(ring + st * S::TILE + b * BOX, map, p.kvh * D + b * 64, p.start + j * PA_BM, &kv_full[st]);
+            }
+            __syncwarp();
+            ++n;
+            if (++st == S::STAGES) { st = 0; ph ^= 1; }
+        };
+        for (;;) {
+            const PromptPair p = walk.next();
+            if (!p.ok) break;
+            kv(p, &a.tm_k, p.jlo);   // ahead of the queries: their buffers become free later than the ring's
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                if (p.hi[t] == 0) continue;
+                if (qn[t] > 0 && !dead && !mbar_wait(&q_empty[t], (qn[t] - 1) & 1, a.status, KID_PROMPT, 2)) dead = true;
+                if (warp_elect()) {
+                    mbar_expect_tx(&q_full[t], S::TILE);
+#pragma unroll
+                    for (int b = 0; b < S::BOXES; ++b)
+                        tma_2d_nh(base + t * S::TILE + b * BOX, &a.tm_q, p.head[t] * D + b * 64, p.start + p.qb[t] * PA_BM, &q_full[t]);
+                }
+                __syncwarp();
+                ++qn[t];
+            }
+            for (int j = p.jlo; j < p.jhi; ++j) {
+                if (j > p.jlo) kv(p, &a.tm_k, j);
+                kv(p, &a.tm_v, j);
+            }
+        }
+    } else if (warp == 9) {
+        // ---------------- tensor core issuer ----------------
+        const uint32_t tmu = warp_uniform(tm);
+        const uint64_t qd0 = warp_uniform(tc_smem_desc(base, 16, 1024, TC_SWIZZLE_128B));
+        const uint64_t kd0 = warp_uniform(tc_smem_desc(ring, 16, 1024, TC_SWIZZLE_128B));
+        const uint64_t vd0 = warp_uniform(tc_smem_desc(ring, BOX, 1024, TC_SWIZZLE_128B));   // column chunks of 64 a box apart, 8 tokens 1024 bytes
+        int st = 0;
+        uint32_t ph = 0, qn[2] = {0, 0}, pn[2] = {0, 0};
+        auto wait_kv = [&]() {
+            if (!dead && !mbar_wait(&kv_full[st], ph, a.status, KID_PROMPT, 3)) dead = true;
+            tc_fence_after();
+        };
+        auto release_kv = [&](int stage) {
+            if (warp_elect()) tc_commit(&kv_empty[stage]);
+            __syncwarp();
+        };
+        auto advance = [&]() {
+            if (++st == S::STAGES) { st = 0; ph ^= 1; }
+        };
+        auto scores = [&](const PromptPair& p, int t, int j, int stage) {
+            if (j == p.lo[t]) {
+                if (!dead && !mbar_wait(&q_full[t], qn[t] & 1, a.status, KID_PROMPT, 4)) dead = true;
+                ++qn[t];
+                tc_fence_after();
+            }
+            if (warp_elect()) {
+#pragma unroll
+                for (int c = 0; c < D / 16; ++c) {
+                    const uint32_t off = (uint32_t)((c >> 2) * BOX + (c & 3) * 32) >> 4;
+                    pa_mma_ss(tmu + t * 128, qd0 + (uint64_t)((t * S::TILE) >> 4) + off, kd0 + (uint64_t)((stage * S::TILE) >> 4) + off, pa_idesc(128, false), c != 0);
+                }
+                tc_commit(&s_full[t]);
+                if (j == p.hi[t] - 1) tc_commit(&q_empty[t]);
+            }
+            __syncwarp();
+        };
+        PromptPair cur = walk.next();
+        if (cur.ok) {
+            wait_kv();
+            for (int t = 0; t < 2; ++t)
+                if (cur.active(t, cur.jlo)) scores(cur, t, cur.jlo, st);
+            release_kv(st);
+            advance();
+        }
+        while (cur.ok) {
+            PromptPair nxt = cur;
+            for (int j = cur.jlo; j < cur.jhi; ++j) {
+                const bool last = j + 1 == cur.jhi;
+                if (last) nxt = walk.next();
+                const bool more = nxt.ok;
+                const int nj = last ? nxt.jlo : j + 1;
+                wait_kv();
+                const int vst = st;
+                advance();
+                const int behind = cur.len - j * PA_BM;      // rows of this tile inside the sequence
+                if (behind < PA_BM) {
+                    for (int i = lane; i < (PA_BM - behind) * 8 * S::BOXES; i += 32) {
+                        const int b = i / ((PA_BM - behind) * 8), r = i % ((PA_BM - behind) * 8);
+                        *reinterpret_cast<uint4*>(ring + vst * S::TILE + b * BOX + behind * 128 + r * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async();
+                    __syncwarp();
+                }
+                bool k_here = false;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (cur.active(t, j)) {
+                        if (!dead && !mbar_wait(&p_full[t], pn[t] & 1, a.status, KID_PROMPT, 5)) dead = true;
+                        ++pn[t];
+                        tc_fence_after();
+                        if (warp_elect()) {
+#pragma unroll
+                            for (int c = 0; c < PA_BM / 16; ++c)
+                                pa_mma_ts(tmu + 256 + t * D, tmu + t * 128 + c * 8, vd0 + (uint64_t)((vst * S::TILE + c * 2048) >> 4), pa_idesc(D, true),
+                                          j > cur.lo[t] || c != 0);
+                            if (j == cur.hi[t] - 1) tc_commit(&o_full[t]);
+                        }
+                        __syncwarp();
+                    }
+                    if (more && nxt.active(t, nj)) {
+                        if (!k_here) wait_kv();
+                        k_here = true;
+                        scores(nxt, t, nj, st);
+                    }
+                }
+                release_kv(vst);
+                if (more) {
+                    release_kv(st);
+                    advance();
+                }
+            }
+            cur = nxt;
+        }
+    } else {
+        // ---------------- softmax: tile t, one row per thread ----------------
+        const int t = warp >> 2;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t tS = tm + lanes + t * 128, tO = tm + lanes + 256 + t * D;
+        const int r = (warp & 3) * 32 + lane;        // row inside the tile
+        const float sl2 = a.scale_log2;
+        uint32_t sn = 0, on = 0;
+        for (;;) {
+            const PromptPair p = walk.next();
+            if (!p.ok) break;
+            if (p.hi[t] == 0) continue;
+            const int row = p.qb[t] * PA_BM + r;
+            float ref = PA_UNSET, sum = 0.f;
+            for (int j = p.lo[t]; j < p.hi[t]; ++j) {
+                if (!dead && !mbar_wait(&s_full[t], sn & 1, a.status, KID_PROMPT, 6)) dead = true;
+                ++sn;
+                tc_fence_after();
+                float s[128];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld_issue<32>(tS + c * 32, s + c * 32);
+                tmem_wait_ld();
+                const int upper = row - j * PA_BM;                                  // last visible column of the tile
+                const int lower = a.window > 0 ? upper - a.window : -1;             // last column hidden by the window
+                if (j == p.hi[t] - 1 || (a.window > 0 && p.qb[t] * PA_BM + PA_BM - 1 - j * PA_BM >= a.window)) {
+#pragma unroll
+                    for (int c = 0; c < 128; ++c) s[c] = c <= upper && c > lower ? s[c] * sl2 : -INFINITY;
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 128; c += 2) mul_f32x2(s[c], s[c + 1], sl2, sl2);
+                }
+                float top = fmaxf(s[0], s[1]);
+#pragma unroll
+                for (int c = 2; c < 128; c += 2) top = fmaxf(top, fmaxf(s[c], s[c + 1]));
+                const bool over = top > ref + PA_TRIGGER;
+                if (__any_sync(0xffffffffu, over)) {
+                    const float to = over ? top : ref;
+                    const float by = pa_exp2(ref - to);
+                    ref = to;
+                    sum *= by;
+                    if (j > p.lo[t]) {   // (this step's scores were issued behind the last step's product: the output is complete)
+#pragma unroll
+                        for (int c = 0; c < D; c += 16) {
+                            float o[16];
+                            tmem_ld<16>(tO + c, o);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[e] *= by;
+                            tmem_st16(tO + c, reinterpret_cast<const uint32_t*>(o));
+                        }
+                    }
+                }
+                float part[2] = {0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float x = pa_exp2(s[c * 32 + 2 * e] - ref), y = pa_exp2(s[c * 32 + 2 * e + 1] - ref);
+                        part[0] += x;
+                        part[1] += y;
+                        w[e] = pa_pack(x, y);
+                    }
+                    tmem_st16(tS + c * 16, w);
+                }
+                sum += part[0] + part[1];
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[t]);
+            }
+            if (!dead && !mbar_wait(&o_full[t], on & 1, a.status, KID_PROMPT, 7)) dead = true;
+            ++on;
+            tc_fence_after();
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            const bool live = row < p.len;
+            bf16* dst = a.out + (size_t)(p.start + row) * a.ldo + (size_t)p.head[t] * D;
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+                float o[32];
+                tmem_ld<32>(tO + c, o);
+                if (live) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8)
+                        *reinterpret_cast<uint4*>(dst + c + e) = make_uint4(pa_pack(o[e] * inv, o[e + 1] * inv), pa_pack(o[e + 2] * inv, o[e + 3] * inv),
+                                                                            pa_pack(o[e + 4] * inv, o[e + 5] * inv), pa_pack(o[e + 6] * inv, o[e + 7] * inv));
+                }
+            }
+            if (live && a.lse) a.lse[(size_t)(p.start + row) * a.q_heads + p.head[t]] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
+            tc_fence_before();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 9) tmem_dealloc(tm, 512);
+}
+
+static int encode_heads(dsuf_ctx* ctx, CUtensorMap* tm, const void* base, long long width, long long ld, long long rows) {
+    cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+    cuuint32_t box[2] = {64u, (cuuint32_t)PA_BM};
+    cuuint32_t es[2] = {1u, 1u};
+    CUresult r = ctx->encode_tiled(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(ctx, DSUF_E_BADARG, "cuTensorMapEncodeTiled(attention) failed: %d", (int)r);
+    return DSUF_OK;
+}
+
+int attn_prompt_setup(dsuf_ctx* ctx) {
+    cudaError_t e = cudaFuncSetAttribute(attn_prompt_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<64>::SMEM);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(attn_prompt_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<128>::SMEM);
+    return e == cudaSuccess ? DSUF_OK : cuda_fail(ctx, e, "cudaFuncSetAttribute(attn_prompt)");
+}
+
+}  // namespace dsuf
+
+using namespace dsuf;
+
+extern "C" int32_t dsuf_attn_prompt(dsuf_ctx* ctx, void* stream, uint64_t q, int32_t ldq, uint64_t k, int32_t ldk, uint64_t v, int32_t ldv, int32_t t,
+                                    int32_t q_heads, int32_t kv_heads, int32_t head_dim, uint64_t cu_seqlens, int32_t n_seqs, float scale,
+                                    int32_t window, uint64_t out, int32_t ldo, uint64_t lse) {
+    if (!ctx) return DSUF_E_BADARG;
+    DSUF_REQUIRE(ctx, head_dim == 64 || head_dim == 128, "attn_prompt: head_dim (%d) must be 64 or 128", head_dim);
+    DSUF_REQUIRE(ctx, kv_heads >= 1 && q_heads >= 1 && q_heads <= 4096 && q_heads % kv_heads == 0,
+                 "attn_prompt: q_heads (%d) must be a multiple of kv_heads (%d), at most 4096", q_heads, kv_heads);
+    DSUF_REQUIRE(ctx, t >= 0 && t <= 0x7fff0000 && n_seqs >= 0, "attn_prompt: t must be in 0..2^31 - 65536 and n_seqs >= 0");
+    DSUF_REQUIRE(ctx, ldq >= q_heads * head_dim && ldq % 8 == 0 && ldo >= q_heads * head_dim && ldo % 8 == 0 && ldk >= kv_heads * head_dim && ldk % 8 == 0 &&
+                 ldv >= kv_heads * head_dim && ldv % 8 == 0, "attn_prompt: row strides must be multiples of 8 and hold all heads");
+    DSUF_REQUIRE(ctx, window >= 0 && scale == scale && scale - scale == 0.f, "attn_prompt: window must be >= 0 and scale finite");
+    if (t == 0 || n_seqs == 0) return DSUF_OK;
+    DSUF_REQUIRE(ctx, q && k && v && out && cu_seqlens && (q & 15) == 0 && (k & 15) == 0 && (v & 15) == 0 && (out & 15) == 0 && (cu_seqlens & 3) == 0 &&
+                 (lse & 3) == 0, "attn_prompt: null or misaligned pointer (q, k, v, out 16 bytes, cu_seqlens and lse 4)");
+    PromptArgs a;
+    memset(&a, 0, sizeof(a));
+    int rc = encode_heads(ctx, &a.tm_q, (const void*)q, (long long)q_heads * head_dim, ldq, t);
+    if (!rc) rc = encode_heads(ctx, &a.tm_k, (const void*)k, (long long)kv_heads * head_dim, ldk, t);
+    if (!rc) rc = encode_heads(ctx, &a.tm_v, (const void*)v, (long long)kv_heads * head_dim, ldv, t);
+    if (rc) return rc;
+    a.out = (bf16*)out; a.lse = (float*)lse; a.ldo = ldo; a.t = t;
+    a.q_heads = q_heads; a.kv_heads = kv_heads; a.group = q_heads / kv_heads; a.n_seqs = n_seqs; a.window = window;
+    a.cu = (const int*)cu_seqlens;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.status = ctx->dev_status;
+    // no more CTAs than pairs there can be (the lengths are only known on the device)
+    const long long blocks = (long long)(t / PA_BM) + (t < n_seqs ? t : n_seqs);
+    const long long cap = (blocks * a.group + 1) * kv_heads;
+    const int grid = (int)(cap < ctx->sm_count ? cap : ctx->sm_count);
+    if (head_dim == 64) return launch(ctx, (cudaStream_t)stream, attn_prompt_kernel<64>, dim3(grid), dim3(PA_THREADS), (size_t)PromptShape<64>::SMEM, a);
+    return launch(ctx, (cudaStream_t)stream, attn_prompt_kernel<128>, dim3(grid), dim3(PA_THREADS), (size_t)PromptShape<128>::SMEM, a);
+}

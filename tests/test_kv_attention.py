@@ -223,3 +223,52 @@ def test_decode(pkg, actx, fp8, d, hq, hkv, lens, page, window):
     assert ((lse.double() - wl)[live].abs() <= 2 ** -12 + 2 ** -22 * wl[live].abs()).all()
     again = pkg.attn_decode(actx, cache, q, table, n, window=window)
     assert torch.equal(out, again)                          # the join's order does not depend on timing
+
+
+# ------------------------------------------------------------------ prompt
+def prompt64(q, k, v, lens, hq, hkv, d, window, scale):
+    t = q.shape[0]
+    q, k, v = (x.double().reshape(t, -1, d) for x in (q, k, v))
+    out = torch.zeros(t, hq, d, dtype=torch.float64, device=DEV)
+    size = torch.zeros_like(out)
+    lse = torch.zeros(t, hq, dtype=torch.float64, device=DEV)
+    b = 0
+    for n in lens:
+        i = torch.arange(n, device=DEV)
+        hidden = i[None, :] > i[:, None]
+        if window:
+            hidden |= i[None, :] <= i[:, None] - window
+        for h in range(hq if n else 0):
+            s = (q[b: b + n, h] @ k[b: b + n, h // (hq // hkv)].T * scale).masked_fill(hidden, -math.inf)
+            p = torch.softmax(s, 1)
+            lse[b: b + n, h] = torch.logsumexp(s, 1)
+            out[b: b + n, h] = p @ v[b: b + n, h // (hq // hkv)]
+            size[b: b + n, h] = p @ v[b: b + n, h // (hq // hkv)].abs()
+        b += n
+    return out.reshape(t, -1), lse, size.reshape(t, -1)
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (7, 1), (6, 3), (5, 5), (16, 2)])
+@pytest.mark.parametrize("lens,window", [([1], 0), ([128], 0), ([129, 0, 127, 1, 300], 0), ([700], 0), ([1000, 3, 257], 128), ([400, 131], 1), ([900], 333),
+                                         ([5] * 70, 0)])
+def test_prompt(pkg, actx, d, hq, hkv, lens, window):
+    g = gen(sum(lens) + hq + d)
+    t = sum(lens) + 9                                       # rows behind the last sequence
+    rows = bf16(g, t, (hq + 2 * hkv) * d)
+    rows[sum(lens):] = math.nan
+    q, k, v = rows.split([hq * d, hkv * d, hkv * d], 1)
+    cu = torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32, device=DEV)
+    out = torch.full((t, hq * d), 5.0, dtype=torch.bfloat16, device=DEV)
+    lse = torch.full((t, hq), 5.0, device=DEV)
+    pkg.attn_prompt(actx, q, k, v, cu, head_dim=d, window=window, out=out, lse=lse)
+    torch.cuda.synchronize()
+    assert actx.status().code == 0
+    n = sum(lens)
+    assert (out[n:] == 5.0).all() and (lse[n:] == 5.0).all()
+    want, wl, size = prompt64(q[:n], k[:n], v[:n], lens, hq, hkv, d, window, d ** -0.5)
+    within(out[:n], want, size, terms=2 ** -8 + 2 ** -12)
+    assert ((lse[:n].double() - wl).abs() <= 2 ** -12 + 2 ** -22 * wl.abs()).all()
+    again = pkg.attn_prompt(actx, q, k, v, cu, head_dim=d, window=window)
+    assert torch.equal(out[:n], again[:n])
