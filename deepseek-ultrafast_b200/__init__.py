@@ -150,6 +150,8 @@ ABI = {
     "dsuf_attn_prompt": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_int32, C.c_uint64, C.c_int32, C.c_uint64, C.c_int32, C.c_int32,
                                      C.c_int32, C.c_int32, C.c_int32, C.c_uint64, C.c_int32, C.c_float, C.c_int32, C.c_uint64, C.c_int32,
                                      C.c_uint64]),
+    "dsuf_sample": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_int64, C.c_int32, C.c_int32, C.c_uint64, C.c_uint64, C.c_uint64,
+                                C.c_uint64, C.c_uint64, C.c_uint64, C.c_uint64]),
 }
 
 
@@ -752,6 +754,32 @@ def attn_prompt(ctx, q, k, v, cu_seqlens, head_dim=128, scale=None, window=0, ou
                                      head_dim ** -0.5 if scale is None else scale, window, out.data_ptr(), _ld(out),
                                      lse.data_ptr() if lse is not None else 0))
     return (out, lse) if return_lse else out
+
+
+def sample(ctx, logits, u, temperature=None, top_k=None, top_p=None, min_p=None, ids=None, logprobs=None, return_logprobs=False):
+    """dsuf_sample: one token per row of fp32 ``logits`` [m][n] (lm_head's) from the given uniform numbers ``u`` f32 [m] in [0, 1), after
+    temperature, top-k, top-p and min-p (tensors of one value per row; None: off; see include/dsuf_qmm.h for the order and ties).
+    Returns ids i32 [m], or (ids, logprobs f32 [m]) with ``return_logprobs``: the raw log-probabilities of the drawn tokens."""
+    t = ctx.torch
+    _need_tensor(ctx, "sample: logits", logits, t.float32, (None, None), rows=True)
+    m, n = logits.shape
+    _need_tensor(ctx, "sample: u", u, t.float32, (m,))
+    ptrs = []
+    for name, x, dtype in (("temperature", temperature, t.float32), ("top_k", top_k, t.int32), ("top_p", top_p, t.float32), ("min_p", min_p, t.float32)):
+        if x is not None:
+            _need_tensor(ctx, "sample: " + name, x, dtype, (m,))
+        ptrs.append(x.data_ptr() if x is not None else 0)
+    if ids is None:
+        ids = t.empty(m, dtype=t.int32, device=ctx.device)
+    else:
+        _need_tensor(ctx, "sample: ids", ids, t.int32, (m,))
+    if logprobs is not None:
+        _need_tensor(ctx, "sample: logprobs", logprobs, t.float32, (m,))
+    elif return_logprobs:
+        logprobs = t.empty(m, dtype=t.float32, device=ctx.device)
+    ctx.check(lib().dsuf_sample(ctx.h, ctx.stream(), logits.data_ptr(), _ld(logits), m, n, *ptrs, u.data_ptr(), ids.data_ptr(),
+                                logprobs.data_ptr() if logprobs is not None else 0))
+    return (ids, logprobs) if return_logprobs else ids
 
 
 def probe_tensor_rate(ctx, n_cols=128, a_is_e2m1=False, iters=20000, reps=5):

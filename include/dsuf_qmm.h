@@ -445,6 +445,20 @@ int32_t dsuf_attn_prompt(dsuf_ctx* ctx, void* stream, uint64_t q, int32_t ldq, u
                          int32_t q_heads, int32_t kv_heads, int32_t head_dim, uint64_t cu_seqlens, int32_t n_seqs, float scale,
                          int32_t window, uint64_t out, int32_t ldo, uint64_t lse);
 
+/* ---- sampling, the step behind the output head (dsuf_lm_head_bf16): one token per row of fp32 logits [m][ld], n <= 2^22.  The reference's
+ * sampler (crates/kernels/cu/sample.cu) works on the head's records; this entry takes any top_k and top_p.
+ * With M the row's largest logit, w_i = exp((l_i - M) / temperature) and tokens ordered by larger logit, lower id first among equals:
+ *   A = the first top_k tokens (top_k <= 0 or beyond the row: all);
+ *   B = those of A whose preceding weight inside A is below top_p * weight(A) (top_p >= 1: all of A; the first token always);
+ *   C = those of B with w_i >= min_p (above 1 counts as 1);
+ *   ids[row] = the lowest id i of C with weight(C, ids up to i) > u * weight(C), u in [0, 1).
+ * temperature <= 0: the largest logit's lowest id.  NaN and -inf logits are never drawn; a row without any other gives -1.
+ * temperature, top_p, min_p f32 [m], top_k i32 [m] (device), 0: 1, 1, 0 and 0 for every row; u f32 [m]; ids i32 [m];
+ * logprobs f32 [m] or 0: log softmax(logits)[id] of the logits as they are (temperature 1, no limits).  Weights are 2^-40 fixed point and
+ * their sums exact, so equal inputs give equal tokens whatever the batch. */
+int32_t dsuf_sample(dsuf_ctx* ctx, void* stream, uint64_t logits, int64_t ld, int32_t m, int32_t n, uint64_t temperature, uint64_t top_k,
+                    uint64_t top_p, uint64_t min_p, uint64_t u, uint64_t ids_out, uint64_t logprobs_out);
+
 #ifdef __cplusplus
 }
 #endif
