@@ -295,6 +295,7 @@ class Ctx:
         import torch
         self.torch = torch
         self.device = torch.device("cuda", device)
+        self.index = device
         h = C.c_void_p()
         rc = lib().dsuf_ctx_create(device, C.byref(h))
         if rc:
@@ -613,21 +614,37 @@ def _need(cond, msg):
         raise DsufError(-1, msg)
 
 
-def _need_tensor(ctx, name, x, dtype, shape, rows=False):
-    """x is a tensor of this type and shape (None: any size) on the context's device; contiguous, or with ``rows`` a matrix
-    whose rows may lie apart."""
-    _need(isinstance(x, ctx.torch.Tensor) and x.device == ctx.device and x.dtype == dtype,
-          f"{name}: a {dtype} tensor on {ctx.device} is wanted")
-    _need(x.dim() == len(shape) and all(w is None or g == w for g, w in zip(x.shape, shape)), f"{name}: shape {tuple(x.shape)}, wanted {tuple(shape)}")
-    if rows:
-        _need(x.numel() == 0 or (x.stride(1) == 1 and (x.shape[0] < 2 or x.stride(0) >= x.shape[1])), f"{name}: rows must be contiguous and not overlap")
-    else:
-        _need(x.is_contiguous(), f"{name}: must be contiguous")
+def _refuse(ctx, name, x, dtype, shape, rows):
+    if not isinstance(x, ctx.torch.Tensor) or x.device != ctx.device or x.dtype != dtype:
+        raise DsufError(-1, f"{name}: a {dtype} tensor on {ctx.device} is wanted")
+    raise DsufError(-1, f"{name}: shape {tuple(x.shape)} with strides {x.stride()}; wanted {shape}, " +
+                    ("rows contiguous and not overlapping" if rows else "contiguous"))
 
 
-def _ld(x):
-    """Row stride of a matrix; that of a single row is its length, whatever the tensor says."""
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+def _vector(ctx, name, x, dtype, n=None):
+    """x is a contiguous vector (of n elements) of this type on the context's device."""
+    try:
+        ok = x.dtype is dtype and x.get_device() == ctx.index and x.dim() == 1 and (n is None or x.shape[0] == n) and x.is_contiguous()
+    except AttributeError:
+        ok = False
+    if not ok:
+        _refuse(ctx, name, x, dtype, (n,), False)
+
+
+def _rows(ctx, name, x, dtype, n=None, width=None):
+    """x is a matrix [n][width] of this type on the context's device whose rows may lie apart; returns its row stride."""
+    try:
+        if x.dtype is dtype and x.get_device() == ctx.index and x.dim() == 2:
+            m, w = x.shape
+            ld, one = x.stride()
+            if (n is None or m == n) and (width is None or w == width):
+                if m < 2 or w == 0:
+                    ld = w          # (a single row's stride says nothing)
+                if (one == 1 or w < 2 or m == 0) and ld >= w:
+                    return ld
+    except AttributeError:
+        pass
+    _refuse(ctx, name, x, dtype, (n, width), True)
 
 
 class KvCache:
@@ -643,12 +660,13 @@ class KvCache:
             _need(x.stride()[1:] == (p * d, d, 1) and x.stride(0) == k.stride(0), f"KvCache: {name}: the heads of a page must be contiguous, k's and v's pages equally far apart")
         for name, x in (("k_scale", k_scale), ("v_scale", v_scale)):
             if x is not None:
-                _need_tensor(ctx, "KvCache: " + name, x, t.float32, (h,))
+                _vector(ctx, "KvCache: " + name, x, t.float32, h)
         self.ctx, self.k, self.v, self.k_scale, self.v_scale = ctx, k, v, k_scale, v_scale   # (keeps the tensors alive)
         self.n_pages, self.kv_heads, self.page_size, self.head_dim = n, h, p, d
         self.c = KvCacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if k_scale is not None else 0,
                                v_scale.data_ptr() if v_scale is not None else 0, max(k.stride(0), h * p * d) if n > 1 else h * p * d,
                                KV_BF16 if k.dtype == t.bfloat16 else KV_E4M3, n, p, h, d)
+        self.ref = C.byref(self.c)
 
     @staticmethod
     def empty(ctx, n_pages, page_size, kv_heads, head_dim, fp8=False, k_scale=None, v_scale=None):
@@ -657,6 +675,13 @@ class KvCache:
         shape = (n_pages, kv_heads, page_size, head_dim)
         k, v = (t.zeros(shape, dtype=t.uint8 if fp8 else t.bfloat16, device=ctx.device) for _ in range(2))
         return KvCache(ctx, k, v, k_scale, v_scale)
+
+
+def _table(ctx, who, table):
+    """(sequences, pages) of a contiguous block table."""
+    if _rows(ctx, who + ": block_table", table, ctx.torch.int32) != table.shape[1]:
+        raise DsufError(-1, who + ": block_table must be contiguous")
+    return table.shape
 
 
 def kv_append(ctx, cache, k, v, pos, block_table, seq=None, rope=None, rope_half=False, q=None, q_out=None):
@@ -668,32 +693,31 @@ def kv_append(ctx, cache, k, v, pos, block_table, seq=None, rope=None, rope_half
     t = ctx.torch
     _need(cache.ctx is ctx, "kv_append: the cache belongs to another context")
     d = cache.head_dim
-    _need_tensor(ctx, "kv_append: k", k, t.bfloat16, (None, cache.kv_heads * d), rows=True)
+    ldk = _rows(ctx, "kv_append: k", k, t.bfloat16, None, cache.kv_heads * d)
     n = k.shape[0]
-    _need_tensor(ctx, "kv_append: v", v, t.bfloat16, (n, cache.kv_heads * d), rows=True)
-    _need_tensor(ctx, "kv_append: pos", pos, t.int32, (n,))
-    _need_tensor(ctx, "kv_append: block_table", block_table, t.int32, (None, None))
+    ldv = _rows(ctx, "kv_append: v", v, t.bfloat16, n, cache.kv_heads * d)
+    _vector(ctx, "kv_append: pos", pos, t.int32, n)
+    n_seqs, pages = _table(ctx, "kv_append", block_table)
     if seq is not None:
-        _need_tensor(ctx, "kv_append: seq", seq, t.int32, (n,))
+        _vector(ctx, "kv_append: seq", seq, t.int32, n)
     r = None
     if rope is not None:
         cos, sin, off = rope
-        _need_tensor(ctx, "kv_append: cos", cos, t.float32, (None, None))
-        _need_tensor(ctx, "kv_append: sin", sin, t.float32, cos.shape)
-        r = RopeStruct(cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1], int(off), int(bool(rope_half)))
-    heads = 0
+        _need(_rows(ctx, "kv_append: cos", cos, t.float32) == cos.shape[1] == _rows(ctx, "kv_append: sin", sin, t.float32, *cos.shape),
+              "kv_append: cos and sin must be contiguous")
+        r = C.byref(RopeStruct(cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1], off, 1 if rope_half else 0))
+    heads = ldq = ldo = qp = op = 0
     if q is not None:
-        _need_tensor(ctx, "kv_append: q", q, t.bfloat16, (n, None), rows=True)
-        _need(q.shape[1] % d == 0 and q.shape[1] > 0, "kv_append: q's rows must hold whole heads")
-        heads = q.shape[1] // d
+        ldq = _rows(ctx, "kv_append: q", q, t.bfloat16, n)
+        width = q.shape[1]
+        heads = width // d
+        _need(heads > 0 and heads * d == width, "kv_append: q's rows must hold whole heads")
         if q_out is None:
-            q_out = t.empty((n, heads * d), dtype=t.bfloat16, device=ctx.device)
-        else:
-            _need_tensor(ctx, "kv_append: q_out", q_out, t.bfloat16, q.shape, rows=True)
-    ctx.check(lib().dsuf_kv_append(ctx.h, ctx.stream(), C.byref(cache.c), k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), n, pos.data_ptr(),
-                                   seq.data_ptr() if seq is not None else 0, block_table.data_ptr(), block_table.shape[0], block_table.shape[1],
-                                   C.byref(r) if r is not None else None, q.data_ptr() if heads else 0, _ld(q) if heads else 0, heads,
-                                   q_out.data_ptr() if heads else 0, _ld(q_out) if heads else 0))
+            q_out = t.empty((n, width), dtype=t.bfloat16, device=ctx.device)
+        ldo = _rows(ctx, "kv_append: q_out", q_out, t.bfloat16, n, width)
+        qp, op = q.data_ptr(), q_out.data_ptr()
+    ctx.check(lib().dsuf_kv_append(ctx.h, ctx.stream(), cache.ref, k.data_ptr(), ldk, v.data_ptr(), ldv, n, pos.data_ptr(),
+                                   seq.data_ptr() if seq is not None else 0, block_table.data_ptr(), n_seqs, pages, r, qp, ldq, heads, op, ldo))
     return q_out
 
 
@@ -705,26 +729,27 @@ def attn_decode(ctx, cache, q, block_table, seq_lens, scale=None, window=0, out=
     t = ctx.torch
     _need(cache.ctx is ctx, "attn_decode: the cache belongs to another context")
     d = cache.head_dim
-    _need_tensor(ctx, "attn_decode: q", q, t.bfloat16, (None, None), rows=True)
+    ldq = _rows(ctx, "attn_decode: q", q, t.bfloat16)
     b, width = q.shape
+    heads = width // d
     _need(width > 0 and width % (d * cache.kv_heads) == 0, "attn_decode: q's rows must hold a multiple of kv_heads heads")
-    _need_tensor(ctx, "attn_decode: block_table", block_table, t.int32, (b, None))
-    _need_tensor(ctx, "attn_decode: seq_lens", seq_lens, t.int32, (b,))
+    n_seqs, pages = _table(ctx, "attn_decode", block_table)
+    _need(n_seqs == b, "attn_decode: block_table holds one row per row of q")
+    _vector(ctx, "attn_decode: seq_lens", seq_lens, t.int32, b)
     if out is None:
         out = t.empty((b, width), dtype=t.bfloat16, device=ctx.device)
-    else:
-        _need_tensor(ctx, "attn_decode: out", out, t.bfloat16, (b, width), rows=True)
+    ldo = _rows(ctx, "attn_decode: out", out, t.bfloat16, b, width)
+    if lse is None and return_lse:
+        lse = t.empty((b, heads), dtype=t.float32, device=ctx.device)
     if lse is not None:
-        _need_tensor(ctx, "attn_decode: lse", lse, t.float32, (b, width // d))
-    elif return_lse:
-        lse = t.empty((b, width // d), dtype=t.float32, device=ctx.device)
+        _need(_rows(ctx, "attn_decode: lse", lse, t.float32, b, heads) == heads, "attn_decode: lse must be contiguous")
     if workspace is None:
         workspace = ctx.attn_workspace
     else:
-        _need_tensor(ctx, "attn_decode: workspace", workspace, t.uint8, (ctx.attn_workspace.numel(),))
-    ctx.check(lib().dsuf_attn_decode(ctx.h, ctx.stream(), C.byref(cache.c), q.data_ptr(), _ld(q), width // d, b, block_table.data_ptr(),
-                                     block_table.shape[1], seq_lens.data_ptr(), d ** -0.5 if scale is None else scale, window, out.data_ptr(), _ld(out),
-                                     lse.data_ptr() if lse is not None else 0, workspace.data_ptr()))
+        _vector(ctx, "attn_decode: workspace", workspace, t.uint8, ctx.attn_workspace.shape[0])
+    ctx.check(lib().dsuf_attn_decode(ctx.h, ctx.stream(), cache.ref, q.data_ptr(), ldq, heads, b, block_table.data_ptr(), pages, seq_lens.data_ptr(),
+                                     d ** -0.5 if scale is None else scale, window, out.data_ptr(), ldo, lse.data_ptr() if lse is not None else 0,
+                                     workspace.data_ptr()))
     return (out, lse) if return_lse else out
 
 
@@ -734,25 +759,25 @@ def attn_prompt(ctx, q, k, v, cu_seqlens, head_dim=128, scale=None, window=0, ou
     included.  ``scale`` None: head_dim ** -0.5.  Rows behind the last sequence are not written.  Returns out bf16
     [t][q_heads * head_dim], or (out, lse f32 [t][q_heads]) with ``return_lse``."""
     t = ctx.torch
-    _need_tensor(ctx, "attn_prompt: q", q, t.bfloat16, (None, None), rows=True)
+    _need(head_dim in (64, 128), "attn_prompt: head_dim is 64 or 128")
+    ldq = _rows(ctx, "attn_prompt: q", q, t.bfloat16)
     n, width = q.shape
-    _need_tensor(ctx, "attn_prompt: k", k, t.bfloat16, (n, None), rows=True)
-    _need_tensor(ctx, "attn_prompt: v", v, t.bfloat16, k.shape, rows=True)
-    _need(head_dim in (64, 128) and width % head_dim == 0 and k.shape[1] % head_dim == 0, "attn_prompt: head_dim is 64 or 128 and rows hold whole heads")
-    _need_tensor(ctx, "attn_prompt: cu_seqlens", cu_seqlens, t.int32, (None,))
+    ldk = _rows(ctx, "attn_prompt: k", k, t.bfloat16, n)
+    ldv = _rows(ctx, "attn_prompt: v", v, t.bfloat16, n, k.shape[1])
+    heads, kv_heads = width // head_dim, k.shape[1] // head_dim
+    _need(heads * head_dim == width and kv_heads * head_dim == k.shape[1], "attn_prompt: rows hold whole heads")
+    _vector(ctx, "attn_prompt: cu_seqlens", cu_seqlens, t.int32)
     _need(cu_seqlens.shape[0] >= 1, "attn_prompt: cu_seqlens holds at least one entry")
     if out is None:
         out = t.empty((n, width), dtype=t.bfloat16, device=ctx.device)
-    else:
-        _need_tensor(ctx, "attn_prompt: out", out, t.bfloat16, (n, width), rows=True)
+    ldo = _rows(ctx, "attn_prompt: out", out, t.bfloat16, n, width)
+    if lse is None and return_lse:
+        lse = t.empty((n, heads), dtype=t.float32, device=ctx.device)
     if lse is not None:
-        _need_tensor(ctx, "attn_prompt: lse", lse, t.float32, (n, width // head_dim))
-    elif return_lse:
-        lse = t.empty((n, width // head_dim), dtype=t.float32, device=ctx.device)
-    ctx.check(lib().dsuf_attn_prompt(ctx.h, ctx.stream(), q.data_ptr(), _ld(q), k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), n, width // head_dim,
-                                     k.shape[1] // head_dim, head_dim, cu_seqlens.data_ptr(), cu_seqlens.shape[0] - 1,
-                                     head_dim ** -0.5 if scale is None else scale, window, out.data_ptr(), _ld(out),
-                                     lse.data_ptr() if lse is not None else 0))
+        _need(_rows(ctx, "attn_prompt: lse", lse, t.float32, n, heads) == heads, "attn_prompt: lse must be contiguous")
+    ctx.check(lib().dsuf_attn_prompt(ctx.h, ctx.stream(), q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, n, heads, kv_heads, head_dim,
+                                     cu_seqlens.data_ptr(), cu_seqlens.shape[0] - 1, head_dim ** -0.5 if scale is None else scale, window,
+                                     out.data_ptr(), ldo, lse.data_ptr() if lse is not None else 0))
     return (out, lse) if return_lse else out
 
 
@@ -761,23 +786,24 @@ def sample(ctx, logits, u, temperature=None, top_k=None, top_p=None, min_p=None,
     temperature, top-k, top-p and min-p (tensors of one value per row; None: off; see include/dsuf_qmm.h for the order and ties).
     Returns ids i32 [m], or (ids, logprobs f32 [m]) with ``return_logprobs``: the raw log-probabilities of the drawn tokens."""
     t = ctx.torch
-    _need_tensor(ctx, "sample: logits", logits, t.float32, (None, None), rows=True)
+    ld = _rows(ctx, "sample: logits", logits, t.float32)
     m, n = logits.shape
-    _need_tensor(ctx, "sample: u", u, t.float32, (m,))
+    _vector(ctx, "sample: u", u, t.float32, m)
     ptrs = []
-    for name, x, dtype in (("temperature", temperature, t.float32), ("top_k", top_k, t.int32), ("top_p", top_p, t.float32), ("min_p", min_p, t.float32)):
+    for name, x, dtype in (("sample: temperature", temperature, t.float32), ("sample: top_k", top_k, t.int32), ("sample: top_p", top_p, t.float32),
+                           ("sample: min_p", min_p, t.float32)):
         if x is not None:
-            _need_tensor(ctx, "sample: " + name, x, dtype, (m,))
-        ptrs.append(x.data_ptr() if x is not None else 0)
+            _vector(ctx, name, x, dtype, m)
+        ptrs.append(0 if x is None else x.data_ptr())
     if ids is None:
         ids = t.empty(m, dtype=t.int32, device=ctx.device)
     else:
-        _need_tensor(ctx, "sample: ids", ids, t.int32, (m,))
-    if logprobs is not None:
-        _need_tensor(ctx, "sample: logprobs", logprobs, t.float32, (m,))
-    elif return_logprobs:
+        _vector(ctx, "sample: ids", ids, t.int32, m)
+    if logprobs is None and return_logprobs:
         logprobs = t.empty(m, dtype=t.float32, device=ctx.device)
-    ctx.check(lib().dsuf_sample(ctx.h, ctx.stream(), logits.data_ptr(), _ld(logits), m, n, *ptrs, u.data_ptr(), ids.data_ptr(),
+    if logprobs is not None:
+        _vector(ctx, "sample: logprobs", logprobs, t.float32, m)
+    ctx.check(lib().dsuf_sample(ctx.h, ctx.stream(), logits.data_ptr(), ld, m, n, *ptrs, u.data_ptr(), ids.data_ptr(),
                                 logprobs.data_ptr() if logprobs is not None else 0))
     return (ids, logprobs) if return_logprobs else ids
 

@@ -45,6 +45,7 @@ int32_t dsuf_ctx_create(int32_t device, dsuf_ctx** out) {
     if (!rc) rc = lm_head_setup(ctx);
     if (!rc) rc = attn_decode_setup(ctx);
     if (!rc) rc = attn_prompt_setup(ctx);
+    if (!rc) rc = sample_setup(ctx);
     if (rc) { cudaFree(ctx->dev_status); delete ctx; return rc; }
     *out = ctx;
     return DSUF_OK;

@@ -127,6 +127,7 @@ int stream_setup(dsuf_ctx* ctx);
 int lm_head_setup(dsuf_ctx* ctx);
 int attn_decode_setup(dsuf_ctx* ctx);
 int attn_prompt_setup(dsuf_ctx* ctx);
+int sample_setup(dsuf_ctx* ctx);
 int check_kv_cache(dsuf_ctx* ctx, const char* who, const dsuf_kv_cache* c);
 int encode_x_map(dsuf_ctx* ctx, CUtensorMap* tm, const void* base, int k_bytes, long long rows, int box_rows);
 

@@ -10,12 +10,14 @@
 // later passes).  Weights are 40-bit fixed point, their sums 64-bit integers: exact, so the result depends neither on the split nor
 // on the order of the histogram's atomics.  Passes:
 //   1. largest and smallest logit
-//   2. weights: their sum and, when top-k or top-p is on, counts and weights of 1024 bins of l (linear from M down, so that bins
-//      are evenly filled; a monotone map, so bins are an order)
-//   3. per limit, the tokens of the one bin where it falls are listed (usually some dozens) and ranked against each other: the limit becomes
-//      a threshold (logit, id).  A bin with more than 512 tokens is split again by the bits of the logits, down to equal
-//      ones, of which the id decides.
+//   2. top-k: counts in 2048 bins of l (linear from M down, so that bins are evenly filled; a monotone map, so bins are an order).  The
+//      tokens of the one bin where the limit falls are listed (usually some dozens) and ranked against each other: the limit becomes a
+//      threshold (logit, id).  A bin with more than 512 tokens is split again by the bits of the logits, down to equal ones, of which
+//      the id decides.
+//   3. top-p: the same with weights, over the tokens inside the first limit (without top-k: all)
 //   4. weight of C per warp, and the owner of the drawn number walks its part.
+// What the CTAs tell each other is pushed into everybody's shared memory before a barrier, not fetched after it: a remote load costs
+// about 250 cycles, and there are many.
 // The exponent is formed in 64 bits ((l - M) / T rounded to fp32 would be off by 1e-6 relative in a far token's weight).
 #include "internal.h"
 
@@ -23,7 +25,7 @@ namespace dsuf {
 
 constexpr int SA_THREADS = 512;
 constexpr int SA_WARPS = SA_THREADS / 32;
-constexpr int SA_BINS = 1024;
+constexpr int SA_BINS = 2048;
 constexpr int SA_LIST = 512;
 constexpr int SA_MAX_CLUSTER = 8;
 constexpr float SA_ONE = 1099511627776.f;   // weight 1 in fixed point: 2^40
@@ -54,25 +56,26 @@ DSUF_DEV uint32_t order_key(float l) {   // unsigned that orders like the float
 DSUF_DEV float key_value(uint32_t k) { return __uint_as_float((k >> 31) ? (k & 0x7fffffffu) : ~k); }
 
 struct SampleShared {
-    uint32_t count[SA_BINS];         // this CTA's histogram
-    u64 mass[SA_BINS];
-    uint32_t all_count[SA_BINS];     // the row's
+    uint32_t count[SA_BINS];                       // this CTA's histogram
+    uint32_t mass_lo[SA_BINS], mass_hi[SA_BINS];
+    uint32_t all_count[SA_BINS];                   // the row's
     u64 all_mass[SA_BINS];
-    uint32_t list_key[SA_LIST];      // this CTA's tokens of the limit's bin
+    uint32_t list_key[SA_LIST];                    // this CTA's tokens of the limit's bin
     int list_id[SA_LIST];
-    uint32_t row_key[SA_LIST];       // the row's
-    int row_id[SA_LIST];
+    u64 row_at[SA_LIST];                           // the row's, as one word that orders them: key, then the complement of the id
     u64 row_w[SA_LIST];
     uint32_t n_list;
+    uint32_t lists[SA_MAX_CLUSTER];
     float top[SA_MAX_CLUSTER], low[SA_MAX_CLUSTER], lp[SA_MAX_CLUSTER];
     int first[SA_MAX_CLUSTER];
     u64 kept[SA_MAX_CLUSTER];
     uint32_t key_hi[SA_MAX_CLUSTER], key_lo[SA_MAX_CLUSTER], ties[SA_MAX_CLUSTER];
+    uint32_t own_hi, own_lo;
     u64 warp_a[SA_WARPS];
     uint32_t warp_b[SA_WARPS];
     float warp_f[SA_WARPS], warp_g[SA_WARPS];
     int found_bin;
-    u64 found_mass, found_a, found_b;
+    u64 found_mass, found_before;
     uint32_t found_count, found_key;
     int found_id;
 };
@@ -87,7 +90,6 @@ struct Sampler {
     uint32_t rank, ctas;
     float top, inv_bin;
     double inv_temp;
-    bool stale;              // the row's histogram has been replaced by a split bin's
 
     DSUF_DEV float clean(float l) const { return l == l ? l + 0.f : -INFINITY; }   // NaN is never drawn; -0 orders as 0
     DSUF_DEV void line(int v, float* l) const {
@@ -133,8 +135,7 @@ struct Sampler {
         const float f = (top - l) * inv_bin;
         return f < (float)(SA_BINS - 1) ? (int)f : SA_BINS - 1;
     }
-    // f(sum, value) over the CTA; the result in every thread
-    DSUF_DEV u64 block_sum(u64 v) {
+    DSUF_DEV u64 block_sum(u64 v) {     // over the CTA, the result in every thread
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
         __syncthreads();
@@ -146,103 +147,105 @@ struct Sampler {
         return r;
     }
 
-    // ---- a limit: by count (top-k: `want` tokens) or by weight (top-p: the token whose weight reaches `target`) ----
+    // The last token inside a limit: everything of a larger key is inside, and of this key the ids up to `id`.
     struct Limit {
-        uint32_t key;     // the last token inside: everything of a larger key, and of this key the ids up to `id`
+        uint32_t key;
         int id;
-        u64 mass;         // weight of all inside
+        DSUF_DEV bool holds(uint32_t k, int i) const { return k > key || (k == key && i <= id); }
     };
-    DSUF_DEV static bool inside(const Limit& lim, uint32_t key, int id) { return key > lim.key || (key == lim.key && id <= lim.id); }
 
     DSUF_DEV void clear_bins() {
-        for (int i = tid; i < SA_BINS; i += SA_THREADS) {
-            s.count[i] = 0;
-            s.mass[i] = 0;
-        }
+        for (int i = tid; i < SA_BINS; i += SA_THREADS) s.count[i] = s.mass_lo[i] = s.mass_hi[i] = 0;
         __syncthreads();
     }
-    // the CTAs' histograms into everybody's all_count / all_mass
-    DSUF_DEV void share_bins() {
+    DSUF_DEV void add(uint32_t b, u64 w, bool with_mass) {
+        atomicAdd(&s.count[b], 1u);
+        if (with_mass) {
+            // a 64-bit sum in two words: the carry of the low one goes with the high one
+            const uint32_t lo = (uint32_t)w, old = atomicAdd(&s.mass_lo[b], lo);
+            const uint32_t hi = (uint32_t)(w >> 32) + (old + lo < old ? 1u : 0u);
+            if (hi) atomicAdd(&s.mass_hi[b], hi);
+        }
+    }
+    // the CTAs' histograms, summed, into everybody's all_count / all_mass
+    DSUF_DEV void share_bins(bool with_mass) {
         cluster_barrier();
         const int per = SA_BINS / ctas;
         for (int i = tid; i < per; i += SA_THREADS) {
             const int b = rank * per + i;
-            uint32_t c = 0;
-            u64 m = 0;
-            for (uint32_t r = 0; r < ctas; ++r) {
-                c += *in_cta(&s.count[b], r);
-                m += *in_cta(&s.mass[b], r);
+            uint32_t c[SA_MAX_CLUSTER], lo[SA_MAX_CLUSTER], hi[SA_MAX_CLUSTER];
+#pragma unroll
+            for (uint32_t r = 0; r < SA_MAX_CLUSTER; ++r) {
+                c[r] = lo[r] = hi[r] = 0;
+                if (r < ctas) {
+                    c[r] = ld_cluster_u32(&s.count[b], r);
+                    if (with_mass) {
+                        lo[r] = ld_cluster_u32(&s.mass_lo[b], r);
+                        hi[r] = ld_cluster_u32(&s.mass_hi[b], r);
+                    }
+                }
+            }
+            uint32_t cs = 0;
+            u64 ms = 0;
+#pragma unroll
+            for (uint32_t r = 0; r < SA_MAX_CLUSTER; ++r) {
+                cs += c[r];
+                ms += ((u64)hi[r] << 32) + lo[r];
             }
             for (uint32_t r = 0; r < ctas; ++r) {
-                *in_cta(&s.all_count[b], r) = c;
-                *in_cta(&s.all_mass[b], r) = m;
+                *in_cta(&s.all_count[b], r) = cs;
+                *in_cta(&s.all_mass[b], r) = ms;
             }
         }
         cluster_barrier();
     }
-    // first bin where count (or weight) reaches the limit, counting from `count0` / `mass0`: bin, and what lies before it
-    DSUF_DEV void find_bin(bool by_mass, u64 want, double target, u64 count0, u64 mass0, int only_bin, u64 only_mass) {
+    // The bin where the limit falls (by count: the first where `want` tokens are reached, by weight: `target`), counting from count0 /
+    // mass0, and what lies before it.
+    DSUF_DEV void find_bin(bool by_mass, u64 want, double target, u64 count0, u64 mass0) {
         constexpr int PER = SA_BINS / SA_THREADS;
-        uint32_t c[PER];
-        u64 m[PER], cs = 0, ms = 0;
+        u64 c[PER], cs = 0;
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
             const int b = tid * PER + e;
-            c[e] = s.all_count[b];
-            m[e] = b == only_bin ? only_mass : b > only_bin ? 0 : s.all_mass[b];   // (top-p inside A: A's last bin counts with its part)
+            c[e] = by_mass ? s.all_mass[b] : s.all_count[b];
             cs += c[e];
-            ms += m[e];
         }
-        u64 ci = cs, mi = ms;
+        u64 ci = cs;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const u64 cv = __shfl_up_sync(0xffffffffu, ci, o), mv = __shfl_up_sync(0xffffffffu, mi, o);
-            if (lane >= o) { ci += cv; mi += mv; }
+            const u64 cv = __shfl_up_sync(0xffffffffu, ci, o);
+            if (lane >= o) ci += cv;
         }
         __syncthreads();
-        if (lane == 31) {
-            s.warp_a[warp] = mi;
-            s.warp_b[warp] = (uint32_t)ci;
-        }
-        if (tid == 0) s.found_bin = -1;
+        if (lane == 31) s.warp_a[warp] = ci;
         __syncthreads();
-        u64 cb = count0 + ci - cs, mb = mass0 + mi - ms;
-        for (int w = 0; w < warp; ++w) { cb += s.warp_b[w]; mb += s.warp_a[w]; }
+        u64 cb = (by_mass ? mass0 : count0) + ci - cs;
+        for (int w = 0; w < warp; ++w) cb += s.warp_a[w];
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
-            const bool hit = by_mass ? (double)mb < target && target <= (double)(mb + m[e]) : cb < want && want <= cb + c[e];
+            const bool hit = by_mass ? (double)cb < target && target <= (double)(cb + c[e]) : cb < want && want <= cb + c[e];
             if (hit) {
                 s.found_bin = tid * PER + e;
-                s.found_a = cb;
-                s.found_mass = mb;
-                s.found_count = c[e];
+                s.found_before = cb;
+                s.found_count = s.all_count[tid * PER + e];
             }
             cb += c[e];
-            mb += m[e];
         }
         __syncthreads();
     }
 
-    // The limit inside the row's histogram (all_count / all_mass of bin()).  `within`: only tokens inside this earlier limit count
-    // (top-p inside A), or null.
-    DSUF_DEV Limit limit(bool by_mass, u64 want, double target, const Limit* within) {
-        int only_bin = SA_BINS;
-        u64 only_mass = 0;
-        if (within) {
-            only_bin = bin(key_value(within->key));
-            u64 before = 0;
-            for (int i = tid; i < only_bin; i += SA_THREADS) before += s.all_mass[i];
-            only_mass = within->mass - block_sum(before);
-        }
-        find_bin(by_mass, want, target, 0, 0, only_bin, only_mass);
+    // The limit inside the row's histogram of bin() over the tokens that `within` holds: `want` tokens, or the token whose weight, added to
+    // that of all before it, reaches `target`.  One of the two exists: want is at most the number of tokens, target at most their weight.
+    DSUF_DEV Limit limit(bool by_mass, u64 want, double target, const Limit within) {
+        find_bin(by_mass, want, target, 0, 0);
         const int b0 = s.found_bin;
-        u64 count0 = s.found_a, mass0 = s.found_mass;
+        u64 before = s.found_before;      // tokens, or weight, ahead of the bin
         uint32_t n_in = s.found_count, k_hi = 0xffffffffu, k_lo = 0;
         __syncthreads();
         auto mine = [&](int id, float l) {
             if (l == -INFINITY || bin(l) != b0) return false;
             const uint32_t k = order_key(l);
-            return k >= k_lo && k <= k_hi && (!within || inside(*within, k, id));
+            return k >= k_lo && k <= k_hi && within.holds(k, id);
         };
         bool first_split = true;
         while (n_in > SA_LIST && k_hi != k_lo) {
@@ -257,42 +260,41 @@ struct Sampler {
                 });
                 hi = __reduce_max_sync(0xffffffffu, hi);
                 lo = __reduce_min_sync(0xffffffffu, lo);
-                if (tid == 0) { s.key_hi[rank] = 0; s.key_lo[rank] = 0xffffffffu; }
+                if (tid == 0) { s.own_hi = 0; s.own_lo = 0xffffffffu; }
                 __syncthreads();
-                if (lane == 0) { atomicMax(&s.key_hi[rank], hi); atomicMin(&s.key_lo[rank], lo); }
+                if (lane == 0) { atomicMax(&s.own_hi, hi); atomicMin(&s.own_lo, lo); }
+                __syncthreads();
+                if (tid < ctas) {
+                    *in_cta(&s.key_hi[rank], tid) = s.own_hi;
+                    *in_cta(&s.key_lo[rank], tid) = s.own_lo;
+                }
                 cluster_barrier();
                 k_hi = 0; k_lo = 0xffffffffu;
                 for (uint32_t r = 0; r < ctas; ++r) {
-                    k_hi = max(k_hi, *in_cta(&s.key_hi[r], r));
-                    k_lo = min(k_lo, *in_cta(&s.key_lo[r], r));
+                    k_hi = max(k_hi, s.key_hi[r]);
+                    k_lo = min(k_lo, s.key_lo[r]);
                 }
                 first_split = false;
             }
             int shift = 0;
             while (((k_hi - k_lo) >> shift) >= (uint32_t)SA_BINS) ++shift;
-            cluster_barrier();               // (the others are through with this CTA's histogram and keys)
-            stale = true;
+            cluster_barrier();               // (the others are through with this CTA's histogram)
             clear_bins();
             each([&](int id, float l) {
-                if (mine(id, l)) {
-                    const uint32_t b = (k_hi - order_key(l)) >> shift;
-                    atomicAdd(&s.count[b], 1u);
-                    atomicAdd(&s.mass[b], fixed(weight(l)));
-                }
+                if (mine(id, l)) add((k_hi - order_key(l)) >> shift, by_mass ? fixed(weight(l)) : 0, by_mass);
             });
-            share_bins();
-            find_bin(by_mass, want, target, count0, mass0, SA_BINS, 0);
+            share_bins(by_mass);
+            find_bin(by_mass, want, target, before, before);
             const uint32_t b = (uint32_t)s.found_bin;
-            count0 = s.found_a;
-            mass0 = s.found_mass;
+            before = s.found_before;
             n_in = s.found_count;
             __syncthreads();
             k_hi -= b << shift;
-            k_lo = max(k_lo, k_hi - ((1u << shift) - 1u));
+            k_lo = max(k_lo, k_hi - min(k_hi, (1u << shift) - 1u));
         }
         Limit out;
         if (n_in <= SA_LIST) {
-            // list the tokens, everybody gets them all, every thread ranks one
+            // list the tokens, everybody gets them all, every thread ranks one or a share of one
             if (tid == 0) s.n_list = 0;
             __syncthreads();
             each([&](int id, float l) {
@@ -304,97 +306,96 @@ struct Sampler {
                     }
                 }
             });
+            __syncthreads();
+            if (tid < ctas) *in_cta(&s.lists[rank], tid) = min(s.n_list, (uint32_t)SA_LIST);
             cluster_barrier();
-            uint32_t base = 0;
+            uint32_t total = 0;
             for (uint32_t r = 0; r < ctas; ++r) {
-                const uint32_t n = min(*in_cta(&s.n_list, r), (uint32_t)SA_LIST);
-                for (uint32_t i = tid; i < n && base + i < SA_LIST; i += SA_THREADS) {
-                    const uint32_t k = *in_cta(&s.list_key[i], r);
-                    s.row_key[base + i] = k;
-                    s.row_id[base + i] = *in_cta(&s.list_id[i], r);
-                    s.row_w[base + i] = fixed(weight(key_value(k)));
-                }
-                base = min(base + n, (uint32_t)SA_LIST);
+                const uint32_t n = s.lists[r];
+                // (the warps of a CTA take the lists in turn, so that their remote loads overlap)
+                if (warp % ctas == r)
+                    for (uint32_t i = (warp / ctas) * 32 + lane; i < n && total + i < SA_LIST; i += (SA_WARPS / ctas) * 32) {
+                        const uint32_t k = ld_cluster_u32(&s.list_key[i], r);
+                        s.row_at[total + i] = ((u64)k << 32) | (0xffffffffu - ld_cluster_u32(&s.list_id[i], r));
+                        s.row_w[total + i] = by_mass ? fixed(weight(key_value(k))) : 1;
+                    }
+                total = min(total + n, (uint32_t)SA_LIST);
             }
             cluster_barrier();               // (nobody reads this CTA's list any more)
-            for (uint32_t i = tid; i < base; i += SA_THREADS) {
-                const uint32_t k = s.row_key[i];
-                const int id = s.row_id[i];
-                u64 c = count0, m = mass0;
-                for (uint32_t j = 0; j < base; ++j) {
-                    const uint32_t kj = s.row_key[j];
-                    if (kj > k || (kj == k && s.row_id[j] < id)) {
-                        ++c;
-                        m += s.row_w[j];
-                    }
-                }
-                const u64 after = m + s.row_w[i];
-                if (by_mass ? (double)m < target && target <= (double)after : c + 1 == want) {
-                    s.found_key = k;
-                    s.found_id = id;
-                    s.found_b = after;
+            int share = 1;                   // threads per token
+            while (share < 32 && total * share * 2 <= SA_THREADS) share <<= 1;
+            const uint32_t i = tid / share;
+            const u64 mine_at = i < total ? s.row_at[i] : 0;
+            u64 c = 0;
+            for (uint32_t j = tid % share; j < total; j += share)
+                if (s.row_at[j] > mine_at) c += s.row_w[j];
+            for (int o = share >> 1; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+            if (i < total && tid % share == 0) {
+                c += before;
+                const u64 after = c + s.row_w[i];
+                if (by_mass ? (double)c < target && target <= (double)after : c < want && want <= after) {
+                    s.found_key = (uint32_t)(mine_at >> 32);
+                    s.found_id = (int)(0xffffffffu - (uint32_t)mine_at);
                 }
             }
             __syncthreads();
             out.key = s.found_key;
             out.id = s.found_id;
-            out.mass = s.found_b;
             __syncthreads();
             return out;
         }
         // many equal logits: the r-th lowest id among them
         const u64 w = fixed(weight(key_value(k_hi)));
-        u64 r = by_mass ? (u64)ceil((target - (double)mass0) / (double)(w ? w : 1)) : want - count0;
-        r = max(r, (u64)1);
-        r = min(r, (u64)n_in);
+        u64 r = by_mass ? (u64)ceil((target - (double)before) / (double)(w ? w : 1)) : want - before;
+        r = min(max(r, (u64)1), (u64)n_in);
         out.key = k_hi;
-        out.mass = mass0 + r * w;
         uint32_t eq = 0;
         each([&](int id, float l) { eq += mine(id, l) ? 1u : 0u; });
         eq = __reduce_add_sync(0xffffffffu, eq);
         __syncthreads();
         if (lane == 0) s.warp_b[warp] = eq;
         __syncthreads();
-        if (tid == 0) {
+        if (tid < ctas) {
             uint32_t t = 0;
             for (int q = 0; q < SA_WARPS; ++q) t += s.warp_b[q];
-            for (uint32_t q = 0; q < ctas; ++q) *in_cta(&s.ties[rank], q) = t;
+            *in_cta(&s.ties[rank], tid) = t;
         }
         cluster_barrier();
-        u64 before = 0;
-        for (uint32_t q = 0; q < rank; ++q) before += s.ties[q];
-        for (int q = 0; q < warp; ++q) before += s.warp_b[q];
-        if (before < r && r <= before + eq) {
+        u64 ahead = 0;
+        for (uint32_t q = 0; q < rank; ++q) ahead += s.ties[q];
+        for (int q = 0; q < warp; ++q) ahead += s.warp_b[q];
+        if (ahead < r && r <= ahead + eq) {
             // this warp holds it: walk its lines in order
             for (int v = v0; v < v1; v += 32) {
                 float l[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                 if (v + lane < v1) line(v + lane, l);
-                uint32_t c = 0;
+                uint32_t n = 0;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) c += mine(4 * (v + lane) - lead + e, l[e]) ? 1u : 0u;
-                uint32_t upto = c;
+                for (int e = 0; e < 4; ++e) n += mine(4 * (v + lane) - lead + e, l[e]) ? 1u : 0u;
+                uint32_t upto = n;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
                     const uint32_t t = __shfl_up_sync(0xffffffffu, upto, o);
                     if (lane >= o) upto += t;
                 }
-                u64 at = before + upto - c;
+                u64 at = ahead + upto - n;
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     if (mine(4 * (v + lane) - lead + e, l[e]) && ++at == r)
                         for (uint32_t q = 0; q < ctas; ++q) *in_cta(&s.found_id, q) = 4 * (v + lane) - lead + e;
-                before += __shfl_sync(0xffffffffu, upto, 31);
+                ahead += __shfl_sync(0xffffffffu, upto, 31);
             }
         }
         cluster_barrier();
         out.id = s.found_id;
-        __syncthreads();
+        cluster_barrier();    // (a faster CTA's next limit does not write into found_id yet)
         return out;
     }
 };
 
 __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleArgs a) {
-    __shared__ SampleShared s;
+    extern __shared__ __align__(16) uint8_t smem[];
+    SampleShared& s = *reinterpret_cast<SampleShared*>(smem);
     pdl_wait();
     pdl_launch_dependents();
     const uint32_t rank = cluster_cta_rank(), ctas = cluster_num_ctas();
@@ -404,7 +405,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleArgs 
     const int lead = (int)(((uintptr_t)x >> 2) & 3);
     const int lines = (int)(((long long)a.n + lead + 3) / 4);
     const long long parts = (long long)ctas * SA_WARPS, part = (long long)rank * SA_WARPS + warp;
-    Sampler z{a, s, x, lead, (int)(lines * part / parts), (int)(lines * (part + 1) / parts), tid, warp, lane, rank, ctas, 0.f, 0.f, 0.0, false};
+    Sampler z{a, s, x, lead, (int)(lines * part / parts), (int)(lines * (part + 1) / parts), tid, warp, lane, rank, ctas, 0.f, 0.f, 0.0};
     const float temp = a.temperature ? a.temperature[row] : 1.f;
     const int top_k = a.top_k ? a.top_k[row] : 0;
     const float top_p = a.top_p ? a.top_p[row] : 1.f, min_p = a.min_p ? fminf(a.min_p[row], 1.f) : 0.f;
@@ -426,20 +427,24 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleArgs 
     }
     if (lane == 0) { s.warp_f[warp] = hi; s.warp_g[warp] = lo; s.warp_b[warp] = (uint32_t)at; }
     __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < SA_WARPS; ++w) {
-            if (s.warp_f[w] > hi || (s.warp_f[w] == hi && (int)s.warp_b[w] < at)) { hi = s.warp_f[w]; at = (int)s.warp_b[w]; }
-            lo = fminf(lo, s.warp_g[w]);
+    if (tid < ctas) {
+        for (int w = 0; w < SA_WARPS; ++w) {
+            const float h = s.warp_f[w];
+            const int i = (int)s.warp_b[w];
+            if (w == 0 || h > hi || (h == hi && i < at)) { hi = h; at = i; }
+            lo = w == 0 ? s.warp_g[w] : fminf(lo, s.warp_g[w]);
         }
-        s.top[rank] = hi; s.low[rank] = lo; s.first[rank] = at;
+        *in_cta(&s.top[rank], tid) = hi;
+        *in_cta(&s.low[rank], tid) = lo;
+        *in_cta(&s.first[rank], tid) = at;
     }
     cluster_barrier();
     hi = -INFINITY; lo = INFINITY; at = 0x7fffffff;
     for (uint32_t r = 0; r < ctas; ++r) {
-        const float h = *in_cta(&s.top[r], r);
-        const int i = *in_cta(&s.first[r], r);
+        const float h = s.top[r];
+        const int i = s.first[r];
         if (h > hi || (h == hi && i < at)) { hi = h; at = i; }
-        lo = fminf(lo, *in_cta(&s.low[r], r));
+        lo = fminf(lo, s.low[r]);
     }
     z.top = hi;
     if (hi == -INFINITY) {    // nothing to draw from
@@ -454,27 +459,48 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleArgs 
     const float span = fminf(hi - lo, fmaxf(24.f, 32.f * temp));
     z.inv_bin = span > 0.f && span < INFINITY ? (float)(SA_BINS - 1) / span : 0.f;
 
-    // ---- pass 2: weights; the log-probability's sum at temperature 1 ----
-    const bool limited = !greedy && (top_k > 0 || top_p < 1.f);
-    if (limited) z.clear_bins();
-    u64 sum = 0;
+    // ---- the limits; the first pass over all tokens also sums for the log-probability (temperature 1) ----
+    bool want_lp = a.logprobs != nullptr;
     float lp = 0.f;
-    uint32_t tokens = 0;
-    if (!greedy || a.logprobs) {
+    u64 sum = 0;
+    Sampler::Limit lim;
+    lim.key = order_key(-INFINITY) + 1;    // every token above -inf
+    lim.id = 0x7fffffff;
+    if (!greedy && top_k > 0) {
+        z.clear_bins();
         z.each([&](int id, float l) {
             if (l == -INFINITY) return;
-            if (a.logprobs) lp += l == hi ? 1.f : expf(l - hi);
-            if (greedy) return;
-            const float w = z.weight(l);
-            const u64 f = z.fixed(w);
-            if (limited) {
-                const int b = z.bin(l);
-                ++tokens;
-                sum += f;
-                atomicAdd(&s.count[b], 1u);
-                atomicAdd(&s.mass[b], f);
-            } else if (w >= min_p || l == hi) {
-                sum += f;
+            if (want_lp) lp += expf(l == hi ? 0.f : l - hi);
+            z.add(z.bin(l), 0, false);
+        });
+        want_lp = false;
+        z.share_bins(false);
+        u64 tokens = 0;
+        for (int i = tid; i < SA_BINS; i += SA_THREADS) tokens += s.all_count[i];
+        if ((u64)top_k < z.block_sum(tokens)) lim = z.limit(false, (u64)top_k, 0.0, lim);
+    }
+    if (!greedy && top_p < 1.f) {
+        if (top_k > 0) cluster_barrier();   // (the others are through with this CTA's histogram)
+        z.clear_bins();
+        z.each([&](int id, float l) {
+            if (l == -INFINITY) return;
+            if (want_lp) lp += expf(l == hi ? 0.f : l - hi);
+            if (lim.holds(order_key(l), id)) z.add(z.bin(l), z.fixed(z.weight(l)), true);
+        });
+        want_lp = false;
+        z.share_bins(true);
+        u64 mass = 0;
+        for (int i = tid; i < SA_BINS; i += SA_THREADS) mass += s.all_mass[i];
+        // the first token is always inside: a target below one unit of weight is reached by it
+        lim = z.limit(true, 0, fmax((double)top_p * (double)z.block_sum(mass), 0.5), lim);
+    }
+    if (!greedy || want_lp) {
+        z.each([&](int id, float l) {
+            if (l == -INFINITY) return;
+            if (want_lp) lp += expf(l == hi ? 0.f : l - hi);
+            if (!greedy && lim.holds(order_key(l), id)) {
+                const float w = z.weight(l);
+                if (w >= min_p || l == hi) sum += z.fixed(w);
             }
         });
     }
@@ -484,52 +510,11 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleArgs 
         __syncthreads();
         if (lane == 0) s.warp_f[warp] = lp;
         __syncthreads();
-        if (tid == 0) {
+        if (tid < ctas) {
             float t = 0.f;
             for (int w = 0; w < SA_WARPS; ++w) t += s.warp_f[w];
-            s.lp[rank] = t;
+            *in_cta(&s.lp[rank], tid) = t;
         }
-    }
-    Sampler::Limit lim;
-    lim.key = order_key(-INFINITY) + 1;    // every token above -inf
-    lim.id = 0x7fffffff;
-    lim.mass = 0;
-    if (limited) {
-        // the row's number of tokens and weight
-        const u64 n_mine = z.block_sum(tokens), m_mine = z.block_sum(sum);
-        if (tid == 0) { s.kept[rank] = m_mine; s.ties[rank] = (uint32_t)n_mine; }
-        z.share_bins();
-        u64 n_all = 0, m_all = 0;
-        for (uint32_t r = 0; r < ctas; ++r) {
-            n_all += *in_cta(&s.ties[r], r);
-            m_all += *in_cta(&s.kept[r], r);
-        }
-        lim.mass = m_all;
-        const bool cut = top_k > 0 && (u64)top_k < n_all;
-        if (cut) lim = z.limit(false, (u64)top_k, 0.0, nullptr);
-        if (top_p < 1.f) {
-            // the first token is always inside: a target below one unit of weight is reached by it
-            const double target = fmax((double)top_p * (double)lim.mass, 0.5);
-            const Sampler::Limit k = lim;
-            if (z.stale) {
-                cluster_barrier();
-                z.clear_bins();
-                z.each([&](int id, float l) {
-                    if (l == -INFINITY) return;
-                    atomicAdd(&s.count[z.bin(l)], 1u);
-                    atomicAdd(&s.mass[z.bin(l)], z.fixed(z.weight(l)));
-                });
-                z.share_bins();
-            }
-            lim = z.limit(true, 0, target, cut ? &k : nullptr);
-        }
-        sum = 0;
-        z.each([&](int id, float l) {
-            if (l > -INFINITY && Sampler::inside(lim, order_key(l), id)) {
-                const float w = z.weight(l);
-                if (w >= min_p || l == hi) sum += z.fixed(w);
-            }
-        });
     }
 
     // ---- the draw ----
@@ -541,11 +526,10 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleArgs 
         __syncthreads();
         if (lane == 0) s.warp_a[warp] = mine;
         __syncthreads();
-        cluster_barrier();      // (kept is read no more as the row's weight)
-        if (tid == 0) {
+        if (tid < ctas) {
             u64 t = 0;
             for (int w = 0; w < SA_WARPS; ++w) t += s.warp_a[w];
-            for (uint32_t r = 0; r < ctas; ++r) *in_cta(&s.kept[rank], r) = t;
+            *in_cta(&s.kept[rank], tid) = t;
         }
         cluster_barrier();
         u64 total = 0, before = 0;
@@ -568,7 +552,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleArgs 
                 for (int e = 0; e < 4; ++e) {
                     const int id = 4 * (v + lane) - lead + e;
                     w[e] = 0;
-                    if (l[e] > -INFINITY && Sampler::inside(lim, order_key(l[e]), id)) {
+                    if (l[e] > -INFINITY && lim.holds(order_key(l[e]), id)) {
                         const float f = z.weight(l[e]);
                         if (f >= min_p || l[e] == hi) w[e] = z.fixed(f);
                     }
@@ -589,7 +573,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleArgs 
                             a.ids[row] = token;
                             if (a.logprobs) {
                                 float t = 0.f;
-                                for (uint32_t r = 0; r < ctas; ++r) t += *in_cta(&s.lp[r], r);
+                                for (uint32_t r = 0; r < ctas; ++r) t += s.lp[r];
                                 a.logprobs[row] = (l[e] == hi ? 0.f : l[e] - hi) - logf(t);
                             }
                         }
@@ -606,12 +590,17 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleArgs 
             a.ids[row] = token;
             if (a.logprobs) {
                 float t = 0.f;
-                for (uint32_t r = 0; r < ctas; ++r) t += *in_cta(&s.lp[r], r);
+                for (uint32_t r = 0; r < ctas; ++r) t += s.lp[r];
                 a.logprobs[row] = -logf(t);
             }
         }
     }
     cluster_barrier();    // nobody leaves while its shared memory may be read
+}
+
+int sample_setup(dsuf_ctx* ctx) {
+    cudaError_t e = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SampleShared));
+    return e == cudaSuccess ? DSUF_OK : cuda_fail(ctx, e, "cudaFuncSetAttribute(sample)");
 }
 
 }  // namespace dsuf
@@ -634,5 +623,5 @@ extern "C" int32_t dsuf_sample(dsuf_ctx* ctx, void* stream, uint64_t logits, int
     // as many CTAs per row as the GPU holds at once (two per SM), each with at least 2048 logits: fewer are not worth the cluster's barriers
     int c = SA_MAX_CLUSTER;
     while (c > 1 && ((long long)m * c > 2ll * ctx->sm_count || n < 2048 * c)) c >>= 1;
-    return launch_cluster(ctx, (cudaStream_t)stream, sample_kernel, dim3(m * c), dim3(SA_THREADS), 0, c, a);
+    return launch_cluster(ctx, (cudaStream_t)stream, sample_kernel, dim3(m * c), dim3(SA_THREADS), sizeof(SampleShared), c, a);
 }
