@@ -340,7 +340,7 @@ class Ctx:
         self.check(lib().dsuf_ctx_set_wait_budget_us(self.h, int(microseconds)))
 
     def stream(self):
-        return C.c_void_p(self.torch.cuda.current_stream(self.device).cuda_stream)
+        return C.c_void_p(self.torch._C._cuda_getCurrentRawStream(self.index))   # (the current stream without an object around it)
 
     def check(self, rc):
         if rc:

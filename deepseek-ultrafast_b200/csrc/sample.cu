@@ -6,19 +6,22 @@
 // The reference's sampler (crates/kernels/cu/sample.cu) merges the output head's records; this one works on the logits themselves, so that
 // top_k and top_p have no limit.
 //
-// Nothing is sorted.  A cluster of up to 8 CTAs shares a row (latency-bound at few rows; the row comes from HBM once and from L2 in the
+// Nothing is sorted.  A cluster of up to 16 CTAs shares a row (latency-bound at few rows; the row comes from HBM once and from L2 in the
 // later passes).  Weights are 40-bit fixed point, their sums 64-bit integers: exact, so the result depends neither on the split nor
 // on the order of the histogram's atomics.  Passes:
-//   1. largest and smallest logit
+//   1. the largest logit
 //   2. top-k: counts in 2048 bins of l (linear from M down, so that bins are evenly filled; a monotone map, so bins are an order).  The
 //      tokens of the one bin where the limit falls are listed (usually some dozens) and ranked against each other: the limit becomes a
-//      threshold (logit, id).  A bin with more than 512 tokens is split again by the bits of the logits, down to equal ones, of which
+//      threshold (logit, id).  A bin with more than 1024 tokens is split again by the bits of the logits, down to equal ones, of which
 //      the id decides.
 //   3. top-p: the same with weights, over the tokens inside the first limit (without top-k: all)
 //   4. weight of C per warp, and the owner of the drawn number walks its part.
+// Where all tokens down to the first limit's bin fit the list (the usual case: top_k up to about a thousand, or a peaked row), one CTA finishes
+// from the list: ranks, both limits, min-p and the draw (129280 logits, top_k 50, top_p 0.9: 16 us instead of 38).
 // What the CTAs tell each other is pushed into everybody's shared memory before a barrier, not fetched after it: a remote load costs
 // about 250 cycles, and there are many.
-// The exponent is formed in 64 bits ((l - M) / T rounded to fp32 would be off by 1e-6 relative in a far token's weight).
+// With many rows the passes are bound by instructions (some 30 per logit and weight), not by bytes, so every pass computes no more than it needs.
+// The exponent is carried in two fp32 numbers ((l - M) / T rounded to one would be off by 1e-6 relative in a far token's weight).
 #include "internal.h"
 
 namespace dsuf {
@@ -26,9 +29,10 @@ namespace dsuf {
 constexpr int SA_THREADS = 512;
 constexpr int SA_WARPS = SA_THREADS / 32;
 constexpr int SA_BINS = 2048;
-constexpr int SA_LIST = 512;
-constexpr int SA_MAX_CLUSTER = 8;
-constexpr float SA_ONE = 1099511627776.f;   // weight 1 in fixed point: 2^40
+constexpr int SA_LIST = 1024;
+constexpr int SA_MAX_CLUSTER = 16;
+constexpr int SA_PER = SA_LIST / SA_THREADS;
+constexpr int SA_FRACTION = 40;             // weight 1 in fixed point is 2^40
 typedef unsigned long long u64;
 
 struct SampleArgs {
@@ -56,28 +60,34 @@ DSUF_DEV uint32_t order_key(float l) {   // unsigned that orders like the float
 DSUF_DEV float key_value(uint32_t k) { return __uint_as_float((k >> 31) ? (k & 0x7fffffffu) : ~k); }
 
 struct SampleShared {
-    uint32_t count[SA_BINS];                       // this CTA's histogram
-    uint32_t mass_lo[SA_BINS], mass_hi[SA_BINS];
-    uint32_t all_count[SA_BINS];                   // the row's
-    u64 all_mass[SA_BINS];
+    uint32_t lo[SA_BINS], hi[SA_BINS];             // this CTA's histogram: counts (lo), or weights in two words
+    u64 all[SA_BINS];                              // the row's
     uint32_t list_key[SA_LIST];                    // this CTA's tokens of the limit's bin
     int list_id[SA_LIST];
     u64 row_at[SA_LIST];                           // the row's, as one word that orders them: key, then the complement of the id
     u64 row_w[SA_LIST];
     uint32_t n_list;
     uint32_t lists[SA_MAX_CLUSTER];
-    float top[SA_MAX_CLUSTER], low[SA_MAX_CLUSTER], lp[SA_MAX_CLUSTER];
+    float top[SA_MAX_CLUSTER], lp[SA_MAX_CLUSTER];
     int first[SA_MAX_CLUSTER];
     u64 kept[SA_MAX_CLUSTER];
     uint32_t key_hi[SA_MAX_CLUSTER], key_lo[SA_MAX_CLUSTER], ties[SA_MAX_CLUSTER];
     uint32_t own_hi, own_lo;
-    u64 warp_a[SA_WARPS];
+    int own_first;
+    u64 warp_a[SA_WARPS], warp_c[SA_WARPS];
     uint32_t warp_b[SA_WARPS];
-    float warp_f[SA_WARPS], warp_g[SA_WARPS];
+    float warp_f[SA_WARPS];
     int found_bin;
-    u64 found_mass, found_before;
-    uint32_t found_count, found_key;
+    u64 found_before;
+    uint32_t found_key;
     int found_id;
+};
+
+// The last token inside a limit: everything larger is inside, and of its equals the ids up to `id`.
+struct Limit {
+    float value;
+    int id;
+    DSUF_DEV bool holds(float l, int i) const { return l > value || (l == value && i <= id); }
 };
 
 struct Sampler {
@@ -88,52 +98,68 @@ struct Sampler {
     int v0, v1;              // this warp's 16-byte lines
     int tid, warp, lane;
     uint32_t rank, ctas;
-    float top, inv_bin;
-    double inv_temp;
+    float top, inv_bin, inv_temp, inv_temp_rest;   // inv_temp: log2(e) / T
 
-    DSUF_DEV float clean(float l) const { return l == l ? l + 0.f : -INFINITY; }   // NaN is never drawn; -0 orders as 0
+    DSUF_DEV static float clean(float l) { return fmaxf(l, -INFINITY); }   // a NaN counts as -inf: never drawn
     DSUF_DEV void line(int v, float* l) const {
         const int i = 4 * v - lead;
-        if (i >= 0 && i + 4 <= a.n) {
-            const float4 q = *reinterpret_cast<const float4*>(x + i);
-            l[0] = clean(q.x); l[1] = clean(q.y); l[2] = clean(q.z); l[3] = clean(q.w);
-        } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) l[e] = i + e >= 0 && i + e < a.n ? clean(x[i + e]) : -INFINITY;
-        }
+        for (int e = 0; e < 4; ++e) l[e] = i + e >= 0 && i + e < a.n ? clean(x[i + e]) : -INFINITY;
     }
-    // f(id, logit) for every element of this warp's part (ids outside the row come as -inf)
+    // f(id, logit) for every element of this warp's part.  Lines that reach over the row's ends are read by elements.
     template <typename F>
     DSUF_DEV void each(F f) const {
-        int v = v0 + lane;
-        for (; v + 96 < v1; v += 128) {     // four lines in flight
-            float l[4][4];
+        const int full0 = lead > 0 ? 1 : 0, full1 = (a.n + lead) >> 2;
+        const float4* lines = reinterpret_cast<const float4*>(x - lead);
+        const int end = min(v1, full1);
+        int v = max(v0, full0) + lane;
+        auto four = [&](int w, float4 q) {
+            f(4 * w - lead, clean(q.x));
+            f(4 * w - lead + 1, clean(q.y));
+            f(4 * w - lead + 2, clean(q.z));
+            f(4 * w - lead + 3, clean(q.w));
+        };
+        for (; v + 96 < end; v += 128) {     // four lines in flight
+            float4 q[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) line(v + 32 * j, l[j]);
+            for (int j = 0; j < 4; ++j) q[j] = lines[v + 32 * j];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) f(4 * (v + 32 * j) - lead + e, l[j][e]);
+            for (int j = 0; j < 4; ++j) four(v + 32 * j, q[j]);
         }
-        for (; v < v1; v += 32) {
-            float l[4];
-            line(v, l);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) f(4 * v - lead + e, l[e]);
+        for (; v < end; v += 32) four(v, lines[v]);
+        if (lane < 2) {                      // lane 0: a cut first line, lane 1: a cut last one
+            const int w = lane ? full1 : 0;
+            const bool cut = lane ? ((a.n + lead) & 3) != 0 && !(full1 == 0 && full0) : full0 != 0;
+            if (cut && w >= v0 && w < v1) {
+                float l[4];
+                line(w, l);
+                for (int e = 0; e < 4; ++e) f(4 * w - lead + e, l[e]);
+            }
         }
     }
+    // exp((l - top) / T).  The difference and the product are carried as unevaluated sums of two fp32 numbers (Knuth's two-sum, an fma for the
+    // product's rest), because a rounding of the exponent is a relative error of the weight; the rests enter as a factor 1 + rest.
     DSUF_DEV float weight(float l) const {
-        if (l == top) return 1.f;
-        const double z = ((double)l - (double)top) * inv_temp;
-        const float hi = (float)z;
-        if (!(hi > -80.f)) return 0.f;
-        return expf(hi) * (1.f + (float)(z - (double)hi));
+        const float d = fminf(l - top, 0.f);          // (inf - inf is NaN: 0)
+        const float v = d - l;
+        const float d_rest = top < INFINITY ? (l - (d - v)) + (-top - v) : 0.f;
+        const float z = d * inv_temp;
+        const float z_rest = fmaf(d, inv_temp, -z) + fmaf(d, inv_temp_rest, d_rest * inv_temp);
+        float w;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(z));
+        return z > -100.f ? fmaf(w, z_rest * 0.6931471805599453f, w) : 0.f;
     }
-    DSUF_DEV u64 fixed(float w) const { return (u64)(w * SA_ONE); }
+    // w * 2^40, truncated
+    DSUF_DEV static u64 fixed(float w) {
+        const uint32_t b = __float_as_uint(w);
+        const int shift = (int)(b >> 23) - (127 + 23 - SA_FRACTION);
+        const uint32_t m = (b & 0x7fffffu) | 0x800000u;
+        return shift >= 0 ? (u64)m << shift : (u64)(m >> min(-shift, 31));
+    }
+    // (rounding to the nearest bin by the addition's own rounding: any map that never goes up with the logit will do)
     DSUF_DEV int bin(float l) const {
-        if (l == top) return 0;
-        const float f = (top - l) * inv_bin;
-        return f < (float)(SA_BINS - 1) ? (int)f : SA_BINS - 1;
+        const float f = fminf((top - l) * inv_bin, (float)(SA_BINS - 1));
+        return l == top ? 0 : (int)(__float_as_uint(f + 8388608.f) & (SA_BINS - 1));
     }
     DSUF_DEV u64 block_sum(u64 v) {     // over the CTA, the result in every thread
 #pragma unroll
@@ -147,67 +173,51 @@ struct Sampler {
         return r;
     }
 
-    // The last token inside a limit: everything of a larger key is inside, and of this key the ids up to `id`.
-    struct Limit {
-        uint32_t key;
-        int id;
-        DSUF_DEV bool holds(uint32_t k, int i) const { return k > key || (k == key && i <= id); }
-    };
-
     DSUF_DEV void clear_bins() {
-        for (int i = tid; i < SA_BINS; i += SA_THREADS) s.count[i] = s.mass_lo[i] = s.mass_hi[i] = 0;
+        for (int i = tid; i < SA_BINS; i += SA_THREADS) s.lo[i] = s.hi[i] = 0;
         __syncthreads();
     }
-    DSUF_DEV void add(uint32_t b, u64 w, bool with_mass) {
-        atomicAdd(&s.count[b], 1u);
-        if (with_mass) {
-            // a 64-bit sum in two words: the carry of the low one goes with the high one
-            const uint32_t lo = (uint32_t)w, old = atomicAdd(&s.mass_lo[b], lo);
-            const uint32_t hi = (uint32_t)(w >> 32) + (old + lo < old ? 1u : 0u);
-            if (hi) atomicAdd(&s.mass_hi[b], hi);
-        }
+    DSUF_DEV void add(uint32_t b, u64 w) {
+        // a 64-bit sum in two words: the carry of the low one goes with the high one
+        const uint32_t lo = (uint32_t)w, old = atomicAdd(&s.lo[b], lo);
+        const uint32_t hi = (uint32_t)(w >> 32) + (old + lo < old ? 1u : 0u);
+        if (hi) atomicAdd(&s.hi[b], hi);
     }
-    // the CTAs' histograms, summed, into everybody's all_count / all_mass
-    DSUF_DEV void share_bins(bool with_mass) {
+    // the CTAs' histograms, summed, into everybody's `all`
+    DSUF_DEV void share_bins(bool two_words) {
         cluster_barrier();
         const int per = SA_BINS / ctas;
         for (int i = tid; i < per; i += SA_THREADS) {
             const int b = rank * per + i;
-            uint32_t c[SA_MAX_CLUSTER], lo[SA_MAX_CLUSTER], hi[SA_MAX_CLUSTER];
+            uint32_t lo[SA_MAX_CLUSTER], hi[SA_MAX_CLUSTER];
 #pragma unroll
             for (uint32_t r = 0; r < SA_MAX_CLUSTER; ++r) {
-                c[r] = lo[r] = hi[r] = 0;
-                if (r < ctas) {
-                    c[r] = ld_cluster_u32(&s.count[b], r);
-                    if (with_mass) {
-                        lo[r] = ld_cluster_u32(&s.mass_lo[b], r);
-                        hi[r] = ld_cluster_u32(&s.mass_hi[b], r);
-                    }
-                }
+                lo[r] = r < ctas ? ld_cluster_u32(&s.lo[b], r) : 0;
+                hi[r] = r < ctas && two_words ? ld_cluster_u32(&s.hi[b], r) : 0;
             }
-            uint32_t cs = 0;
-            u64 ms = 0;
+            u64 sum = 0;
 #pragma unroll
-            for (uint32_t r = 0; r < SA_MAX_CLUSTER; ++r) {
-                cs += c[r];
-                ms += ((u64)hi[r] << 32) + lo[r];
-            }
-            for (uint32_t r = 0; r < ctas; ++r) {
-                *in_cta(&s.all_count[b], r) = cs;
-                *in_cta(&s.all_mass[b], r) = ms;
-            }
+            for (uint32_t r = 0; r < SA_MAX_CLUSTER; ++r) sum += ((u64)hi[r] << 32) + lo[r];
+            for (uint32_t r = 0; r < ctas; ++r) *in_cta(&s.all[b], r) = sum;
         }
         cluster_barrier();
     }
-    // The bin where the limit falls (by count: the first where `want` tokens are reached, by weight: `target`), counting from count0 /
-    // mass0, and what lies before it.
-    DSUF_DEV void find_bin(bool by_mass, u64 want, double target, u64 count0, u64 mass0) {
+    DSUF_DEV u64 bins_sum() {
+        u64 v = 0;
+        for (int i = tid; i < SA_BINS; i += SA_THREADS) v += s.all[i];
+        return block_sum(v);
+    }
+    // Whether an amount that goes from `from` to `to` is where the limit falls: the first to reach `want` tokens, or the weight `target`.
+    DSUF_DEV static bool reaches(bool by_mass, u64 want, double target, u64 from, u64 to) {
+        return by_mass ? (double)from < target && target <= (double)to : from < want && want <= to;
+    }
+    // The bin where the limit falls, counting from `start`, and the amount before it.
+    DSUF_DEV int find_bin(bool by_mass, u64 want, double target, u64& start) {
         constexpr int PER = SA_BINS / SA_THREADS;
         u64 c[PER], cs = 0;
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
-            const int b = tid * PER + e;
-            c[e] = by_mass ? s.all_mass[b] : s.all_count[b];
+            c[e] = s.all[tid * PER + e];
             cs += c[e];
         }
         u64 ci = cs;
@@ -219,43 +229,215 @@ struct Sampler {
         __syncthreads();
         if (lane == 31) s.warp_a[warp] = ci;
         __syncthreads();
-        u64 cb = (by_mass ? mass0 : count0) + ci - cs;
+        u64 cb = start + ci - cs;
         for (int w = 0; w < warp; ++w) cb += s.warp_a[w];
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
-            const bool hit = by_mass ? (double)cb < target && target <= (double)(cb + c[e]) : cb < want && want <= cb + c[e];
-            if (hit) {
+            if (reaches(by_mass, want, target, cb, cb + c[e])) {
                 s.found_bin = tid * PER + e;
                 s.found_before = cb;
-                s.found_count = s.all_count[tid * PER + e];
             }
             cb += c[e];
         }
         __syncthreads();
+        const int b = s.found_bin;
+        start = s.found_before;
+        __syncthreads();
+        return b;
+    }
+
+    DSUF_DEV static uint32_t key(float l) { return order_key(l + 0.f); }     // (-0 orders as 0)
+    // Lists this CTA's tokens that `take` wants (as far as there is room) and returns how many the row has.
+    template <typename F>
+    DSUF_DEV uint32_t list(F take) {
+        if (tid == 0) s.n_list = 0;
+        __syncthreads();
+        each([&](int id, float l) {
+            if (take(id, l)) {
+                const uint32_t at = atomicAdd(&s.n_list, 1u);
+                if (at < SA_LIST) {
+                    s.list_key[at] = key(l);
+                    s.list_id[at] = id;
+                }
+            }
+        });
+        __syncthreads();
+        if (tid < ctas) *in_cta(&s.lists[rank], tid) = s.n_list;
+        cluster_barrier();
+        uint32_t total = 0;
+        for (uint32_t r = 0; r < ctas; ++r) total += s.lists[r];    // (at most n)
+        return total;
+    }
+    // All CTAs' lists (at most SA_LIST tokens together) into row_at.  The warps take the CTAs in turn, so that their remote loads overlap.
+    DSUF_DEV void fetch_list() {
+        uint32_t base = 0;
+        for (uint32_t r = 0; r < ctas; ++r) {
+            const uint32_t n = s.lists[r];
+            if (warp % ctas == r)
+                for (uint32_t i = (warp / ctas) * 32 + lane; i < n; i += (SA_WARPS / ctas) * 32)
+                    s.row_at[base + i] = ((u64)ld_cluster_u32(&s.list_key[i], r) << 32) | (0xffffffffu - ld_cluster_u32(&s.list_id[i], r));
+            base += n;
+        }
+    }
+    // Sorts row_at (distinct words), largest first.  Up to 256 tokens by counting: a token's place is the number of larger ones, counted by
+    // 2 to 32 threads of a warp (64 tokens: 0.5 us; a bitonic network, whose 21 steps each wait for shared memory twice, 3 us).  More by
+    // a bitonic network (1024 tokens: 4 us against 20), where a warp's 32 pairs at distances up to 32 lie in 64 words of its own.
+    DSUF_DEV void sort_list(uint32_t total) {
+        __syncthreads();
+        if (total <= 256) {
+            uint32_t bits = 1;
+            while (bits < 5 && (total << (bits + 1)) <= SA_THREADS) ++bits;
+            const uint32_t share = 1u << bits, first = tid & (share - 1), i = tid >> bits;
+            const u64 at = i < total ? s.row_at[i] : ~0ull;
+            uint32_t place = 0;
+            if ((uint32_t)(tid & ~31) >> bits < total) {
+#pragma unroll 4
+                for (uint32_t j = first; j < total; j += share) place += s.row_at[j] > at ? 1u : 0u;
+                for (uint32_t o = share >> 1; o > 0; o >>= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
+            }
+            __syncthreads();
+            if (first == 0 && i < total) s.row_at[place] = at;
+            __syncthreads();
+            return;
+        }
+        uint32_t n = 512;
+        while (n < total) n <<= 1;
+        for (uint32_t i = total + tid; i < n; i += SA_THREADS) s.row_at[i] = 0;     // (below every token)
+        __syncthreads();
+        for (uint32_t k = 2; k <= n; k <<= 1)
+            for (uint32_t j = k >> 1; j > 0; j >>= 1) {
+                if (tid < n / 2) {
+                    const uint32_t lo = tid + (tid & ~(j - 1)), hi = lo + j;      // the pairs of distance j, numbered by tid
+                    const u64 p = s.row_at[lo], q = s.row_at[hi];
+                    if ((p < q) == ((lo & k) == 0)) {
+                        s.row_at[lo] = q;
+                        s.row_at[hi] = p;
+                    }
+                }
+                if (j > 32 || (j == 1 && k >= 64)) __syncthreads();
+                else __syncwarp();
+            }
+    }
+    // Sums of what the earlier threads, and this thread earlier, hold (w: SA_PER values of each).
+    DSUF_DEV u64 block_ahead(const u64* w, u64* ahead) {
+        u64 own = 0;
+#pragma unroll
+        for (int e = 0; e < SA_PER; ++e) own += w[e];
+        u64 upto = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        __syncthreads();
+        if (lane == 31) s.warp_a[warp] = upto;
+        __syncthreads();
+        u64 at = upto - own, all = 0;
+#pragma unroll
+        for (int q = 0; q < SA_WARPS; ++q) {
+            if (q < warp) at += s.warp_a[q];
+            all += s.warp_a[q];
+        }
+#pragma unroll
+        for (int e = 0; e < SA_PER; ++e) {
+            ahead[e] = at;
+            at += w[e];
+        }
+        return all;
+    }
+    // The whole rest of a row whose candidates are all listed (one CTA): the first `want` of the order, of these the ones whose preceding weight
+    // is below top_p of `mass` (0: of their own), of these min_p, and the draw.
+    template <typename F>
+    DSUF_DEV void finish(uint32_t total, u64 want, float top_p, u64 mass, float min_p, float u, F store) {
+        sort_list(total);
+        float l[SA_PER], f[SA_PER];
+        u64 w[SA_PER], ahead[SA_PER];
+        uint32_t id[SA_PER];
+#pragma unroll
+        for (int e = 0; e < SA_PER; ++e) {
+            const uint32_t i = tid * SA_PER + e;
+            const bool in = i < total && i < want;
+            const u64 at = in ? s.row_at[i] : 0;
+            id[e] = 0xffffffffu - (uint32_t)at;
+            l[e] = key_value((uint32_t)(at >> 32));
+            f[e] = in ? weight(l[e]) : 0.f;
+            w[e] = in ? fixed(f[e]) : 0;
+        }
+        const u64 own = block_ahead(w, ahead);
+        const double target = top_p < 1.f ? fmax((double)top_p * (double)(mass ? mass : own), 0.5) : INFINITY;
+        // the tokens that stay, in the order of their ids
+        if (tid == 0) s.n_list = 0;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < SA_PER; ++e) {
+            s.row_w[tid * SA_PER + e] = w[e];
+            if (w[e] && (double)ahead[e] < target && (f[e] >= min_p || l[e] == top))
+                s.row_at[atomicAdd(&s.n_list, 1u)] = ((u64)(0xffffffffu - id[e]) << 32) | (uint32_t)(tid * SA_PER + e);
+        }
+        __syncthreads();
+        const uint32_t stay = s.n_list;
+        sort_list(stay);
+#pragma unroll
+        for (int e = 0; e < SA_PER; ++e) {
+            const uint32_t i = tid * SA_PER + e;
+            w[e] = i < stay ? s.row_w[(uint32_t)s.row_at[i]] : 0;
+        }
+        const u64 kept = block_ahead(w, ahead);
+        u64 draw = u > 0.f ? (u64)((double)u * (double)kept) : 0;
+        draw = min(draw, kept - 1);
+#pragma unroll
+        for (int e = 0; e < SA_PER; ++e)
+            if (ahead[e] <= draw && draw < ahead[e] + w[e]) {
+                const uint32_t token = 0xffffffffu - (uint32_t)(s.row_at[tid * SA_PER + e] >> 32);
+                store((int)token, clean(x[token]));
+            }
     }
 
     // The limit inside the row's histogram of bin() over the tokens that `within` holds: `want` tokens, or the token whose weight, added to
     // that of all before it, reaches `target`.  One of the two exists: want is at most the number of tokens, target at most their weight.
-    DSUF_DEV Limit limit(bool by_mass, u64 want, double target, const Limit within) {
-        find_bin(by_mass, want, target, 0, 0);
-        const int b0 = s.found_bin;
-        u64 before = s.found_before;      // tokens, or weight, ahead of the bin
-        uint32_t n_in = s.found_count, k_hi = 0xffffffffu, k_lo = 0;
-        __syncthreads();
+    // b0: the bin where it falls, before: tokens, or weight, ahead of it.
+    DSUF_DEV Limit limit(bool by_mass, u64 want, double target, const Limit within, int b0, u64 before) {
+        uint32_t k_hi = 0xffffffffu, k_lo = 0;
         auto mine = [&](int id, float l) {
-            if (l == -INFINITY || bin(l) != b0) return false;
-            const uint32_t k = order_key(l);
-            return k >= k_lo && k <= k_hi && within.holds(k, id);
+            if (bin(l) != b0 || !within.holds(l, id)) return false;
+            const uint32_t k = key(l);
+            return k >= k_lo && k <= k_hi;
         };
-        bool first_split = true;
-        while (n_in > SA_LIST && k_hi != k_lo) {
-            // split the bin by its logits' bits
+        for (bool first_split = true;; first_split = false) {
+            // everybody gets the bin's tokens, every thread ranks some or a share of one
+            const uint32_t total = list(mine);
+            if (total <= SA_LIST) {
+                fetch_list();
+                cluster_barrier();               // (nobody reads this CTA's list any more)
+                sort_list(total);
+                u64 w[SA_PER], ahead[SA_PER];
+#pragma unroll
+                for (int e = 0; e < SA_PER; ++e) {
+                    const uint32_t i = tid * SA_PER + e;
+                    w[e] = i < total ? by_mass ? fixed(weight(key_value((uint32_t)(s.row_at[i] >> 32)))) : 1 : 0;
+                }
+                block_ahead(w, ahead);
+#pragma unroll
+                for (int e = 0; e < SA_PER; ++e) {
+                    const uint32_t i = tid * SA_PER + e;
+                    if (i < total && reaches(by_mass, want, target, before + ahead[e], before + ahead[e] + w[e])) {
+                        s.found_key = (uint32_t)(s.row_at[i] >> 32);
+                        s.found_id = (int)(0xffffffffu - (uint32_t)s.row_at[i]);
+                    }
+                }
+                __syncthreads();
+                const Limit out = {key_value(s.found_key), s.found_id};
+                __syncthreads();
+                return out;
+            }
+            if (k_hi == k_lo) break;
+            // too many: split the bin by its logits' bits
             if (first_split) {
                 uint32_t hi = 0, lo = 0xffffffffu;
                 each([&](int id, float l) {
                     if (mine(id, l)) {
-                        hi = max(hi, order_key(l));
-                        lo = min(lo, order_key(l));
+                        hi = max(hi, key(l));
+                        lo = min(lo, key(l));
                     }
                 });
                 hi = __reduce_max_sync(0xffffffffu, hi);
@@ -274,81 +456,19 @@ struct Sampler {
                     k_hi = max(k_hi, s.key_hi[r]);
                     k_lo = min(k_lo, s.key_lo[r]);
                 }
-                first_split = false;
             }
             int shift = 0;
             while (((k_hi - k_lo) >> shift) >= (uint32_t)SA_BINS) ++shift;
-            cluster_barrier();               // (the others are through with this CTA's histogram)
-            clear_bins();
+            clear_bins();      // (the others read this CTA's histogram before the last barrier)
             each([&](int id, float l) {
-                if (mine(id, l)) add((k_hi - order_key(l)) >> shift, by_mass ? fixed(weight(l)) : 0, by_mass);
+                if (mine(id, l)) add((k_hi - key(l)) >> shift, by_mass ? fixed(weight(l)) : 1);
             });
             share_bins(by_mass);
-            find_bin(by_mass, want, target, before, before);
-            const uint32_t b = (uint32_t)s.found_bin;
-            before = s.found_before;
-            n_in = s.found_count;
-            __syncthreads();
+            const uint32_t b = (uint32_t)find_bin(by_mass, want, target, before);
             k_hi -= b << shift;
             k_lo = max(k_lo, k_hi - min(k_hi, (1u << shift) - 1u));
         }
-        Limit out;
-        if (n_in <= SA_LIST) {
-            // list the tokens, everybody gets them all, every thread ranks one or a share of one
-            if (tid == 0) s.n_list = 0;
-            __syncthreads();
-            each([&](int id, float l) {
-                if (mine(id, l)) {
-                    const uint32_t at = atomicAdd(&s.n_list, 1u);
-                    if (at < SA_LIST) {
-                        s.list_key[at] = order_key(l);
-                        s.list_id[at] = id;
-                    }
-                }
-            });
-            __syncthreads();
-            if (tid < ctas) *in_cta(&s.lists[rank], tid) = min(s.n_list, (uint32_t)SA_LIST);
-            cluster_barrier();
-            uint32_t total = 0;
-            for (uint32_t r = 0; r < ctas; ++r) {
-                const uint32_t n = s.lists[r];
-                // (the warps of a CTA take the lists in turn, so that their remote loads overlap)
-                if (warp % ctas == r)
-                    for (uint32_t i = (warp / ctas) * 32 + lane; i < n && total + i < SA_LIST; i += (SA_WARPS / ctas) * 32) {
-                        const uint32_t k = ld_cluster_u32(&s.list_key[i], r);
-                        s.row_at[total + i] = ((u64)k << 32) | (0xffffffffu - ld_cluster_u32(&s.list_id[i], r));
-                        s.row_w[total + i] = by_mass ? fixed(weight(key_value(k))) : 1;
-                    }
-                total = min(total + n, (uint32_t)SA_LIST);
-            }
-            cluster_barrier();               // (nobody reads this CTA's list any more)
-            int share = 1;                   // threads per token
-            while (share < 32 && total * share * 2 <= SA_THREADS) share <<= 1;
-            const uint32_t i = tid / share;
-            const u64 mine_at = i < total ? s.row_at[i] : 0;
-            u64 c = 0;
-            for (uint32_t j = tid % share; j < total; j += share)
-                if (s.row_at[j] > mine_at) c += s.row_w[j];
-            for (int o = share >> 1; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
-            if (i < total && tid % share == 0) {
-                c += before;
-                const u64 after = c + s.row_w[i];
-                if (by_mass ? (double)c < target && target <= (double)after : c < want && want <= after) {
-                    s.found_key = (uint32_t)(mine_at >> 32);
-                    s.found_id = (int)(0xffffffffu - (uint32_t)mine_at);
-                }
-            }
-            __syncthreads();
-            out.key = s.found_key;
-            out.id = s.found_id;
-            __syncthreads();
-            return out;
-        }
         // many equal logits: the r-th lowest id among them
-        const u64 w = fixed(weight(key_value(k_hi)));
-        u64 r = by_mass ? (u64)ceil((target - (double)before) / (double)(w ? w : 1)) : want - before;
-        r = min(max(r, (u64)1), (u64)n_in);
-        out.key = k_hi;
         uint32_t eq = 0;
         each([&](int id, float l) { eq += mine(id, l) ? 1u : 0u; });
         eq = __reduce_add_sync(0xffffffffu, eq);
@@ -361,9 +481,15 @@ struct Sampler {
             *in_cta(&s.ties[rank], tid) = t;
         }
         cluster_barrier();
-        u64 ahead = 0;
-        for (uint32_t q = 0; q < rank; ++q) ahead += s.ties[q];
+        u64 ahead = 0, all = 0;
+        for (uint32_t q = 0; q < ctas; ++q) {
+            if (q < rank) ahead += s.ties[q];
+            all += s.ties[q];
+        }
         for (int q = 0; q < warp; ++q) ahead += s.warp_b[q];
+        const u64 w = fixed(weight(key_value(k_hi)));
+        u64 r = by_mass ? (u64)ceil((target - (double)before) / (double)(w ? w : 1)) : want - before;
+        r = min(max(r, (u64)1), all);
         if (ahead < r && r <= ahead + eq) {
             // this warp holds it: walk its lines in order
             for (int v = v0; v < v1; v += 32) {
@@ -387,7 +513,7 @@ struct Sampler {
             }
         }
         cluster_barrier();
-        out.id = s.found_id;
+        const Limit out = {key_value(k_hi), s.found_id};
         cluster_barrier();    // (a faster CTA's next limit does not write into found_id yet)
         return out;
     }
@@ -403,108 +529,53 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleArgs 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const float* x = a.logits + (size_t)row * a.ld;
     const int lead = (int)(((uintptr_t)x >> 2) & 3);
-    const int lines = (int)(((long long)a.n + lead + 3) / 4);
+    const int lines = (a.n + lead + 3) / 4;
     const long long parts = (long long)ctas * SA_WARPS, part = (long long)rank * SA_WARPS + warp;
-    Sampler z{a, s, x, lead, (int)(lines * part / parts), (int)(lines * (part + 1) / parts), tid, warp, lane, rank, ctas, 0.f, 0.f, 0.0};
+    Sampler z{a, s, x, lead, (int)(lines * part / parts), (int)(lines * (part + 1) / parts), tid, warp, lane, rank, ctas, 0.f, 0.f, 0.f, 0.f};
     const float temp = a.temperature ? a.temperature[row] : 1.f;
     const int top_k = a.top_k ? a.top_k[row] : 0;
     const float top_p = a.top_p ? a.top_p[row] : 1.f, min_p = a.min_p ? fminf(a.min_p[row], 1.f) : 0.f;
     const bool greedy = !(temp > 0.f);
 
-    // ---- pass 1: largest and smallest logit, and the first place of the largest ----
-    float hi = -INFINITY, lo = INFINITY;
-    int at = 0x7fffffff;
-    z.each([&](int id, float l) {
-        if (l > hi) { hi = l; at = id; }           // (a thread meets its ids in ascending order)
-        if (l > -INFINITY) lo = fminf(lo, l);
-    });
+    // ---- the largest logit ----
+    float hi = -INFINITY;
+    z.each([&](int id, float l) { hi = fmaxf(hi, l); });
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float h = __shfl_xor_sync(0xffffffffu, hi, o);
-        const int i = __shfl_xor_sync(0xffffffffu, at, o);
-        if (h > hi || (h == hi && i < at)) { hi = h; at = i; }
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    }
-    if (lane == 0) { s.warp_f[warp] = hi; s.warp_g[warp] = lo; s.warp_b[warp] = (uint32_t)at; }
+    for (int o = 16; o > 0; o >>= 1) hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    if (lane == 0) s.warp_f[warp] = hi;
+    if (tid == 0) s.own_first = 0x7fffffff;
     __syncthreads();
     if (tid < ctas) {
-        for (int w = 0; w < SA_WARPS; ++w) {
-            const float h = s.warp_f[w];
-            const int i = (int)s.warp_b[w];
-            if (w == 0 || h > hi || (h == hi && i < at)) { hi = h; at = i; }
-            lo = w == 0 ? s.warp_g[w] : fminf(lo, s.warp_g[w]);
-        }
+        for (int w = 0; w < SA_WARPS; ++w) hi = fmaxf(hi, s.warp_f[w]);
         *in_cta(&s.top[rank], tid) = hi;
-        *in_cta(&s.low[rank], tid) = lo;
-        *in_cta(&s.first[rank], tid) = at;
     }
     cluster_barrier();
-    hi = -INFINITY; lo = INFINITY; at = 0x7fffffff;
-    for (uint32_t r = 0; r < ctas; ++r) {
-        const float h = s.top[r];
-        const int i = s.first[r];
-        if (h > hi || (h == hi && i < at)) { hi = h; at = i; }
-        lo = fminf(lo, s.low[r]);
-    }
+    hi = -INFINITY;
+    for (uint32_t r = 0; r < ctas; ++r) hi = fmaxf(hi, s.top[r]);
     z.top = hi;
     if (hi == -INFINITY) {    // nothing to draw from
         if (rank == 0 && tid == 0) {
             a.ids[row] = -1;
             if (a.logprobs) a.logprobs[row] = -INFINITY;
         }
-        cluster_barrier();
-        return;
+        return;               // (all CTAs of the row alike, and nobody reads remote memory any more)
     }
-    z.inv_temp = greedy ? 1.0 : 1.0 / (double)temp;
-    const float span = fminf(hi - lo, fmaxf(24.f, 32.f * temp));
-    z.inv_bin = span > 0.f && span < INFINITY ? (float)(SA_BINS - 1) / span : 0.f;
+    const double inv = greedy ? 1.0 : 1.4426950408889634 / (double)temp;
+    z.inv_temp = (float)inv;
+    z.inv_temp_rest = isinf(z.inv_temp) ? 0.f : (float)(inv - (double)z.inv_temp);
+    const float span = fmaxf(24.f, 32.f * temp);
+    z.inv_bin = span < INFINITY ? (float)(SA_BINS - 1) / span : 0.f;
 
     // ---- the limits; the first pass over all tokens also sums for the log-probability (temperature 1) ----
     bool want_lp = a.logprobs != nullptr;
     float lp = 0.f;
-    u64 sum = 0;
-    Sampler::Limit lim;
-    lim.key = order_key(-INFINITY) + 1;    // every token above -inf
-    lim.id = 0x7fffffff;
-    if (!greedy && top_k > 0) {
-        z.clear_bins();
-        z.each([&](int id, float l) {
-            if (l == -INFINITY) return;
-            if (want_lp) lp += expf(l == hi ? 0.f : l - hi);
-            z.add(z.bin(l), 0, false);
-        });
-        want_lp = false;
-        z.share_bins(false);
-        u64 tokens = 0;
-        for (int i = tid; i < SA_BINS; i += SA_THREADS) tokens += s.all_count[i];
-        if ((u64)top_k < z.block_sum(tokens)) lim = z.limit(false, (u64)top_k, 0.0, lim);
-    }
-    if (!greedy && top_p < 1.f) {
-        if (top_k > 0) cluster_barrier();   // (the others are through with this CTA's histogram)
-        z.clear_bins();
-        z.each([&](int id, float l) {
-            if (l == -INFINITY) return;
-            if (want_lp) lp += expf(l == hi ? 0.f : l - hi);
-            if (lim.holds(order_key(l), id)) z.add(z.bin(l), z.fixed(z.weight(l)), true);
-        });
-        want_lp = false;
-        z.share_bins(true);
-        u64 mass = 0;
-        for (int i = tid; i < SA_BINS; i += SA_THREADS) mass += s.all_mass[i];
-        // the first token is always inside: a target below one unit of weight is reached by it
-        lim = z.limit(true, 0, fmax((double)top_p * (double)z.block_sum(mass), 0.5), lim);
-    }
-    if (!greedy || want_lp) {
-        z.each([&](int id, float l) {
-            if (l == -INFINITY) return;
-            if (want_lp) lp += expf(l == hi ? 0.f : l - hi);
-            if (!greedy && lim.holds(order_key(l), id)) {
-                const float w = z.weight(l);
-                if (w >= min_p || l == hi) sum += z.fixed(w);
-            }
-        });
-    }
-    if (a.logprobs) {
+    auto add_lp = [&](float l) {
+        float e;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fminf(l - hi, 0.f) * 1.4426950408889634f));
+        lp += e;
+    };
+    // this CTA's sum into everybody's table; visible behind the next cluster barrier
+    auto share_lp = [&]() {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) lp += __shfl_xor_sync(0xffffffffu, lp, o);
         __syncthreads();
@@ -515,91 +586,179 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleArgs 
             for (int w = 0; w < SA_WARPS; ++w) t += s.warp_f[w];
             *in_cta(&s.lp[rank], tid) = t;
         }
+    };
+    auto store = [&](int token, float l) {
+        a.ids[row] = token;
+        if (a.logprobs) {
+            float t = 0.f;
+            for (uint32_t r = 0; r < ctas; ++r) t += s.lp[r];
+            a.logprobs[row] = fminf(l - hi, 0.f) - logf(t);
+        }
+    };
+    if (greedy) {
+        int at = 0x7fffffff;
+        if (want_lp)
+            z.each([&](int id, float l) { add_lp(l); if (l == hi) at = min(at, id); });
+        else
+            z.each([&](int id, float l) { if (l == hi) at = min(at, id); });
+        at = __reduce_min_sync(0xffffffffu, at);
+        if (lane == 0) atomicMin(&s.own_first, at);
+        if (want_lp) share_lp();
+        __syncthreads();
+        if (tid < ctas) *in_cta(&s.first[rank], tid) = s.own_first;
+        cluster_barrier();
+        if (rank == 0 && tid == 0) {
+            at = 0x7fffffff;
+            for (uint32_t r = 0; r < ctas; ++r) at = min(at, s.first[r]);
+            store(at, hi);
+        }
+        return;
+    }
+    const float u = a.u[row];
+    u64 sum = 0;
+    Limit lim = {-INFINITY, -1};           // every token above -inf
+    bool cut = false;
+    if (top_k > 0) {
+        z.clear_bins();
+        if (want_lp)
+            z.each([&](int id, float l) { add_lp(l); if (l > -INFINITY) atomicAdd(&s.lo[z.bin(l)], 1u); });
+        else
+            z.each([&](int id, float l) { if (l > -INFINITY) atomicAdd(&s.lo[z.bin(l)], 1u); });
+        if (want_lp) share_lp();
+        want_lp = false;
+        z.share_bins(false);
+        cut = (u64)top_k < z.bins_sum();
+        if (cut) {
+            u64 before = 0;
+            const int b = z.find_bin(false, (u64)top_k, 0.0, before);
+            if (before + s.all[b] <= SA_LIST) {
+                const uint32_t total = z.list([&](int id, float l) { return l > -INFINITY && z.bin(l) <= b; });
+                if (rank == 0) z.fetch_list();
+                cluster_barrier();
+                if (rank == 0) z.finish(total, (u64)top_k, top_p, 0, min_p, u, store);
+                return;
+            }
+            lim = z.limit(false, (u64)top_k, 0.0, lim, b, before);
+        }
+    }
+    if (top_p < 1.f) {
+        z.clear_bins();    // (the others read this CTA's histogram before the last barrier)
+        z.each([&](int id, float l) {
+            if (want_lp) add_lp(l);
+            if (!cut || lim.holds(l, id)) z.add(z.bin(l), z.fixed(z.weight(l)));
+        });
+        if (want_lp) share_lp();
+        want_lp = false;
+        z.share_bins(true);
+        // the first token is always inside: a target below one unit of weight is reached by it
+        const u64 mass = z.bins_sum();
+        const double target = fmax((double)top_p * (double)mass, 0.5);
+        u64 before = 0;
+        const int b = z.find_bin(true, 0, target, before);
+        // Every token down to bin b weighs at least what the bin's edge does, which bounds their number; of flat rows the bound is near the
+        // truth and far above the list's size: they do not try.
+        const float edge = z.weight(hi - (float)(b + 1) / z.inv_bin);
+        if (!cut && (double)(before + s.all[b]) <= 4.0 * SA_LIST * (double)z.fixed(edge)) {
+            const uint32_t total = z.list([&](int id, float l) { return l > -INFINITY && z.bin(l) <= b; });
+            if (total <= SA_LIST) {
+                if (rank == 0) z.fetch_list();
+                cluster_barrier();
+                if (rank == 0) z.finish(total, ~0ull, top_p, mass, min_p, u, store);
+                return;
+            }
+            cluster_barrier();    // (everybody has read the lists' lengths: the next ones may be written)
+        }
+        lim = z.limit(true, 0, target, lim, b, before);
+        cut = true;
+    }
+    if (cut) {
+        z.each([&](int id, float l) {
+            if (lim.holds(l, id)) {
+                const float w = z.weight(l);
+                if (w >= min_p || l == hi) sum += z.fixed(w);
+            }
+        });
+    } else {
+        z.each([&](int id, float l) {
+            if (want_lp) add_lp(l);
+            const float w = z.weight(l);
+            sum += w >= min_p || l == hi ? z.fixed(w) : 0;
+        });
+        if (want_lp) share_lp();
     }
 
     // ---- the draw ----
-    int token = at;
-    if (!greedy) {
-        u64 mine = sum;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-        __syncthreads();
-        if (lane == 0) s.warp_a[warp] = mine;
-        __syncthreads();
-        if (tid < ctas) {
-            u64 t = 0;
-            for (int w = 0; w < SA_WARPS; ++w) t += s.warp_a[w];
-            *in_cta(&s.kept[rank], tid) = t;
-        }
-        cluster_barrier();
-        u64 total = 0, before = 0;
-        for (uint32_t r = 0; r < ctas; ++r) {
-            if (r < rank) before += s.kept[r];
-            total += s.kept[r];
-        }
-        for (int w = 0; w < warp; ++w) before += s.warp_a[w];
-        const float u = a.u[row];
-        u64 draw = u > 0.f ? (u64)((double)u * (double)total) : 0;
-        draw = min(draw, total - 1);
-        if (before <= draw && draw < before + mine) {
-            // this warp's part holds the token: walk it in the order of the ids
-            bool done = false;
-            for (int v = z.v0; v < z.v1 && !done; v += 32) {
-                float l[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                if (v + lane < z.v1) z.line(v + lane, l);
-                u64 w[4], part_sum = 0;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int id = 4 * (v + lane) - lead + e;
-                    w[e] = 0;
-                    if (l[e] > -INFINITY && lim.holds(order_key(l[e]), id)) {
-                        const float f = z.weight(l[e]);
-                        if (f >= min_p || l[e] == hi) w[e] = z.fixed(f);
-                    }
-                    part_sum += w[e];
-                }
-                u64 upto = part_sum;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const u64 t = __shfl_up_sync(0xffffffffu, upto, o);
-                    if (lane >= o) upto += t;
-                }
-                u64 c = before + upto - part_sum;
-                if (c <= draw && draw < c + part_sum) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (c <= draw && draw < c + w[e]) {
-                            token = 4 * (v + lane) - lead + e;
-                            a.ids[row] = token;
-                            if (a.logprobs) {
-                                float t = 0.f;
-                                for (uint32_t r = 0; r < ctas; ++r) t += s.lp[r];
-                                a.logprobs[row] = (l[e] == hi ? 0.f : l[e] - hi) - logf(t);
-                            }
-                        }
-                        c += w[e];
-                    }
-                }
-                before += __shfl_sync(0xffffffffu, upto, 31);
-                done = before > draw;
-            }
-        }
-    } else {
-        cluster_barrier();
-        if (rank == 0 && tid == 0) {
-            a.ids[row] = token;
-            if (a.logprobs) {
-                float t = 0.f;
-                for (uint32_t r = 0; r < ctas; ++r) t += s.lp[r];
-                a.logprobs[row] = -logf(t);
-            }
-        }
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    __syncthreads();
+    if (lane == 0) s.warp_a[warp] = sum;
+    __syncthreads();
+    if (tid < ctas) {
+        u64 t = 0;
+        for (int w = 0; w < SA_WARPS; ++w) t += s.warp_a[w];
+        *in_cta(&s.kept[rank], tid) = t;
     }
-    cluster_barrier();    // nobody leaves while its shared memory may be read
+    cluster_barrier();
+    u64 total = 0, before = 0;
+    for (uint32_t r = 0; r < ctas; ++r) {
+        if (r < rank) before += s.kept[r];
+        total += s.kept[r];
+    }
+    u64 draw = u > 0.f ? (u64)((double)u * (double)total) : 0;
+    draw = min(draw, total - 1);
+    if (draw < before || draw >= before + s.kept[rank]) return;
+    // This CTA holds the token.  The part of the warp that holds it is dealt to all warps, then the warp of that share walks it in the order
+    // of the ids.
+    auto mass = [&](int id, float l) {
+        if (!lim.holds(l, id)) return (u64)0;
+        const float w = z.weight(l);
+        return w >= min_p || l == hi ? z.fixed(w) : 0;
+    };
+    int holder = 0;
+    while (before + s.warp_a[holder] <= draw) before += s.warp_a[holder++];
+    const long long p0 = lines * ((long long)rank * SA_WARPS + holder) / parts, p1 = lines * ((long long)rank * SA_WARPS + holder + 1) / parts;
+    const int w0 = (int)(p0 + (p1 - p0) * warp / SA_WARPS), w1 = (int)(p0 + (p1 - p0) * (warp + 1) / SA_WARPS);
+    u64 share = 0;
+    for (int v = w0 + lane; v < w1; v += 32) {
+        float l[4];
+        z.line(v, l);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) share += mass(4 * v - lead + e, l[e]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) share += __shfl_xor_sync(0xffffffffu, share, o);
+    if (lane == 0) s.warp_c[warp] = share;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) before += s.warp_c[w];
+    if (draw < before || draw >= before + share) return;
+    for (int v = w0; v < w1 && before <= draw; v += 32) {
+        float l[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (v + lane < w1) z.line(v + lane, l);
+        u64 w[4], here = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            w[e] = mass(4 * (v + lane) - lead + e, l[e]);
+            here += w[e];
+        }
+        u64 upto = here;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 t = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += t;
+        }
+        u64 c = before + upto - here;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (c <= draw && draw < c + w[e]) store(4 * (v + lane) - lead + e, l[e]);
+            c += w[e];
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
 }
 
 int sample_setup(dsuf_ctx* ctx) {
     cudaError_t e = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SampleShared));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(sample_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);   // clusters of 16
     return e == cudaSuccess ? DSUF_OK : cuda_fail(ctx, e, "cudaFuncSetAttribute(sample)");
 }
 
