@@ -375,7 +375,6 @@ __global__ void __launch_bounds__(AD_THREADS, 2) attn_decode_kernel(const Decode
                     const bool va = ta >= at.beg && ta < at.len, vb = tb >= at.beg && tb < at.len;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        // (scale may be negative: the hidden score is -inf after the scaling below)
                         st[nt][0] = va ? st[nt][0] * sl2 : -INFINITY;
                         st[nt][1] = va ? st[nt][1] * sl2 : -INFINITY;
                         st[nt][2] = vb ? st[nt][2] * sl2 : -INFINITY;
@@ -627,7 +626,7 @@ int32_t dsuf_attn_decode(dsuf_ctx* ctx, void* stream, const dsuf_kv_cache* cache
                  q_heads, cache->kv_heads);
     DSUF_REQUIRE(ctx, ldq >= q_heads * D && ldq % 8 == 0 && ldo >= q_heads * D && ldo % 8 == 0,
                  "attn_decode: ldq and ldo must be multiples of 8 and hold q_heads * head_dim elements");
-    DSUF_REQUIRE(ctx, window >= 0 && scale == scale && scale - scale == 0.f, "attn_decode: window must be >= 0 and scale finite");
+    DSUF_REQUIRE(ctx, window >= 0 && scale > 0.f && scale - scale == 0.f, "attn_decode: window must be >= 0, scale positive and finite");
     if (b == 0) return DSUF_OK;
     DSUF_REQUIRE(ctx, q && out && block_table && seq_lens && workspace && (q & 15) == 0 && (out & 15) == 0 && (block_table & 3) == 0 &&
                  (seq_lens & 3) == 0 && (lse & 3) == 0 && (workspace & 15) == 0, "attn_decode: null or misaligned pointer (q, out, workspace 16 bytes, indexes and lse 4)");

@@ -9,12 +9,14 @@
 // and has one causal boundary (an odd group pairs the last head of a block with the first of the next).  Roles:
 //   warps 0-3, 4-7   softmax of tile 0 / 1: a thread owns a row; scores from tensor memory, p back to tensor memory
 //   warp 8           TMA: query tiles, and a ring of key / value tiles (K0 V0 K1 V1 ...)
-//   warp 9           tcgen05.mma: S_t = Q_t K^T (operands in shared memory), O_t += P_t V (P in tensor memory, V as it lies,
-//                    tokens by columns, through the MN-major operand form)
-// The issue order P0 V, S0, P1 V, S1 keeps the tensor core on one tile while the other tile's softmax runs; S of step j + 1 is issued
-// behind PV of step j, so its completion also says that the output may be rescaled.  The steps of successive pairs form one stream: the
-// next pair's first scores are issued before the last output is stored.
-//
+//   warp 9, 10       tcgen05.mma of tile 0 / 1: S_t = Q_t K^T (operands in shared memory), O_t += P_t V (P in tensor memory, V as it
+//                    lies, tokens by columns, through the MN-major operand form)
+// The tensor core works on one tile while the other tile's softmax runs; S of step j + 1 is issued behind PV of step j, so its
+// completion also says that the output may be rescaled.  The steps of successive pairs form one stream: the next pair's first scores are
+// issued before the last output is stored.  The two issuing warps take strict turns (P0 V, S0, P1 V, S1): issuing blocks while the tensor
+// core's short queue is full, so the barrier waits of one tile (100 cycles and more each, even when met) have to pass while the
+// other's products are issued; without turns the tiles fall into step, and both softmaxes share the exponential unit and then both wait.
+// (8192 tokens, 56 / 8 heads of 128: one issuing warp 867 us, two without turns 1022, two with turns 778.)
 // Tensor memory (512 columns): S0 S1 (128 fp32 columns each; P_t overwrites the first 64 of S_t as packed bf16), O0 O1 (D each).
 // The reference point of a row only moves when a score exceeds it by 2^8 (exact: the sum and the output share it), which makes
 // rescaling rare after the first tile.  p is rounded once to bf16 as operand; sums, statistics and outputs are fp32.
@@ -27,7 +29,7 @@
 namespace dsuf {
 
 constexpr int KID_PROMPT = 9;
-constexpr int PA_THREADS = 320;
+constexpr int PA_THREADS = 352;
 constexpr int PA_BM = 128;
 constexpr float PA_UNSET = -1e30f;
 constexpr float PA_TRIGGER = 8.f;
@@ -36,8 +38,9 @@ template <int D>
 struct PromptShape {
     static constexpr int BOXES = D / 64;                       // 128-byte wide operand boxes of a tile
     static constexpr int TILE = PA_BM * D * 2;                 // bytes of a query, key or value tile
-    static constexpr int STAGES = D == 128 ? 5 : 8;            // ring of key / value tiles
-    static constexpr int SMEM = 2 * TILE + STAGES * TILE + 1024;
+    static constexpr int STAGES = D == 128 ? 4 : 8;            // ring of key / value tiles
+    static constexpr int OUT = 32 * 128;                       // a warp's staging for its output: 32 rows of 64 columns
+    static constexpr int SMEM = 2 * TILE + STAGES * TILE + 8 * OUT + 1024;
 };
 
 struct PromptArgs {
@@ -98,13 +101,25 @@ DSUF_DEV uint32_t pa_pack(float lo, float hi) {
     return r;
 }
 
-// A pair of query tiles: tile t covers rows [qb[t] * 128, ..) of the sequence, query head head[t], key tiles [lo[t], hi[t]).
+// A query tile: rows [qb * 128, ..) of the sequence, query head, key tiles [lo, hi) (hi = 0: no tile).
+struct PromptTile {
+    int qb, head, lo, hi;
+    DSUF_DEV bool active(int j) const { return j >= lo && j < hi; }
+};
+// A pair of them, of sequence rows start .. start + len - 1; together they need the key tiles [jlo, jhi).
 struct PromptPair {
     int start, len, kvh;
-    int qb[2], head[2], lo[2], hi[2];
+    PromptTile t0, t1;
     int jlo, jhi;
     bool ok;
-    DSUF_DEV bool active(int t, int j) const { return j >= lo[t] && j < hi[t]; }
+    DSUF_DEV PromptTile tile(int t) const {     // (selects, so that the pair stays in registers)
+        PromptTile r;
+        r.qb = t ? t1.qb : t0.qb;
+        r.head = t ? t1.head : t0.head;
+        r.lo = t ? t1.lo : t0.lo;
+        r.hi = t ? t1.hi : t0.hi;
+        return r;
+    }
 };
 
 // Walks the pairs of one CTA: row r of the deal takes index r * grid + c, or counted from the other end in odd rows.  A whole warp calls
@@ -120,6 +135,14 @@ struct PromptWalk {
             start = min(max(__ldg(a.cu + s), 0), a.t);
             len = max(min(max(__ldg(a.cu + s + 1), 0), a.t) - start, 0);
         }
+    }
+    DSUF_DEV PromptTile tile(int it, int tiles, int kvh) const {
+        PromptTile t;
+        t.qb = it / a.group;
+        t.head = kvh * a.group + it % a.group;
+        t.hi = it < tiles ? t.qb + 1 : 0;
+        t.lo = it < tiles && a.window > 0 ? max(0, t.qb * PA_BM - a.window + 1) / PA_BM : 0;
+        return t;
     }
     DSUF_DEV PromptPair next() {
         const int lane = threadIdx.x & 31;
@@ -147,21 +170,10 @@ struct PromptWalk {
                 const int rank = local / a.kv_heads;
                 p.kvh = local % a.kv_heads;
                 const int pair = (tiles + 1) / 2 - 1 - rank;
-                p.jlo = 0x7fffffff;
-                p.jhi = 0;
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const int it = 2 * pair + t;
-                    p.qb[t] = it / a.group;
-                    p.head[t] = p.kvh * a.group + it % a.group;
-                    p.lo[t] = p.hi[t] = 0;
-                    if (it < tiles) {
-                        p.hi[t] = p.qb[t] + 1;
-                        p.lo[t] = a.window > 0 ? max(0, p.qb[t] * PA_BM - a.window + 1) / PA_BM : 0;
-                        p.jlo = min(p.jlo, p.lo[t]);
-                        p.jhi = max(p.jhi, p.hi[t]);
-                    }
-                }
+                p.t0 = tile(2 * pair, tiles, p.kvh);
+                p.t1 = tile(2 * pair + 1, tiles, p.kvh);
+                p.jlo = p.t0.lo;                              // (the second tile's rows are the same or later ones)
+                p.jhi = max(p.t0.hi, p.t1.hi);
                 p.ok = true;
                 return p;
             }
@@ -170,6 +182,49 @@ struct PromptWalk {
         return p;
     }
 };
+
+// One row's 128 scores in chunks of 32 columns, the next chunk's load under way while `f(chunk, values)` works on one.
+template <typename F>
+DSUF_DEV void pa_chunks(uint32_t tS, F f) {
+    float s[2][32];
+    tmem_ld_issue<32>(tS, s[0]);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        tmem_wait_ld();
+        if (c < 3) tmem_ld_issue<32>(tS + (c + 1) * 32, s[(c + 1) & 1]);
+        f(c, s[c & 1]);
+    }
+}
+// p = 2^(s sl2 - ref) of a row, packed to bf16 in w, their sum and the largest visible score.  MASK 0: all columns are visible, 1: those up
+// to `upper`, 2: those above `lower` as well.  (Moving a part of the exponentials to the fp32 pipe, as a polynomial of degree 4, made the
+// kernel slower: a third of them 957 us instead of 867 at 8192 tokens; the exponential unit is not what the row waits for.)
+template <int MASK>
+DSUF_DEV void pa_weights(uint32_t tS, float sl2, float ref, int upper, int lower, uint32_t* w, float& part, float& top) {
+    const unsigned long long scale2 = pack_f32x2(sl2, sl2), ref2 = pack_f32x2(-ref, -ref);
+    unsigned long long sum2 = pack_f32x2(0.f, 0.f);
+    pa_chunks(tS, [&](int c, float* s) {
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+            if constexpr (MASK > 0) {
+                const int col = c * 32 + e;
+                s[e] = col <= upper && (MASK < 2 || col > lower) ? s[e] : -INFINITY;
+                s[e + 1] = col + 1 <= upper && (MASK < 2 || col + 1 > lower) ? s[e + 1] : -INFINITY;
+            }
+            top = fmaxf(top, fmaxf(s[e], s[e + 1]));
+            unsigned long long v;
+            asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(pack_f32x2(s[e], s[e + 1])), "l"(scale2), "l"(ref2));
+            float x, y;
+            asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+            x = pa_exp2(x);
+            y = pa_exp2(y);
+            asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sum2) : "l"(pack_f32x2(x, y)));
+            w[c * 16 + e / 2] = pa_pack(x, y);
+        }
+    });
+    float x, y;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(sum2));
+    part = x + y;
+}
 
 template <int D>
 __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid_constant__ PromptArgs a) {
@@ -183,7 +238,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     bool dead = false;
 
-    if (warp == 9) {
+    if (warp == 8) {
         tmem_alloc(&s_tmem, 512);
         tmem_relinquish();
     }
@@ -197,7 +252,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
         }
         for (int s = 0; s < S::STAGES; ++s) {
             mbar_init(&kv_full[s], 1);
-            mbar_init(&kv_empty[s], 1);
+            mbar_init(&kv_empty[s], 2);
         }
         mbar_fence_init();
     }
@@ -237,13 +292,14 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
             kv(p, &a.tm_k, p.jlo);   // ahead of the queries: their buffers become free later than the ring's
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                if (p.hi[t] == 0) continue;
+                const PromptTile q = t ? p.t1 : p.t0;
+                if (q.hi == 0) continue;
                 if (qn[t] > 0 && !dead && !mbar_wait(&q_empty[t], (qn[t] - 1) & 1, a.status, KID_PROMPT, 2)) dead = true;
                 if (warp_elect()) {
                     mbar_expect_tx(&q_full[t], S::TILE);
 #pragma unroll
                     for (int b = 0; b < S::BOXES; ++b)
-                        tma_2d_nh(base + t * S::TILE + b * BOX, &a.tm_q, p.head[t] * D + b * 64, p.start + p.qb[t] * PA_BM, &q_full[t]);
+                        tma_2d_nh(base + t * S::TILE + b * BOX, &a.tm_q, q.head * D + b * 64, p.start + q.qb * PA_BM, &q_full[t]);
                 }
                 __syncwarp();
                 ++qn[t];
@@ -253,18 +309,22 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
                 kv(p, &a.tm_v, j);
             }
         }
-    } else if (warp == 9) {
-        // ---------------- tensor core issuer ----------------
-        const uint32_t tmu = warp_uniform(tm);
-        const uint64_t qd0 = warp_uniform(tc_smem_desc(base, 16, 1024, TC_SWIZZLE_128B));
-        const uint64_t kd0 = warp_uniform(tc_smem_desc(ring, 16, 1024, TC_SWIZZLE_128B));
-        const uint64_t vd0 = warp_uniform(tc_smem_desc(ring, BOX, 1024, TC_SWIZZLE_128B));   // column chunks of 64 a box apart, 8 tokens 1024 bytes
+    } else if (warp >= 9) {
+        // ---------------- tensor core issuer of tile t ----------------
+        const int t = warp - 9;
+        const uint32_t tmS = warp_uniform(tm + t * 128), tmO = warp_uniform(tm + 256 + t * D);
+        // operand descriptors: the address is in the low word, so steps are 32-bit additions
+        const uint64_t kmajor = tc_smem_desc(base, 16, 1024, TC_SWIZZLE_128B);
+        const uint32_t desc_hi = warp_uniform((uint32_t)(kmajor >> 32)), q_lo = warp_uniform((uint32_t)kmajor + ((t * S::TILE) >> 4));
+        const uint32_t ring_lo = warp_uniform((uint32_t)tc_smem_desc(ring, 16, 1024, TC_SWIZZLE_128B));
+        const uint32_t ring_lo_v = warp_uniform((uint32_t)tc_smem_desc(ring, BOX, 1024, TC_SWIZZLE_128B));   // column chunks of 64 a box apart, 8 tokens 1024 bytes
         int st = 0;
-        uint32_t ph = 0, qn[2] = {0, 0}, pn[2] = {0, 0};
+        uint32_t ph = 0, qn = 0, pn = 0;
         auto wait_kv = [&]() {
             if (!dead && !mbar_wait(&kv_full[st], ph, a.status, KID_PROMPT, 3)) dead = true;
             tc_fence_after();
         };
+        // the stage is free once what this warp has issued is done, and the other tile's warp says the same
         auto release_kv = [&](int stage) {
             if (warp_elect()) tc_commit(&kv_empty[stage]);
             __syncwarp();
@@ -272,43 +332,62 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
         auto advance = [&]() {
             if (++st == S::STAGES) { st = 0; ph ^= 1; }
         };
-        auto scores = [&](const PromptPair& p, int t, int j, int stage) {
-            if (j == p.lo[t]) {
-                if (!dead && !mbar_wait(&q_full[t], qn[t] & 1, a.status, KID_PROMPT, 4)) dead = true;
-                ++qn[t];
+        auto desc = [&](uint32_t lo) { return ((uint64_t)desc_hi << 32) | lo; };
+        // the turn, handed to and fro on two named barriers; both warps walk the same steps, so every arrival is awaited
+        auto take_turn = [&]() { named_bar_sync(2 + t, 64); };
+        auto pass_turn = [&]() { named_bar_arrive(2 + (t ^ 1), 64); };
+        auto wait_q = [&](const PromptTile& q, int j) {
+            if (j == q.lo) {
+                if (!dead && !mbar_wait(&q_full[t], qn & 1, a.status, KID_PROMPT, 4)) dead = true;
+                ++qn;
                 tc_fence_after();
             }
+        };
+        auto scores = [&](const PromptTile& q, int j, uint32_t k_lo) {
+            const bool last = j == q.hi - 1;
             if (warp_elect()) {
 #pragma unroll
                 for (int c = 0; c < D / 16; ++c) {
                     const uint32_t off = (uint32_t)((c >> 2) * BOX + (c & 3) * 32) >> 4;
-                    pa_mma_ss(tmu + t * 128, qd0 + (uint64_t)((t * S::TILE) >> 4) + off, kd0 + (uint64_t)((stage * S::TILE) >> 4) + off, pa_idesc(128, false), c != 0);
+                    pa_mma_ss(tmS, desc(q_lo + off), desc(k_lo + off), pa_idesc(128, false), c != 0);
                 }
                 tc_commit(&s_full[t]);
-                if (j == p.hi[t] - 1) tc_commit(&q_empty[t]);
+                if (last) tc_commit(&q_empty[t]);
             }
             __syncwarp();
         };
+        if (t == 1) pass_turn();     // tile 0 begins
         PromptPair cur = walk.next();
+        PromptTile mine = cur.tile(t);
         if (cur.ok) {
             wait_kv();
-            for (int t = 0; t < 2; ++t)
-                if (cur.active(t, cur.jlo)) scores(cur, t, cur.jlo, st);
+            const uint32_t k_lo = warp_uniform(ring_lo + ((st * S::TILE) >> 4));
+            const bool go = mine.active(cur.jlo);
+            if (go) wait_q(mine, cur.jlo);
+            take_turn();
+            if (go) scores(mine, cur.jlo, k_lo);
+            pass_turn();
             release_kv(st);
             advance();
         }
         while (cur.ok) {
             PromptPair nxt = cur;
+            PromptTile then = mine;      // what the next step's scores belong to
             for (int j = cur.jlo; j < cur.jhi; ++j) {
                 const bool last = j + 1 == cur.jhi;
-                if (last) nxt = walk.next();
+                if (last) {
+                    nxt = walk.next();
+                    then = nxt.tile(t);
+                }
                 const bool more = nxt.ok;
                 const int nj = last ? nxt.jlo : j + 1;
+                const bool here = mine.active(j), next = more && then.active(nj);
                 wait_kv();
                 const int vst = st;
                 advance();
                 const int behind = cur.len - j * PA_BM;      // rows of this tile inside the sequence
-                if (behind < PA_BM) {
+                if (here && behind < PA_BM) {
+                    // (both tiles' warps may write these zeros, the second while the first one's product reads them)
                     for (int i = lane; i < (PA_BM - behind) * 8 * S::BOXES; i += 32) {
                         const int b = i / ((PA_BM - behind) * 8), r = i % ((PA_BM - behind) * 8);
                         *reinterpret_cast<uint4*>(ring + vst * S::TILE + b * BOX + behind * 128 + r * 16) = make_uint4(0, 0, 0, 0);
@@ -316,28 +395,26 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
                     fence_proxy_async();
                     __syncwarp();
                 }
-                bool k_here = false;
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    if (cur.active(t, j)) {
-                        if (!dead && !mbar_wait(&p_full[t], pn[t] & 1, a.status, KID_PROMPT, 5)) dead = true;
-                        ++pn[t];
-                        tc_fence_after();
-                        if (warp_elect()) {
-#pragma unroll
-                            for (int c = 0; c < PA_BM / 16; ++c)
-                                pa_mma_ts(tmu + 256 + t * D, tmu + t * 128 + c * 8, vd0 + (uint64_t)((vst * S::TILE + c * 2048) >> 4), pa_idesc(D, true),
-                                          j > cur.lo[t] || c != 0);
-                            if (j == cur.hi[t] - 1) tc_commit(&o_full[t]);
-                        }
-                        __syncwarp();
-                    }
-                    if (more && nxt.active(t, nj)) {
-                        if (!k_here) wait_kv();
-                        k_here = true;
-                        scores(nxt, t, nj, st);
-                    }
+                const uint32_t v_lo = warp_uniform(ring_lo_v + ((vst * S::TILE) >> 4)), k_lo = warp_uniform(ring_lo + ((st * S::TILE) >> 4));
+                const bool first = j == mine.lo, end = j == mine.hi - 1;
+                if (more) wait_kv();
+                if (next) wait_q(then, nj);
+                if (here) {
+                    if (!dead && !mbar_wait(&p_full[t], pn & 1, a.status, KID_PROMPT, 5)) dead = true;
+                    ++pn;
+                    tc_fence_after();
                 }
+                take_turn();
+                if (here) {
+                    if (warp_elect()) {
+#pragma unroll
+                        for (int c = 0; c < PA_BM / 16; ++c) pa_mma_ts(tmO, tmS + c * 8, desc(v_lo + c * 128), pa_idesc(D, true), c != 0 || !first);
+                        if (end) tc_commit(&o_full[t]);
+                    }
+                    __syncwarp();
+                }
+                if (next) scores(then, nj, k_lo);
+                pass_turn();
                 release_kv(vst);
                 if (more) {
                     release_kv(st);
@@ -345,7 +422,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
                 }
             }
             cur = nxt;
+            mine = then;
         }
+        if (t == 0) take_turn();     // (the last turn that tile 1 has passed on)
     } else {
         // ---------------- softmax: tile t, one row per thread ----------------
         const int t = warp >> 2;
@@ -353,41 +432,43 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
         const uint32_t tS = tm + lanes + t * 128, tO = tm + lanes + 256 + t * D;
         const int r = (warp & 3) * 32 + lane;        // row inside the tile
         const float sl2 = a.scale_log2;
+        uint8_t* stage = ring + S::STAGES * S::TILE + warp * S::OUT;
         uint32_t sn = 0, on = 0;
         for (;;) {
             const PromptPair p = walk.next();
             if (!p.ok) break;
-            if (p.hi[t] == 0) continue;
-            const int row = p.qb[t] * PA_BM + r;
+            const PromptTile q = p.tile(t);
+            if (q.hi == 0) continue;
+            const int row = q.qb * PA_BM + r;
             float ref = PA_UNSET, sum = 0.f;
-            for (int j = p.lo[t]; j < p.hi[t]; ++j) {
+            for (int j = q.lo; j < q.hi; ++j) {
                 if (!dead && !mbar_wait(&s_full[t], sn & 1, a.status, KID_PROMPT, 6)) dead = true;
                 ++sn;
                 tc_fence_after();
-                float s[128];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld_issue<32>(tS + c * 32, s + c * 32);
-                tmem_wait_ld();
                 const int upper = row - j * PA_BM;                                  // last visible column of the tile
                 const int lower = a.window > 0 ? upper - a.window : -1;             // last column hidden by the window
-                if (j == p.hi[t] - 1 || (a.window > 0 && p.qb[t] * PA_BM + PA_BM - 1 - j * PA_BM >= a.window)) {
+                const bool windowed = a.window > 0 && q.qb * PA_BM + PA_BM - 1 - j * PA_BM >= a.window, diagonal = j == q.hi - 1;
+                uint32_t w[64];
+                float part, top = -INFINITY;
+                if (j == q.lo) {
+                    // the first tile's reference: the largest of 32 scores (every row sees column 0, but for a window)
+                    float s[32];
+                    tmem_ld<32>(tS, s);
 #pragma unroll
-                    for (int c = 0; c < 128; ++c) s[c] = c <= upper && c > lower ? s[c] * sl2 : -INFINITY;
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 128; c += 2) mul_f32x2(s[c], s[c + 1], sl2, sl2);
+                    for (int e = 0; e < 32; ++e) top = fmaxf(top, e <= upper && e > lower ? s[e] : -INFINITY);
+                    ref = fmaxf(top * sl2, PA_UNSET);
                 }
-                float top = fmaxf(s[0], s[1]);
-#pragma unroll
-                for (int c = 2; c < 128; c += 2) top = fmaxf(top, fmaxf(s[c], s[c + 1]));
-                const bool over = top > ref + PA_TRIGGER;
-                if (__any_sync(0xffffffffu, over)) {
-                    const float to = over ? top : ref;
+                // exponentials against the reference as it is, while the maximum is only looked at for whether it may stay
+                if (windowed) pa_weights<2>(tS, sl2, ref, upper, lower, w, part, top);
+                else if (diagonal) pa_weights<1>(tS, sl2, ref, upper, lower, w, part, top);
+                else pa_weights<0>(tS, sl2, ref, upper, lower, w, part, top);
+                if (!__all_sync(0xffffffffu, top * sl2 <= ref + PA_TRIGGER)) {
+                    // (seldom) the reference moves; so do the sum and the output, which is complete: this step's scores were issued behind the
+                    // last step's product
+                    const float to = top * sl2 > ref + PA_TRIGGER ? top * sl2 : ref;
                     const float by = pa_exp2(ref - to);
-                    ref = to;
-                    sum *= by;
-                    if (j > p.lo[t]) {   // (this step's scores were issued behind the last step's product: the output is complete)
-#pragma unroll
+                    if (j > q.lo) {
+#pragma unroll 1
                         for (int c = 0; c < D; c += 16) {
                             float o[16];
                             tmem_ld<16>(tO + c, o);
@@ -396,21 +477,13 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
                             tmem_st16(tO + c, reinterpret_cast<const uint32_t*>(o));
                         }
                     }
+                    ref = to;
+                    sum *= by;
+                    pa_weights<2>(tS, sl2, ref, upper, lower, w, part, top);
                 }
-                float part[2] = {0.f, 0.f};
+                sum += part;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t w[16];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float x = pa_exp2(s[c * 32 + 2 * e] - ref), y = pa_exp2(s[c * 32 + 2 * e + 1] - ref);
-                        part[0] += x;
-                        part[1] += y;
-                        w[e] = pa_pack(x, y);
-                    }
-                    tmem_st16(tS + c * 16, w);
-                }
-                sum += part[0] + part[1];
+                for (int c = 0; c < 4; ++c) tmem_st16(tS + c * 16, w + c * 16);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -421,26 +494,38 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
             tc_fence_after();
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
             const bool live = row < p.len;
-            bf16* dst = a.out + (size_t)(p.start + row) * a.ldo + (size_t)p.head[t] * D;
+            // through shared memory, so that a store instruction writes four rows of 128 bytes instead of 32 pieces of 16
+            const int row0 = q.qb * PA_BM + (warp & 3) * 32;      // the warp's first row
 #pragma unroll
-            for (int c = 0; c < D; c += 32) {
-                float o[32];
-                tmem_ld<32>(tO + c, o);
-                if (live) {
+            for (int c = 0; c < D; c += 64) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float o[32];
+                    tmem_ld<32>(tO + c + h * 32, o);
 #pragma unroll
                     for (int e = 0; e < 32; e += 8)
-                        *reinterpret_cast<uint4*>(dst + c + e) = make_uint4(pa_pack(o[e] * inv, o[e + 1] * inv), pa_pack(o[e + 2] * inv, o[e + 3] * inv),
-                                                                            pa_pack(o[e + 4] * inv, o[e + 5] * inv), pa_pack(o[e + 6] * inv, o[e + 7] * inv));
+                        *reinterpret_cast<uint4*>(stage + lane * 128 + ((((h * 32 + e) / 8) ^ (lane & 7)) << 4)) =
+                            make_uint4(pa_pack(o[e] * inv, o[e + 1] * inv), pa_pack(o[e + 2] * inv, o[e + 3] * inv),
+                                       pa_pack(o[e + 4] * inv, o[e + 5] * inv), pa_pack(o[e + 6] * inv, o[e + 7] * inv));
                 }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int rr = i * 4 + (lane >> 3), cc = lane & 7;
+                    if (row0 + rr < p.len)
+                        *reinterpret_cast<uint4*>(a.out + (size_t)(p.start + row0 + rr) * a.ldo + (size_t)q.head * D + c + cc * 8) =
+                            *reinterpret_cast<const uint4*>(stage + rr * 128 + ((cc ^ (rr & 7)) << 4));
+                }
+                __syncwarp();
             }
-            if (live && a.lse) a.lse[(size_t)(p.start + row) * a.q_heads + p.head[t]] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
+            if (live && a.lse) a.lse[(size_t)(p.start + row) * a.q_heads + q.head] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
             tc_fence_before();
         }
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 9) tmem_dealloc(tm, 512);
+    if (warp == 8) tmem_dealloc(tm, 512);
 }
 
 static int encode_heads(dsuf_ctx* ctx, CUtensorMap* tm, const void* base, long long width, long long ld, long long rows) {
@@ -474,7 +559,7 @@ extern "C" int32_t dsuf_attn_prompt(dsuf_ctx* ctx, void* stream, uint64_t q, int
     DSUF_REQUIRE(ctx, t >= 0 && t <= 0x7fff0000 && n_seqs >= 0, "attn_prompt: t must be in 0..2^31 - 65536 and n_seqs >= 0");
     DSUF_REQUIRE(ctx, ldq >= q_heads * head_dim && ldq % 8 == 0 && ldo >= q_heads * head_dim && ldo % 8 == 0 && ldk >= kv_heads * head_dim && ldk % 8 == 0 &&
                  ldv >= kv_heads * head_dim && ldv % 8 == 0, "attn_prompt: row strides must be multiples of 8 and hold all heads");
-    DSUF_REQUIRE(ctx, window >= 0 && scale == scale && scale - scale == 0.f, "attn_prompt: window must be >= 0 and scale finite");
+    DSUF_REQUIRE(ctx, window >= 0 && scale > 0.f && scale - scale == 0.f, "attn_prompt: window must be >= 0, scale positive and finite");
     if (t == 0 || n_seqs == 0) return DSUF_OK;
     DSUF_REQUIRE(ctx, q && k && v && out && cu_seqlens && (q & 15) == 0 && (k & 15) == 0 && (v & 15) == 0 && (out & 15) == 0 && (cu_seqlens & 3) == 0 &&
                  (lse & 3) == 0, "attn_prompt: null or misaligned pointer (q, k, v, out 16 bytes, cu_seqlens and lse 4)");
