@@ -18,8 +18,9 @@
 // other's products are issued; without turns the tiles fall into step, and both softmaxes share the exponential unit and then both wait.
 // (8192 tokens, 56 / 8 heads of 128: one issuing warp 867 us, two without turns 1022, two with turns 778.)
 // Tensor memory (512 columns): S0 S1 (128 fp32 columns each; P_t overwrites the first 64 of S_t as packed bf16), O0 O1 (D each).
-// The reference point of a row only moves when a score exceeds it by 2^8 (exact: the sum and the output share it), which makes
-// rescaling rare after the first tile.  p is rounded once to bf16 as operand; sums, statistics and outputs are fp32.
+// The reference point of a row is the largest of its first 32 scores and only moves when a tile's weights add up to more than 2^24 (exact: the
+// sum and the output share the reference, and bf16's and fp32's precision does not depend on the magnitude), so usual tiles need no maximum at
+// all.  p is rounded once to bf16 as operand; sums, statistics and outputs are fp32.
 //
 // Pairs are ordered from the longest rows to the shortest inside a sequence and dealt to the CTAs back and forth, so that a CTA's
 // long and short pairs balance.  Values behind a sequence's end inside its last tile belong to another sequence (or nobody) and are
@@ -32,7 +33,7 @@ constexpr int KID_PROMPT = 9;
 constexpr int PA_THREADS = 352;
 constexpr int PA_BM = 128;
 constexpr float PA_UNSET = -1e30f;
-constexpr float PA_TRIGGER = 8.f;
+constexpr float PA_TRIGGER = 16777216.f;
 
 template <int D>
 struct PromptShape {
@@ -195,26 +196,25 @@ DSUF_DEV void pa_chunks(uint32_t tS, F f) {
         f(c, s[c & 1]);
     }
 }
-// p = 2^(s sl2 - ref) of a row, packed to bf16 in w, their sum and the largest visible score.  MASK 0: all columns are visible, 1: those up
-// to `upper`, 2: those above `lower` as well.  (Moving a part of the exponentials to the fp32 pipe, as a polynomial of degree 4, made the
-// kernel slower: a third of them 957 us instead of 867 at 8192 tokens; the exponential unit is not what the row waits for.)
+DSUF_DEV bool pa_seen(int col, int upper, int lower) { return col <= upper && col > lower; }
+// p = 2^(s sl2 - ref) of a row, packed to bf16 in w, and their sum.  MASK 0: all columns are visible, 1: those up to `upper`, 2: those above
+// `lower` as well.
 template <int MASK>
-DSUF_DEV void pa_weights(uint32_t tS, float sl2, float ref, int upper, int lower, uint32_t* w, float& part, float& top) {
+DSUF_DEV float pa_weights(uint32_t tS, float sl2, float ref, int upper, int lower, uint32_t* w) {
     const unsigned long long scale2 = pack_f32x2(sl2, sl2), ref2 = pack_f32x2(-ref, -ref);
     unsigned long long sum2 = pack_f32x2(0.f, 0.f);
     pa_chunks(tS, [&](int c, float* s) {
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
-            if constexpr (MASK > 0) {
-                const int col = c * 32 + e;
-                s[e] = col <= upper && (MASK < 2 || col > lower) ? s[e] : -INFINITY;
-                s[e + 1] = col + 1 <= upper && (MASK < 2 || col + 1 > lower) ? s[e + 1] : -INFINITY;
-            }
-            top = fmaxf(top, fmaxf(s[e], s[e + 1]));
             unsigned long long v;
             asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(pack_f32x2(s[e], s[e + 1])), "l"(scale2), "l"(ref2));
             float x, y;
             asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+            if constexpr (MASK > 0) {
+                const int col = c * 32 + e;
+                x = pa_seen(col, upper, MASK > 1 ? lower : -1) ? x : -INFINITY;
+                y = pa_seen(col + 1, upper, MASK > 1 ? lower : -1) ? y : -INFINITY;
+            }
             x = pa_exp2(x);
             y = pa_exp2(y);
             asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sum2) : "l"(pack_f32x2(x, y)));
@@ -223,7 +223,7 @@ DSUF_DEV void pa_weights(uint32_t tS, float sl2, float ref, int upper, int lower
     });
     float x, y;
     asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(sum2));
-    part = x + y;
+    return x + y;
 }
 
 template <int D>
@@ -434,11 +434,15 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
         const float sl2 = a.scale_log2;
         uint8_t* stage = ring + S::STAGES * S::TILE + warp * S::OUT;
         uint32_t sn = 0, on = 0;
+        PromptPair ahead = walk.next();
         for (;;) {
-            const PromptPair p = walk.next();
+            const PromptPair p = ahead;
             if (!p.ok) break;
             const PromptTile q = p.tile(t);
-            if (q.hi == 0) continue;
+            if (q.hi == 0) {
+                ahead = walk.next();
+                continue;
+            }
             const int row = q.qb * PA_BM + r;
             float ref = PA_UNSET, sum = 0.f;
             for (int j = q.lo; j < q.hi; ++j) {
@@ -449,23 +453,30 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
                 const int lower = a.window > 0 ? upper - a.window : -1;             // last column hidden by the window
                 const bool windowed = a.window > 0 && q.qb * PA_BM + PA_BM - 1 - j * PA_BM >= a.window, diagonal = j == q.hi - 1;
                 uint32_t w[64];
-                float part, top = -INFINITY;
                 if (j == q.lo) {
                     // the first tile's reference: the largest of 32 scores (every row sees column 0, but for a window)
-                    float s[32];
+                    float s[32], top = -INFINITY;
                     tmem_ld<32>(tS, s);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) top = fmaxf(top, e <= upper && e > lower ? s[e] : -INFINITY);
+                    for (int e = 0; e < 32; ++e) top = fmaxf(top, pa_seen(e, upper, lower) ? s[e] : -INFINITY);
                     ref = fmaxf(top * sl2, PA_UNSET);
                 }
-                // exponentials against the reference as it is, while the maximum is only looked at for whether it may stay
-                if (windowed) pa_weights<2>(tS, sl2, ref, upper, lower, w, part, top);
-                else if (diagonal) pa_weights<1>(tS, sl2, ref, upper, lower, w, part, top);
-                else pa_weights<0>(tS, sl2, ref, upper, lower, w, part, top);
-                if (!__all_sync(0xffffffffu, top * sl2 <= ref + PA_TRIGGER)) {
-                    // (seldom) the reference moves; so do the sum and the output, which is complete: this step's scores were issued behind the
-                    // last step's product
-                    const float to = top * sl2 > ref + PA_TRIGGER ? top * sl2 : ref;
+                float part;
+                if (windowed) part = pa_weights<2>(tS, sl2, ref, upper, lower, w);
+                else if (diagonal) part = pa_weights<1>(tS, sl2, ref, upper, lower, w);
+                else part = pa_weights<0>(tS, sl2, ref, upper, lower, w);
+                if (!__all_sync(0xffffffffu, part <= PA_TRIGGER)) {
+                    // (seldom, or NaN) the reference moves up to the tile's largest score where that is larger; so do the sum and the output, which is
+                    // complete: this step's scores were issued behind the last step's product
+                    float top = PA_UNSET;
+#pragma unroll 1
+                    for (int c = 0; c < 128; c += 16) {
+                        float s[16];
+                        tmem_ld<16>(tS + c, s);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) top = fmaxf(top, pa_seen(c + e, upper, lower) ? s[e] * sl2 : -INFINITY);
+                    }
+                    const float to = fmaxf(ref, top);
                     const float by = pa_exp2(ref - to);
                     if (j > q.lo) {
 #pragma unroll 1
@@ -479,7 +490,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
                     }
                     ref = to;
                     sum *= by;
-                    pa_weights<2>(tS, sl2, ref, upper, lower, w, part, top);
+                    part = pa_weights<2>(tS, sl2, ref, upper, lower, w);
                 }
                 sum += part;
 #pragma unroll
@@ -489,6 +500,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[t]);
             }
+            ahead = walk.next();     // (while the last product is under way)
             if (!dead && !mbar_wait(&o_full[t], on & 1, a.status, KID_PROMPT, 7)) dead = true;
             ++on;
             tc_fence_after();
@@ -496,25 +508,26 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
             const bool live = row < p.len;
             // through shared memory, so that a store instruction writes four rows of 128 bytes instead of 32 pieces of 16
             const int row0 = q.qb * PA_BM + (warp & 3) * 32;      // the warp's first row
+            bf16* dst = a.out + (size_t)(p.start + row0) * a.ldo + (size_t)q.head * D;
 #pragma unroll
             for (int c = 0; c < D; c += 64) {
+                float o[64];
+                tmem_ld_issue<32>(tO + c, o);
+                tmem_ld_issue<32>(tO + c + 32, o + 32);
+                tmem_wait_ld();
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float o[32];
-                    tmem_ld<32>(tO + c + h * 32, o);
-#pragma unroll
-                    for (int e = 0; e < 32; e += 8)
-                        *reinterpret_cast<uint4*>(stage + lane * 128 + ((((h * 32 + e) / 8) ^ (lane & 7)) << 4)) =
-                            make_uint4(pa_pack(o[e] * inv, o[e + 1] * inv), pa_pack(o[e + 2] * inv, o[e + 3] * inv),
-                                       pa_pack(o[e + 4] * inv, o[e + 5] * inv), pa_pack(o[e + 6] * inv, o[e + 7] * inv));
-                }
+                for (int e = 0; e < 64; e += 8)
+                    *reinterpret_cast<uint4*>(stage + lane * 128 + (((e / 8) ^ (lane & 7)) << 4)) =
+                        make_uint4(pa_pack(o[e] * inv, o[e + 1] * inv), pa_pack(o[e + 2] * inv, o[e + 3] * inv),
+                                   pa_pack(o[e + 4] * inv, o[e + 5] * inv), pa_pack(o[e + 6] * inv, o[e + 7] * inv));
                 __syncwarp();
+                uint4 v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = *reinterpret_cast<const uint4*>(stage + (i * 4 + (lane >> 3)) * 128 + (((lane & 7) ^ ((i * 4 + (lane >> 3)) & 7)) << 4));
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const int rr = i * 4 + (lane >> 3), cc = lane & 7;
-                    if (row0 + rr < p.len)
-                        *reinterpret_cast<uint4*>(a.out + (size_t)(p.start + row0 + rr) * a.ldo + (size_t)q.head * D + c + cc * 8) =
-                            *reinterpret_cast<const uint4*>(stage + rr * 128 + ((cc ^ (rr & 7)) << 4));
+                    const int rr = i * 4 + (lane >> 3);
+                    if (row0 + rr < p.len) *reinterpret_cast<uint4*>(dst + (size_t)rr * a.ldo + c + (lane & 7) * 8) = v[i];
                 }
                 __syncwarp();
             }
