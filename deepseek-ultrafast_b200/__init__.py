@@ -634,15 +634,14 @@ def _vector(ctx, name, x, dtype, n=None):
 def _rows(ctx, name, x, dtype, n=None, width=None):
     """x is a matrix [n][width] of this type on the context's device whose rows may lie apart; returns its row stride."""
     try:
-        if x.dtype is dtype and x.get_device() == ctx.index and x.dim() == 2:
-            m, w = x.shape
-            ld, one = x.stride()
-            if (n is None or m == n) and (width is None or w == width):
-                if m < 2 or w == 0:
-                    ld = w          # (a single row's stride says nothing)
-                if (one == 1 or w < 2 or m == 0) and ld >= w:
-                    return ld
-    except AttributeError:
+        m, w = x.shape
+        ld, one = x.stride()
+        if x.dtype is dtype and x.get_device() == ctx.index and (n is None or m == n) and (width is None or w == width):
+            if m < 2 or w == 0:
+                ld = w          # (a single row's stride says nothing)
+            if (one == 1 or w < 2 or m == 0) and ld >= w:
+                return ld
+    except (AttributeError, ValueError):
         pass
     _refuse(ctx, name, x, dtype, (n, width), True)
 
@@ -713,7 +712,7 @@ def kv_append(ctx, cache, k, v, pos, block_table, seq=None, rope=None, rope_half
         heads = width // d
         _need(heads > 0 and heads * d == width, "kv_append: q's rows must hold whole heads")
         if q_out is None:
-            q_out = t.empty((n, width), dtype=t.bfloat16, device=ctx.device)
+            q_out = q.new_empty((n, width))
         ldo = _rows(ctx, "kv_append: q_out", q_out, t.bfloat16, n, width)
         qp, op = q.data_ptr(), q_out.data_ptr()
     ctx.check(lib().dsuf_kv_append(ctx.h, ctx.stream(), cache.ref, k.data_ptr(), ldk, v.data_ptr(), ldv, n, pos.data_ptr(),
@@ -737,10 +736,10 @@ def attn_decode(ctx, cache, q, block_table, seq_lens, scale=None, window=0, out=
     _need(n_seqs == b, "attn_decode: block_table holds one row per row of q")
     _vector(ctx, "attn_decode: seq_lens", seq_lens, t.int32, b)
     if out is None:
-        out = t.empty((b, width), dtype=t.bfloat16, device=ctx.device)
+        out = q.new_empty((b, width))
     ldo = _rows(ctx, "attn_decode: out", out, t.bfloat16, b, width)
     if lse is None and return_lse:
-        lse = t.empty((b, heads), dtype=t.float32, device=ctx.device)
+        lse = q.new_empty((b, heads), dtype=t.float32)
     if lse is not None:
         _need(_rows(ctx, "attn_decode: lse", lse, t.float32, b, heads) == heads, "attn_decode: lse must be contiguous")
     if workspace is None:
@@ -769,10 +768,10 @@ def attn_prompt(ctx, q, k, v, cu_seqlens, head_dim=128, scale=None, window=0, ou
     _vector(ctx, "attn_prompt: cu_seqlens", cu_seqlens, t.int32)
     _need(cu_seqlens.shape[0] >= 1, "attn_prompt: cu_seqlens holds at least one entry")
     if out is None:
-        out = t.empty((n, width), dtype=t.bfloat16, device=ctx.device)
+        out = q.new_empty((n, width))
     ldo = _rows(ctx, "attn_prompt: out", out, t.bfloat16, n, width)
     if lse is None and return_lse:
-        lse = t.empty((n, heads), dtype=t.float32, device=ctx.device)
+        lse = q.new_empty((n, heads), dtype=t.float32)
     if lse is not None:
         _need(_rows(ctx, "attn_prompt: lse", lse, t.float32, n, heads) == heads, "attn_prompt: lse must be contiguous")
     ctx.check(lib().dsuf_attn_prompt(ctx.h, ctx.stream(), q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, n, heads, kv_heads, head_dim,
@@ -796,11 +795,11 @@ def sample(ctx, logits, u, temperature=None, top_k=None, top_p=None, min_p=None,
             _vector(ctx, name, x, dtype, m)
         ptrs.append(0 if x is None else x.data_ptr())
     if ids is None:
-        ids = t.empty(m, dtype=t.int32, device=ctx.device)
+        ids = u.new_empty(m, dtype=t.int32)
     else:
         _vector(ctx, "sample: ids", ids, t.int32, m)
     if logprobs is None and return_logprobs:
-        logprobs = t.empty(m, dtype=t.float32, device=ctx.device)
+        logprobs = u.new_empty(m)
     if logprobs is not None:
         _vector(ctx, "sample: logprobs", logprobs, t.float32, m)
     ctx.check(lib().dsuf_sample(ctx.h, ctx.stream(), logits.data_ptr(), ld, m, n, *ptrs, u.data_ptr(), ids.data_ptr(),

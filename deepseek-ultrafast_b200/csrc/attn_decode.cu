@@ -36,6 +36,7 @@ constexpr int AD_STAGES = 3;
 constexpr int AD_HALF = 4096;                              // bytes of keys (and of values) in a warp's stage
 constexpr int AD_RING = AD_WARPS * AD_STAGES * 2 * AD_HALF;
 constexpr int AD_PART = 16 * 128;                          // floats of one partial output
+constexpr int AD_JOIN = 8;                                 // partials whose loads are in flight together when a piece is joined
 constexpr float AD_UNSET = -1e30f;
 constexpr float AD_TRIGGER = 15.f, AD_HEADROOM = 7.f;
 
@@ -524,18 +525,18 @@ __global__ void __launch_bounds__(AD_THREADS, 2) attn_decode_kernel(const Decode
                     const int r = i / (D / 4), c = (i % (D / 4)) * 4;
                     float top = AD_UNSET, l = 0.f;
                     float4 acc = make_float4(0, 0, 0, 0);
-                    for (int x0 = first; x0 <= last; x0 += 8) {
-                        float2 ml[8];
-                        float4 v[8];
+                    for (int x0 = first; x0 <= last; x0 += AD_JOIN) {
+                        float2 ml[AD_JOIN];
+                        float4 v[AD_JOIN];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
+                        for (int j = 0; j < AD_JOIN; ++j) {
                             const int x = min(x0 + j, last);
                             const size_t sl = (size_t)x * 2 + (x == first ? 1 : 0);
                             ml[j] = __ldcg(reinterpret_cast<const float2*>(a.part_ml + sl * 32 + 2 * r));
                             v[j] = __ldcg(reinterpret_cast<const float4*>(a.part + sl * AD_PART + r * D + c));
                         }
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
+                        for (int j = 0; j < AD_JOIN; ++j) {
                             if (x0 + j <= last && ml[j].y != 0.f) {
                                 const float to = fmaxf(top, ml[j].x);
                                 const float f0 = exp2_approx(top - to), f1 = exp2_approx(ml[j].x - to);
