@@ -142,7 +142,7 @@ ABI = {
                                              C.c_int32, C.c_uint64, C.c_int32, C.c_int32, C.c_uint64, C.c_uint64]),
     "dsuf_kv_append": (C.c_int32, [C.c_void_p, C.c_void_p, C.POINTER(KvCacheStruct), C.c_uint64, C.c_int32, C.c_uint64, C.c_int32, C.c_int32,
                                    C.c_uint64, C.c_uint64, C.c_uint64, C.c_int32, C.c_int32, C.POINTER(RopeStruct), C.c_uint64, C.c_int32,
-                                   C.c_int32, C.c_uint64, C.c_int32]),
+                                   C.c_int32, C.c_uint64, C.c_int32, C.c_uint64, C.c_int32]),
     "dsuf_attn_workspace_bytes": (C.c_size_t, [C.c_void_p]),
     "dsuf_attn_workspace_init": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_uint64, C.c_size_t]),
     "dsuf_attn_decode": (C.c_int32, [C.c_void_p, C.c_void_p, C.POINTER(KvCacheStruct), C.c_uint64, C.c_int32, C.c_int32, C.c_int32, C.c_uint64,
@@ -683,12 +683,13 @@ def _table(ctx, who, table):
     return table.shape
 
 
-def kv_append(ctx, cache, k, v, pos, block_table, seq=None, rope=None, rope_half=False, q=None, q_out=None):
+def kv_append(ctx, cache, k, v, pos, block_table, seq=None, rope=None, rope_half=False, q=None, q_out=None, k_out=None):
     """dsuf_kv_append: writes the tokens' keys (rotated) and values bf16 [t][kv_heads * head_dim] into the cache at positions
     ``pos`` i32 [t] of sequences ``seq`` i32 [t] (None: token i is sequence i), pages from ``block_table`` i32 [seqs][pages]; a
     negative pos or seq is padding.  ``rope`` = (cos f32 [positions][rot/2], sin, off): columns [off, off + rot) of every head, in
     (even, odd) pairs or with ``rope_half`` in pairs rot/2 apart.  ``q`` bf16 [t][q_heads * head_dim]: rotated as well, into
-    ``q_out`` (None: a new tensor; q itself: in place).  Returns q_out."""
+    ``q_out`` (None: a new tensor; q itself: in place).  ``k_out``: receives the rotated keys as rows, for attn_prompt over these tokens (k
+    itself: in place).  Returns q_out."""
     t = ctx.torch
     _need(cache.ctx is ctx, "kv_append: the cache belongs to another context")
     d = cache.head_dim
@@ -715,8 +716,12 @@ def kv_append(ctx, cache, k, v, pos, block_table, seq=None, rope=None, rope_half
             q_out = q.new_empty((n, width))
         ldo = _rows(ctx, "kv_append: q_out", q_out, t.bfloat16, n, width)
         qp, op = q.data_ptr(), q_out.data_ptr()
+    kp = ldko = 0
+    if k_out is not None:
+        ldko = _rows(ctx, "kv_append: k_out", k_out, t.bfloat16, n, cache.kv_heads * d)
+        kp = k_out.data_ptr()
     ctx.check(lib().dsuf_kv_append(ctx.h, ctx.stream(), cache.ref, k.data_ptr(), ldk, v.data_ptr(), ldv, n, pos.data_ptr(),
-                                   seq.data_ptr() if seq is not None else 0, block_table.data_ptr(), n_seqs, pages, r, qp, ldq, heads, op, ldo))
+                                   seq.data_ptr() if seq is not None else 0, block_table.data_ptr(), n_seqs, pages, r, qp, ldq, heads, op, ldo, kp, ldko))
     return q_out
 
 
@@ -821,6 +826,75 @@ def probe_tensor_rate(ctx, n_cols=128, a_is_e2m1=False, iters=20000, reps=5):
         t.cuda.synchronize()
         best = max(best, flop.value / (e0.elapsed_time(e1) * 1e-3) / 1e12)
     return best
+
+
+def project(ctx, w, xq, xs, out):
+    """gemm_fp8 for any number of token rows: one launch on the tcgen05 path, slabs of 16 rows on the mma.sync path."""
+    m = out.shape[0]
+    slab = max(m, 1) if ctx.tcgen05 else 16
+    for r in range(0, m, slab):
+        e = min(m, r + slab)
+        gemm_fp8(ctx, w, xq[r:e], xs[r:e], e - r, out[r:e])
+    return out
+
+
+class AttnLayer:
+    """Self-attention of one layer over its paged cache: quant -> merged q/k/v projection -> kv_append (rotary embedding, cache write) ->
+    attn_decode or attn_prompt -> quant -> output projection.  ``wqkv`` is a dense FP8 Weight of (q_heads + 2 kv_heads) * head_dim
+    rows (queries, keys, values), ``wo`` one of q_heads * head_dim columns; ``rope`` = (cos, sin, off) as kv_append takes it.
+    All scratch for up to ``tokens`` rows is allocated once here; the calls only launch kernels."""
+
+    def __init__(self, ctx, wqkv, wo, cache, q_heads, tokens, rope=None, rope_half=False, window=0, scale=None, workspace=None):
+        t = ctx.torch
+        d, hkv = cache.head_dim, cache.kv_heads
+        _need(wqkv.n == (q_heads + 2 * hkv) * d, f"AttnLayer: wqkv has {wqkv.n} rows, wanted (q_heads + 2 kv_heads) * head_dim = {(q_heads + 2 * hkv) * d}")
+        _need(wo.k == q_heads * d, f"AttnLayer: wo has {wo.k} columns, wanted q_heads * head_dim = {q_heads * d}")
+        _need(q_heads % hkv == 0, "AttnLayer: q_heads must be a multiple of the cache's kv_heads")
+        self.ctx, self.wqkv, self.wo, self.cache, self.tokens = ctx, wqkv, wo, cache, tokens
+        self.rope, self.rope_half, self.window, self.scale, self.workspace = rope, rope_half, window, scale, workspace
+        self.widths = [q_heads * d, hkv * d, hkv * d]
+        self.xq, self.xs = self._codes(wqkv.mode, tokens, wqkv.k)
+        self.qkv = t.empty((tokens, wqkv.n), dtype=t.bfloat16, device=ctx.device)
+        self.o = t.empty((tokens, wo.k), dtype=t.bfloat16, device=ctx.device)
+        self.oq, self.os = self._codes(wo.mode, tokens, wo.k)
+
+    def _codes(self, mode, m, k):
+        t = self.ctx.torch
+        blk, dt = (32, t.uint8) if mode == MODE_MX else (128, t.float32)
+        return t.empty((m, k), dtype=t.uint8, device=self.ctx.device), t.empty((m, k // blk), dtype=dt, device=self.ctx.device)
+
+    def _project(self, x, quantized):
+        n = x.shape[0]
+        _need(n <= self.tokens, f"AttnLayer: {n} rows, room for {self.tokens}")
+        if quantized is None:
+            quantized = act_quant(self.ctx, self.wqkv.mode, x, self.xq[:n], self.xs[:n])
+        return project(self.ctx, self.wqkv, *quantized, self.qkv[:n]).split(self.widths, dim=1)
+
+    def _output(self, o, out):
+        n = o.shape[0]
+        act_quant(self.ctx, self.wo.mode, o, self.oq[:n], self.os[:n])
+        return project(self.ctx, self.wo, self.oq[:n], self.os[:n], out)
+
+    def decode(self, x, pos, seq_lens, block_table, out, quantized=None):
+        """One new token per sequence: x bf16 [b][hidden] at positions ``pos`` i32 [b], contexts ``seq_lens`` i32 [b] that count it
+        (pos + 1; 0 with a negative pos: a padded row, its attention is 0).  ``quantized``: (codes, scales) of x if a kernel before has left
+        them."""
+        q, k, v = self._project(x, quantized)
+        kv_append(self.ctx, self.cache, k, v, pos, block_table, rope=self.rope, rope_half=self.rope_half, q=q, q_out=q)
+        o = attn_decode(self.ctx, self.cache, q, block_table, seq_lens, scale=self.scale, window=self.window, out=self.o[:x.shape[0]],
+                        workspace=self.workspace)
+        return self._output(o, out)
+
+    def prompt(self, x, pos, seq, cu_seqlens, block_table, out, quantized=None):
+        """Whole prompts packed: x bf16 [t][hidden], token i at position ``pos[i]`` of sequence ``seq[i]`` (both i32 [t], negative: padding behind
+        the last sequence), ``cu_seqlens`` i32 [sequences + 1].  The sequences begin here: nothing cached before is attended to.  Rows
+        behind the last sequence give 0 attention."""
+        q, k, v = self._project(x, quantized)
+        kv_append(self.ctx, self.cache, k, v, pos, block_table, seq=seq, rope=self.rope, rope_half=self.rope_half, q=q, q_out=q, k_out=k)
+        o = self.o[:x.shape[0]]
+        o.zero_()      # (rows that no sequence holds are not written)
+        attn_prompt(self.ctx, q, k, v, cu_seqlens, head_dim=self.cache.head_dim, scale=self.scale, window=self.window, out=o)
+        return self._output(o, out)
 
 
 class MoePlan:

@@ -476,7 +476,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
 #pragma unroll
                         for (int e = 0; e < 16; ++e) top = fmaxf(top, pa_seen(c + e, upper, lower) ? s[e] * sl2 : -INFINITY);
                     }
-                    const float to = fmaxf(ref, top);
+                    const float to = part <= PA_TRIGGER ? ref : fmaxf(ref, top);      // (a row's result does not depend on its neighbours)
                     const float by = pa_exp2(ref - to);
                     if (j > q.lo) {
 #pragma unroll 1

@@ -17,8 +17,8 @@ constexpr int AP_BATCH = 3;   // heads of a thread whose loads are issued togeth
 
 struct AppendArgs {
     const bf16 *q, *k, *v;
-    bf16* q_out;
-    int ldq, ldk, ldv, ldqo;
+    bf16 *q_out, *k_out;
+    int ldq, ldk, ldv, ldqo, ldko;
     int q_heads, kv_heads, n_seqs, max_pages, n_pages, page_shift;
     const int *pos, *seq, *table;
     uint8_t *ck, *cv;
@@ -144,6 +144,7 @@ __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(const AppendArgs 
                 const int kh = h - a.q_heads - (is_v ? a.kv_heads : 0);
                 const size_t at = (size_t)page * a.page_stride + ((((size_t)kh << a.page_shift) + slot) * D + c8 * 8);
                 uint8_t* dst = is_v ? a.cv : a.ck;
+                if (!is_v && a.k_out) *reinterpret_cast<uint4*>(a.k_out + (size_t)tok * a.ldko + (size_t)kh * D + c8 * 8) = pack8(x);
                 if constexpr (FP8) {
                     const float* sc = is_v ? a.v_scale : a.k_scale;
                     const float s = sc ? __ldg(sc + kh) : 1.0f;
@@ -180,7 +181,8 @@ using namespace dsuf;
 
 extern "C" int32_t dsuf_kv_append(dsuf_ctx* ctx, void* stream, const dsuf_kv_cache* cache, uint64_t k, int32_t ldk, uint64_t v, int32_t ldv,
                                   int32_t t, uint64_t pos, uint64_t seq, uint64_t block_table, int32_t n_seqs, int32_t max_pages,
-                                  const dsuf_rope* rope, uint64_t q, int32_t ldq, int32_t q_heads, uint64_t q_out, int32_t ldqo) {
+                                  const dsuf_rope* rope, uint64_t q, int32_t ldq, int32_t q_heads, uint64_t q_out, int32_t ldqo,
+                                  uint64_t k_out, int32_t ldko) {
     if (!ctx) return DSUF_E_BADARG;
     int rc = check_kv_cache(ctx, "kv_append", cache);
     if (rc) return rc;
@@ -193,6 +195,8 @@ extern "C" int32_t dsuf_kv_append(dsuf_ctx* ctx, void* stream, const dsuf_kv_cac
                  "kv_append: ldk and ldv must be multiples of 8 and hold kv_heads * head_dim elements");
     DSUF_REQUIRE(ctx, !q_heads || (ldq >= q_heads * D && ldq % 8 == 0 && ldqo >= q_heads * D && ldqo % 8 == 0),
                  "kv_append: ldq and ldqo must be multiples of 8 and hold q_heads * head_dim elements");
+    DSUF_REQUIRE(ctx, !k_out || (ldko >= cache->kv_heads * D && ldko % 8 == 0 && (k_out & 15) == 0),
+                 "kv_append: k_out must be 16-byte aligned, ldko a multiple of 8 that holds kv_heads * head_dim elements");
     DSUF_REQUIRE(ctx, !rope || (rope->rot >= 16 && rope->rot % 16 == 0 && rope->off >= 0 && rope->off % 8 == 0 && rope->off + rope->rot <= D),
                  "kv_append: rope needs rot a multiple of 16, off a multiple of 8, off + rot <= head_dim");
     DSUF_REQUIRE(ctx, !rope || (rope->cos && rope->sin && (rope->cos & 15) == 0 && (rope->sin & 15) == 0 && rope->positions >= 1),
@@ -203,8 +207,8 @@ extern "C" int32_t dsuf_kv_append(dsuf_ctx* ctx, void* stream, const dsuf_kv_cac
     DSUF_REQUIRE(ctx, !q_heads || (q && q_out && (q & 15) == 0 && (q_out & 15) == 0), "kv_append: q and q_out must be 16-byte aligned");
     AppendArgs a;
     memset(&a, 0, sizeof(a));
-    a.q = (const bf16*)q; a.k = (const bf16*)k; a.v = (const bf16*)v; a.q_out = (bf16*)q_out;
-    a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldqo = ldqo;
+    a.q = (const bf16*)q; a.k = (const bf16*)k; a.v = (const bf16*)v; a.q_out = (bf16*)q_out; a.k_out = (bf16*)k_out;
+    a.ldq = ldq; a.ldk = ldk; a.ldv = ldv; a.ldqo = ldqo; a.ldko = ldko;
     a.q_heads = q_heads; a.kv_heads = cache->kv_heads; a.n_seqs = n_seqs; a.max_pages = max_pages; a.n_pages = cache->n_pages;
     a.page_shift = __builtin_ctz((unsigned)cache->page_size);
     a.pos = (const int*)pos; a.seq = (const int*)seq; a.table = (const int*)block_table;

@@ -6,21 +6,28 @@ sharded world-ways (rank r owns experts [r*E/W, (r+1)*E/W)), tokens are data par
 per layer the exchanges are an all-gather of the column slices of the output-sharded dense projection, which delivers
 every token row to every expert owner (dispatch), and the sum of the per-rank expert outputs (combine), which also is the
 next layer's input (ep.py).
+With ``kv_heads`` > 0 the single-GPU stack is one of whole layers: the dense projection becomes the output projection of an attention
+over a paged key/value cache per layer (AttnLayer), with a merged q/k/v projection in front.
 The reference is tensor-parallel only and combines with its own push all-reduce (cu/comm.cu:134-279); the
 expert-parallel exchange here is this library's design.
 """
 import os
 import sys
 
-from . import (MODE_DS, MODE_MX, SCORE_SOFTMAX, MoeLayer, Weight, act_quant, gemm_fp8, moe_route_tokens)
+from . import (MODE_DS, MODE_MX, SCORE_SOFTMAX, AttnLayer, KvCache, MoeLayer, Weight, act_quant, gemm_fp8, moe_route_tokens)
 from . import synth
 
 
 class StackConfig:
     def __init__(self, hidden=7168, inter=2048, n_experts=256, topk=8, layers=4, tokens=64, act_mode=MODE_DS,
-                 dense_mode=MODE_DS, std=0.02, seed=0):
+                 dense_mode=MODE_DS, std=0.02, seed=0, kv_heads=0, head_dim=128, page_size=64, cache_pages=0, cache_scale=None, rope=None,
+                 window=0):
         self.hidden, self.inter, self.n_experts, self.topk = hidden, inter, n_experts, topk
         self.layers, self.tokens, self.act_mode, self.dense_mode, self.std, self.seed = layers, tokens, act_mode, dense_mode, std, seed
+        # kv_heads > 0: attention with hidden / head_dim query heads in front of the output (dense) projection, over cache_pages pages per
+        # layer, bf16 or with a cache_scale e4m3 (keys and values stored as multiples of it: 2^-6 to 448 times the scale keep their precision)
+        self.kv_heads, self.head_dim, self.page_size, self.cache_pages, self.cache_scale = kv_heads, head_dim, page_size, cache_pages, cache_scale
+        self.rope, self.window = rope, window   # rope: (cos, sin, off) as kv_append takes it
 
 
 class LayerStack:
@@ -33,7 +40,7 @@ class LayerStack:
         dev = ctx.device
         self.ctx, self.cfg = ctx, cfg
         H, I, E = cfg.hidden, cfg.inter, cfg.n_experts
-        self.dense, self.moe, self.logits = [], [], []
+        self.dense, self.moe, self.logits, self.attn = [], [], [], []
         # decode: 8-row slots; prefill (tens of rows per expert and more): 128-row tiles (tcgen05 path only)
         tile_rows = 128 if ctx.tcgen05 and cfg.tokens * cfg.topk >= 32 * E else 8
         for l in range(cfg.layers):
@@ -47,6 +54,16 @@ class LayerStack:
                 w2 = synth.fp4_experts(t, E, H, I, cfg.std, cfg.seed + 1000 * l + 3, False, dev)
                 W13 = Weight.experts_fp4_packed(ctx, w13, 2 * I, H, E, True)
                 W2 = Weight.experts_fp4_packed(ctx, w2, H, I, E, False)
+            if cfg.kv_heads > 0:
+                if weights_from is not None:      # the same sequences: the other stack's cache as well
+                    wqkv, cache = weights_from.attn[l].wqkv, weights_from.attn[l].cache
+                else:
+                    n = H + 2 * cfg.kv_heads * cfg.head_dim
+                    tiles, sds = synth.fp8_dense(t, cfg.dense_mode == MODE_MX, n, H, cfg.std, cfg.seed + 1000 * l + 5, dev)
+                    wqkv = Weight(ctx, 0, cfg.dense_mode, n, H, 1, False, tiles, sds)
+                    scale = None if cfg.cache_scale is None else t.full((cfg.kv_heads,), cfg.cache_scale, dtype=t.float32, device=dev)
+                    cache = KvCache.empty(ctx, cfg.cache_pages, cfg.page_size, cfg.kv_heads, cfg.head_dim, scale is not None, scale, scale)
+                self.attn.append(AttnLayer(ctx, wqkv, self.dense[l], cache, H // cfg.head_dim, cfg.tokens, rope=cfg.rope, window=cfg.window))
             self.moe.append(MoeLayer(ctx, W13, W2, cfg.tokens, cfg.topk, cfg.act_mode, tile_rows=tile_rows))
             g = t.Generator(device=dev).manual_seed(cfg.seed + 1000 * l + 4)
             self.logits.append(t.randn(cfg.tokens, E, generator=g, device=dev, dtype=t.float32))
@@ -74,12 +91,20 @@ class LayerStack:
             gemm_fp8(ctx, w, self.xq[r0:r0 + m], self.xs[r0:r0 + m], m, out[r0:r0 + m])
         return out
 
-    def forward(self, x, events=None, layers=None):
+    def forward(self, x, events=None, layers=None, step=None):
+        """``step``: what a stack with attention needs of the tokens, (pos, seq_lens, block_table) of a decode step or (pos, seq,
+        cu_seqlens, block_table) of packed prompts (AttnLayer.decode / prompt)."""
         cfg = self.cfg
+        if (cfg.kv_heads > 0) != (step is not None):
+            raise ValueError("a stack with attention needs `step`, one without takes none")
         cur = x
         n_layers = cfg.layers if layers is None else layers
         for l in range(n_layers):
-            self.dense_forward(l, cur, self.h, prequantized=l > 0 and self.fuse_quant)
+            ready = l > 0 and self.fuse_quant
+            if step is None:
+                self.dense_forward(l, cur, self.h, prequantized=ready)
+            else:
+                (self.attn[l].decode if len(step) == 3 else self.attn[l].prompt)(cur, *step, self.h, quantized=(self.xq, self.xs) if ready else None)
             out = self.y[l & 1]
             # router inside the layer: decode-size batches take one launch for router + plan + gather/quant; the unpermute
             # leaves its result quantized for the next layer's projection
@@ -94,6 +119,8 @@ class LayerStack:
         slabs = (cfg.tokens + slab - 1) // slab
         if self.ctx.tcgen05:
             slabs = 1
+        if cfg.kv_heads > 0:
+            raise ValueError("the launch count is the benchmark stack's, without attention")
         # act_quant + dense slabs + front end (router + plan + gather/quant: 1 launch up to 1024 pairs, else 1 + 3 + 1)
         # + w13 + quant + w2 + unpermute
         front = 1 if cfg.tokens * cfg.topk <= 1024 else 5
@@ -153,6 +180,8 @@ class EpLayerStack:
 
     def __init__(self, ctx, cfg, dist, rank, world):
         from . import ep
+        if cfg.kv_heads > 0:
+            raise ValueError("the expert-parallel stack has no attention: use LayerStack")
         t = ctx.torch
         dev = ctx.device
         self.ctx, self.cfg, self.rank, self.world = ctx, cfg, rank, world

@@ -417,13 +417,14 @@ typedef struct {
     int32_t positions, rot, off, half;
 } dsuf_rope;
 /* Writes t tokens' keys (rotated to their positions when rope is given) and values into the cache and, with q_heads > 0, the
- * rotated queries to q_out (q_out = q: in place).  k, v bf16 [t][kv_heads * head_dim] (row strides ldk, ldv), q / q_out bf16
+ * rotated queries to q_out (q_out = q: in place).  k_out (or 0) receives the rotated keys as bf16 rows, for dsuf_attn_prompt over the same
+ * tokens (k_out = k: in place).  k, v bf16 [t][kv_heads * head_dim] (row strides ldk, ldv), q / q_out bf16
  * [t][q_heads * head_dim]; pos i32 [t], seq i32 [t] (0: token i belongs to sequence i, t <= n_seqs).  A token with a negative
  * pos or seq is padding: nothing of it is written.  The (seq, pos) pairs of one call must be distinct, and distinct sequences must not
  * share the pages that are written: which of two writes to one slot lands is undefined. */
 int32_t dsuf_kv_append(dsuf_ctx* ctx, void* stream, const dsuf_kv_cache* cache, uint64_t k, int32_t ldk, uint64_t v, int32_t ldv, int32_t t,
                        uint64_t pos, uint64_t seq, uint64_t block_table, int32_t n_seqs, int32_t max_pages, const dsuf_rope* rope,
-                       uint64_t q, int32_t ldq, int32_t q_heads, uint64_t q_out, int32_t ldqo);
+                       uint64_t q, int32_t ldq, int32_t q_heads, uint64_t q_out, int32_t ldqo, uint64_t k_out, int32_t ldko);
 /* Attention of one new token per sequence over the cache: out[b][h] = sum_j softmax_j(scale * <q[b][h], K_j>) V_j over positions
  * j in [max(0, len - window), len) (window 0: all), kv head = h / (q_heads / kv_heads).  The new token's own key is in the cache
  * already (dsuf_kv_append); seq_lens i32 [b] counts it.  A sequence of length <= 0 gives zeros and lse -inf.

@@ -272,3 +272,181 @@ def test_prompt(pkg, actx, d, hq, hkv, lens, window):
     assert ((lse[:n].double() - wl).abs() <= 2 ** -12 + 2 ** -22 * wl.abs()).all()
     again = pkg.attn_prompt(actx, q, k, v, cu, head_dim=d, window=window)
     assert torch.equal(out[:n], again[:n])
+
+
+# ------------------------------------------------------------------ strides, streams, workspaces
+@gpu
+@pytest.mark.parametrize("fp8", [False, True])
+def test_interleaved_layers_and_far_pages(pkg, actx, fp8):
+    """Pages of two layers interleaved in one allocation (a page stride of its own), and a pool of more than 2^31 elements, so that an offset
+    into it passes 32 bits."""
+    d, hkv, page, far = 128, 8, 64, 33000                    # 33000 * 8 * 64 * 128 = 2.16e9 elements per layer of k
+    dt = torch.uint8 if fp8 else torch.bfloat16
+    pool = torch.zeros(far, hkv, page, d, dtype=dt, device=DEV)
+    both = torch.zeros(6, 2, hkv, page, d, dtype=dt, device=DEV)
+    g = gen(8)
+    k, v, q = bf16(g, 3, hkv * d), bf16(g, 3, hkv * d), bf16(g, 3, 2 * hkv * d)
+    pos = torch.tensor([0, 63, 64], dtype=torch.int32, device=DEV)
+    for cache, table in ((pkg.KvCache(actx, pool, pool.clone()), torch.tensor([[far - 1, far - 7]], dtype=torch.int32, device=DEV)),
+                         (pkg.KvCache(actx, both[:, 1], both.clone()[:, 1]), torch.tensor([[5, 2]], dtype=torch.int32, device=DEV))):
+        pkg.kv_append(actx, cache, k, v, pos, table, seq=torch.zeros(3, dtype=torch.int32, device=DEV))
+        assert (cache.k[table[0, 0].long(), :, 0] != 0).any() and (cache.v[table[0, 1].long(), :, 0] != 0).any()
+        out = pkg.attn_decode(actx, cache, q[:1], table, torch.tensor([65], dtype=torch.int32, device=DEV))
+        live = table[0].long()
+        small = pkg.KvCache(actx, cache.k[live].contiguous(), cache.v[live].contiguous())
+        want, _, size = decode64(small, q[:1], torch.tensor([[0, 1]], dtype=torch.int32, device=DEV), [65], 0, d ** -0.5)
+        within(out, want, size, terms=2 ** -8 + 2 ** -12)
+    assert (both[:, 0] == 0).all() and actx.status().code == 0
+
+
+@gpu
+def test_two_streams_with_workspaces_of_their_own(pkg, actx):
+    cache, q, table, n = decode_inputs(pkg, actx, 3, [4000, 77, 1500], 8, 2, 128, 32, False)
+    alone = pkg.attn_decode(actx, cache, q, table, n)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    spaces = [actx.attn_workspace, actx.new_attn_workspace()]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        for st, w in zip(streams, spaces):
+            with torch.cuda.stream(st):
+                got.append(pkg.attn_decode(actx, cache, q, table, n, workspace=w))
+    torch.cuda.synchronize()
+    assert all(torch.equal(alone, x) for x in got)
+
+
+@gpu
+def test_captured_decode_follows_new_lengths(pkg, actx):
+    cache, q, table, n = decode_inputs(pkg, actx, 7, [900, 300, 2000, 31], 6, 2, 64, 16, True)
+    out = torch.empty(4, 6 * 64, dtype=torch.bfloat16, device=DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            pkg.attn_decode(actx, cache, q, table, n, out=out)
+    torch.cuda.current_stream().wait_stream(side)
+    for lens in ([900, 300, 2000, 31], [1, 0, 16, 17], [0, 0, 0, 0], [333, 300, 1, 30]):
+        n.copy_(torch.tensor(lens))
+        graph.replay()
+        assert torch.equal(out, pkg.attn_decode(actx, cache, q, table, n))
+
+
+@gpu
+def test_many_sequences(pkg, actx):
+    """More sequences than a warp has lanes, most of them empty or of one token, next to a long one."""
+    lens = [0] * 700
+    for i in range(0, 700, 7):
+        lens[i] = 1 + i % 40
+    lens[333], lens[699] = 5000, 3
+    cache, q, table, n = decode_inputs(pkg, actx, 11, lens, 3, 1, 64, 16, False)
+    out, lse = pkg.attn_decode(actx, cache, q, table, n, return_lse=True)
+    want, wl, size = decode64(cache, q, table, lens, 0, 64 ** -0.5)
+    within(out, want, size, terms=2 ** -8 + 2 ** -12)
+    assert torch.equal(wl > -math.inf, lse > -math.inf)
+
+
+@gpu
+def test_bad_pages_and_lengths_are_reported(pkg, actx):
+    cache, q, table, n = decode_inputs(pkg, actx, 12, [100, 40], 4, 2, 128, 16, False)
+    good = pkg.attn_decode(actx, cache, q, table, n)
+    bad = table.clone()
+    bad[0, 2] = cache.n_pages
+    out = pkg.attn_decode(actx, cache, q, bad, n)
+    with pytest.raises(pkg.DsufError, match="status 2 from kernel 8"):
+        actx.status()
+    assert torch.equal(out[1], good[1]) and not torch.isnan(out).any()
+    pkg.attn_decode(actx, cache, q, table, torch.tensor([100, 10 ** 9], dtype=torch.int32, device=DEV))
+    with pytest.raises(pkg.DsufError, match="status 2 from kernel 8"):
+        actx.status()
+    assert torch.equal(good, pkg.attn_decode(actx, cache, q, table, n)) and actx.status().code == 0
+
+
+@gpu
+def test_large_scores_move_the_reference(pkg, actx):
+    """Scores that grow along the context by far more than the reference's slack, in both kernels, and scores of thousands."""
+    g = gen(21)
+    d, n = 128, 700
+    q, k, v = bf16(g, n, 2 * d), bf16(g, n, d), bf16(g, n, d)
+    k *= (1.0 + torch.arange(n, device=DEV)[:, None] * 0.2).to(torch.bfloat16)
+    cu = torch.tensor([0, n], dtype=torch.int32, device=DEV)
+    for scale in (d ** -0.5, 1.0, 20.0):
+        out, lse = pkg.attn_prompt(actx, q, k, v, cu, scale=scale, return_lse=True)
+        want, wl, size = prompt64(q, k, v, [n], 2, 1, d, 0, scale)
+        # a score of magnitude s carries an fp32 error of up to 128 2^-24 s' (s' the sum of its terms' magnitudes): with s' below 2^17 here that
+        # is below 1 at scale 20, so outputs are only compared where the largest weight is beyond doubt
+        if scale < 1:
+            within(out, want, size, terms=2 ** -8 + 2 ** -6)
+        assert not torch.isnan(out).any() and ((lse.double() - wl).abs() <= 2 ** -12 + 2 ** -16 * wl.abs() + 128 * 2.0 ** -24 * scale * 2 ** 17).all()
+        cache = pkg.KvCache.empty(actx, 44, 16, 1, d)
+        table = torch.arange(44, dtype=torch.int32, device=DEV).reshape(1, 44)
+        pkg.kv_append(actx, cache, k, v, torch.arange(n, dtype=torch.int32, device=DEV), table, seq=torch.zeros(n, dtype=torch.int32, device=DEV))
+        o1, l1 = pkg.attn_decode(actx, cache, q[-1:], table, torch.tensor([n], dtype=torch.int32, device=DEV), scale=scale, return_lse=True)
+        if scale < 1:
+            within(o1, want[-1:], size[-1:], terms=2 ** -8 + 2 ** -6)
+        assert ((l1.double() - wl[-1:]).abs() <= 2 ** -12 + 2 ** -16 * wl[-1:].abs() + 128 * 2.0 ** -24 * scale * 2 ** 17).all()
+
+
+@gpu
+def test_nan_stays_with_the_rows_that_see_it(pkg, actx):
+    g = gen(22)
+    d, lens = 64, [200, 60]
+    q, k, v = bf16(g, 260, d), bf16(g, 260, d), bf16(g, 260, d)
+    cu = torch.tensor([0, 200, 260], dtype=torch.int32, device=DEV)
+    clean = pkg.attn_prompt(actx, q, k, v, cu, head_dim=d)
+    k2 = k.clone()
+    k2[150, 3] = math.nan                                   # seen by rows 150 .. 199
+    out = pkg.attn_prompt(actx, q, k2, v, cu, head_dim=d)
+    assert torch.equal(out[:150], clean[:150]) and torch.equal(out[200:], clean[200:]) and torch.isnan(out[150:200]).all()
+    v2 = v.clone()
+    v2[200:] = math.inf                                     # the next sequence's values, in the first one's last tile
+    out = pkg.attn_prompt(actx, q, k, v2, cu, head_dim=d)
+    assert torch.equal(out[:200], clean[:200])
+
+
+# ------------------------------------------------------------------ refusals
+@gpu
+def test_refusals(pkg, actx):
+    E, d = pkg.DsufError, 128
+    z = lambda *s, dt=torch.bfloat16, dev=DEV: torch.zeros(*s, dtype=dt, device=dev)   # noqa: E731
+    i = lambda *s: z(*s, dt=torch.int32)   # noqa: E731
+    cache = pkg.KvCache.empty(actx, 4, 16, 2, d)
+    k, v, q, pos, table = z(3, 2 * d), z(3, 2 * d), z(3, 4 * d), i(3), i(3, 1)
+    ok = dict(ctx=actx, cache=cache, k=k, v=v, pos=pos, block_table=table)
+    pkg.kv_append(**ok)
+    bad_append = [dict(k=k.float()), dict(k=k.cpu()), dict(k=z(3, d)), dict(v=z(2, 2 * d)), dict(pos=pos.long()), dict(pos=i(2)), dict(pos=i(6)[::2]),
+                  dict(block_table=i(3)), dict(block_table=i(2, 1)), dict(seq=i(2)), dict(q=z(3, d + 8)), dict(q=z(3, 0)), dict(q=q, q_out=z(3, 2 * d)),
+                  dict(k=z(3, 2 * d + 1)[:, 1:]), dict(k=z(3, 2 * d + 4)[:, : 2 * d]), dict(k_out=z(3, d)), dict(rope=(z(8, 4), z(8, 4), 0)),
+                  dict(rope=(z(8, 4, dt=torch.float32), z(8, 4, dt=torch.float32), 0)), dict(rope=(z(8, 64, dt=torch.float32), z(8, 32, dt=torch.float32), 0)),
+                  dict(rope=(z(8, 64, dt=torch.float32), z(8, 64, dt=torch.float32), 8)), dict(rope=(z(8, 32, dt=torch.float32), z(8, 32, dt=torch.float32), 4)),
+                  dict(k=[1, 2]), dict(k=None)]
+    for b in bad_append:
+        with pytest.raises(E):
+            pkg.kv_append(**{**ok, **b})
+    okd = dict(ctx=actx, cache=cache, q=q, block_table=table, seq_lens=pos)
+    pkg.attn_decode(**okd)
+    for b in [dict(q=z(3, 3 * d)), dict(q=z(3, 0)), dict(q=q.half()), dict(q=z(3, 4 * d + 2)[:, : 4 * d]), dict(block_table=i(2, 1)), dict(seq_lens=i(4)), dict(seq_lens=pos.float()),
+              dict(out=z(3, 2 * d)), dict(lse=z(3, 3, dt=torch.float32)), dict(lse=z(3, 4)), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf),
+              dict(window=-1), dict(workspace=z(16, dt=torch.uint8))]:
+        with pytest.raises(E):
+            pkg.attn_decode(**{**okd, **b})
+    cu = torch.tensor([0, 3], dtype=torch.int32, device=DEV)
+    okp = dict(ctx=actx, q=q, k=k, v=v, cu_seqlens=cu, head_dim=d)
+    pkg.attn_prompt(**okp)
+    for b in [dict(head_dim=96), dict(head_dim=32), dict(q=z(3, 3 * d)), dict(k=z(2, 2 * d)), dict(v=z(3, d)), dict(cu_seqlens=cu.long()), dict(cu_seqlens=i(0)), dict(out=z(3, d)),
+              dict(lse=z(4, 3, dt=torch.float32)), dict(scale=0.0), dict(scale=math.nan), dict(window=-2), dict(q=z(3, 4 * d + 4)[:, : 4 * d])]:
+        with pytest.raises(E):
+            pkg.attn_prompt(**{**okp, **b})
+    for a in [(z(4, 2, 16, 96),) * 2, (z(4, 2, 24, d),) * 2, (z(4, 2, 8, d),) * 2, (z(4, 2, 2048, d),) * 2]:
+        with pytest.raises(E):
+            pkg.attn_decode(actx, pkg.KvCache(actx, *a), z(1, 2 * a[0].shape[3]), i(1, 1), i(1))
+    for a in [(z(4, 2, 16, d), z(4, 2, 16, d).view(4, 2, 16, d)[:, :1]), (z(4, 2, 16, d), z(4, 2, 16, d, dt=torch.uint8)), (z(4, 2, 16, d, dt=torch.float32),) * 2,
+              (z(4, 16, 2, d).transpose(1, 2),) * 2, (z(4, 2, 16, d, dev="cpu"),) * 2, (z(4, 2, 16, d, dt=torch.uint8),) * 2 + (z(3, dt=torch.float32),)]:
+        with pytest.raises(E):
+            pkg.KvCache(actx, *a)
+    # empty batches are no error
+    assert pkg.attn_decode(actx, cache, z(0, 4 * d), i(0, 1), i(0)).shape == (0, 4 * d)
+    assert pkg.attn_prompt(actx, z(0, 4 * d), z(0, 2 * d), z(0, 2 * d), i(1)).shape == (0, 4 * d)
+    assert pkg.kv_append(actx, cache, z(0, 2 * d), z(0, 2 * d), i(0), i(0, 1)) is None
+    assert actx.status().code == 0

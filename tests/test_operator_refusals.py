@@ -1,0 +1,129 @@
+"""Argument checks of the cache, attention and sampling entries, without a GPU: the C entries refuse before they touch a device (a zeroed block
+stands in for the context, which they only write their message into), the Python mirror before it calls them."""
+import ctypes as C
+import math
+import types
+
+import pytest
+import torch
+
+P = 1 << 20          # an aligned address that nothing follows
+BAD = -1
+
+
+@pytest.fixture()
+def cctx():
+    return C.create_string_buffer(64 << 10)
+
+
+def cache(pkg, **kw):
+    f = dict(k=P, v=P, k_scale=0, v_scale=0, page_stride=2 * 16 * 128, dtype=0, n_pages=4, page_size=16, kv_heads=2, head_dim=128)
+    f.update(kw)
+    return pkg.KvCacheStruct(*(f[n] for n, _ in pkg.KvCacheStruct._fields_))
+
+
+def rope(pkg, **kw):
+    f = dict(cos=P, sin=P, positions=8, rot=128, off=0, half=0)
+    f.update(kw)
+    return pkg.RopeStruct(*(f[n] for n, _ in pkg.RopeStruct._fields_))
+
+
+BAD_CACHES = [dict(dtype=2), dict(head_dim=96), dict(head_dim=256), dict(page_size=8), dict(page_size=24), dict(page_size=2048), dict(page_size=0), dict(kv_heads=0),
+              dict(kv_heads=-1), dict(n_pages=0), dict(page_stride=16), dict(page_stride=2 * 16 * 128 + 8), dict(page_stride=-4096), dict(k=0), dict(v=P + 8),
+              dict(k_scale=P), dict(dtype=1, k_scale=P + 2)]
+
+
+def append(pkg, c, ctx, **kw):
+    a = dict(k=P, ldk=256, v=P, ldv=256, t=3, pos=P, seq=P, table=P, n_seqs=2, max_pages=4, rope=None, q=P, ldq=512, q_heads=4, q_out=P, ldqo=512, k_out=0, ldko=0)
+    a.update(kw)
+    r = a["rope"]
+    return pkg.lib().dsuf_kv_append(ctx, None, C.byref(c), a["k"], a["ldk"], a["v"], a["ldv"], a["t"], a["pos"], a["seq"], a["table"], a["n_seqs"], a["max_pages"],
+                                    C.byref(r) if r is not None else None, a["q"], a["ldq"], a["q_heads"], a["q_out"], a["ldqo"], a["k_out"], a["ldko"])
+
+
+def test_append_refuses(pkg, cctx):
+    for kw in BAD_CACHES:
+        assert append(pkg, cache(pkg, **kw), cctx) == BAD, kw
+    for kw in [dict(t=-1), dict(n_seqs=-1), dict(max_pages=0), dict(max_pages=1 << 28), dict(seq=0), dict(q_heads=-1), dict(q_heads=5000), dict(ldk=255), dict(ldk=260), dict(ldv=128),
+               dict(ldq=511), dict(ldqo=256), dict(ldq=516), dict(k=0), dict(k=P + 8), dict(v=0), dict(pos=0), dict(pos=P + 1), dict(table=0), dict(seq=P + 2), dict(q=0), dict(q_out=0),
+               dict(q_out=P + 4), dict(k_out=P, ldko=128), dict(k_out=P + 2, ldko=256)]:
+        assert append(pkg, cache(pkg), cctx, **kw) == BAD, kw
+    for kw in [dict(rot=0), dict(rot=24), dict(rot=144), dict(off=-8), dict(off=8), dict(rot=64, off=4), dict(cos=0), dict(sin=P + 4), dict(positions=0)]:
+        assert append(pkg, cache(pkg), cctx, rope=rope(pkg, **kw)) == BAD, kw
+    buf = C.create_string_buffer(512)
+    pkg.lib().dsuf_last_error(cctx, buf, 512)
+    assert b"rope" in buf.value
+    assert append(pkg, cache(pkg), cctx, t=0, k=0, v=0, pos=0, seq=0, table=0, q=0, q_out=0) == 0      # an empty batch
+    assert append(pkg, cache(pkg), None) == BAD
+    assert pkg.lib().dsuf_kv_append(cctx, None, None, P, 256, P, 256, 1, P, P, P, 1, 1, None, 0, 0, 0, 0, 0, 0, 0) == BAD
+
+
+def decode(pkg, c, ctx, **kw):
+    a = dict(q=P, ldq=512, q_heads=4, b=2, table=P, max_pages=4, lens=P, scale=0.1, window=0, out=P, ldo=512, lse=0, ws=P)
+    a.update(kw)
+    return pkg.lib().dsuf_attn_decode(ctx, None, C.byref(c), a["q"], a["ldq"], a["q_heads"], a["b"], a["table"], a["max_pages"], a["lens"], a["scale"], a["window"], a["out"],
+                                      a["ldo"], a["lse"], a["ws"])
+
+
+def test_decode_refuses(pkg, cctx):
+    for kw in BAD_CACHES:
+        assert decode(pkg, cache(pkg, **kw), cctx) == BAD, kw
+    for kw in [dict(b=-1), dict(max_pages=0), dict(max_pages=1 << 27), dict(q_heads=3), dict(q_heads=0), dict(q_heads=8192), dict(ldq=256), dict(ldq=514), dict(ldo=511), dict(scale=0.0),
+               dict(scale=-0.1), dict(scale=math.nan), dict(scale=math.inf), dict(window=-1), dict(q=0), dict(q=P + 8), dict(out=0), dict(table=0), dict(lens=0), dict(lens=P + 2),
+               dict(lse=P + 1), dict(ws=0), dict(ws=P + 8), dict(b=1 << 24, max_pages=1 << 20)]:
+        assert decode(pkg, cache(pkg), cctx, **kw) == BAD, kw
+    assert decode(pkg, cache(pkg), cctx, b=0, q=0, out=0, table=0, lens=0, ws=0) == 0
+    assert decode(pkg, cache(pkg), None) == BAD
+    assert pkg.lib().dsuf_attn_workspace_bytes(None) == 0
+    assert pkg.lib().dsuf_attn_workspace_init(cctx, None, 0, 1 << 30) == BAD
+
+
+def prompt(pkg, ctx, **kw):
+    a = dict(q=P, ldq=512, k=P, ldk=256, v=P, ldv=256, t=9, hq=4, hkv=2, d=128, cu=P, n=1, scale=0.1, window=0, out=P, ldo=512, lse=0)
+    a.update(kw)
+    return pkg.lib().dsuf_attn_prompt(ctx, None, a["q"], a["ldq"], a["k"], a["ldk"], a["v"], a["ldv"], a["t"], a["hq"], a["hkv"], a["d"], a["cu"], a["n"], a["scale"], a["window"],
+                                      a["out"], a["ldo"], a["lse"])
+
+
+def test_prompt_refuses(pkg, cctx):
+    for kw in [dict(d=96), dict(d=32), dict(hq=3), dict(hkv=0), dict(hq=0), dict(hq=4098, ldq=1 << 20), dict(t=-1), dict(n=-1), dict(ldq=504), dict(ldk=252), dict(ldv=128), dict(ldo=516),
+               dict(scale=0.0), dict(scale=math.nan), dict(window=-1), dict(q=0), dict(k=P + 8), dict(v=0), dict(out=P + 2), dict(cu=0), dict(cu=P + 2), dict(lse=P + 3)]:
+        assert prompt(pkg, cctx, **kw) == BAD, kw
+    assert prompt(pkg, cctx, t=0, q=0, k=0, v=0, out=0, cu=0) == 0 and prompt(pkg, cctx, n=0, cu=0) == 0
+    assert prompt(pkg, None) == BAD
+
+
+def test_sample_refuses(pkg, cctx):
+    def call(ctx=cctx, logits=P, ld=100, m=2, n=100, t=0, k=0, p=0, q=0, u=P, ids=P, lp=0):
+        return pkg.lib().dsuf_sample(ctx, None, logits, ld, m, n, t, k, p, q, u, ids, lp)
+    for kw in [dict(m=-1), dict(n=0), dict(n=(1 << 22) + 1, ld=1 << 23), dict(ld=99), dict(logits=0), dict(u=0), dict(ids=0), dict(ids=P + 1), dict(t=P + 2), dict(lp=P + 3), dict(m=1 << 28),
+               dict(ctx=None)]:
+        assert call(**kw) == BAD, kw
+    assert call(m=0, logits=0, u=0, ids=0) == 0
+
+
+def test_the_mirror_refuses(pkg):
+    """Shapes, types, devices and strides, on CPU tensors with a stand-in for the context."""
+    dev = torch.device("cpu")
+    ctx = types.SimpleNamespace(torch=torch, device=dev, index=-1)
+    E = pkg.DsufError
+    z = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt)   # noqa: E731
+    for a in [(z(4, 2, 16),) * 2, (z(4, 2, 16, 128, dt=torch.float32),) * 2, (z(4, 2, 16, 128), z(4, 2, 16, 64)), (z(4, 16, 2, 128).transpose(1, 2),) * 2,
+              (z(4, 2, 16, 128), z(8, 2, 16, 128)[::2]), (z(4, 2, 16, 128, dt=torch.uint8),) * 2 + (z(2),)]:
+        with pytest.raises(E):
+            pkg.KvCache(ctx, *a)
+    c = pkg.KvCache(ctx, z(8, 2, 16, 128)[::2], z(8, 2, 16, 128)[::2])
+    assert c.c.page_stride == 2 * 2 * 16 * 128 and (c.n_pages, c.kv_heads, c.page_size, c.head_dim) == (4, 2, 16, 128)
+    assert pkg._rows(ctx, "x", z(3, 10)[:, :8], torch.bfloat16, 3, 8) == 10
+    assert pkg._rows(ctx, "x", z(1, 8).as_strided((1, 8), (3, 1)), torch.bfloat16) == 8
+    for x in (z(3, 8).t(), z(3), z(2, 8).as_strided((2, 8), (4, 1)), z(3, 8, dt=torch.float16), None, 3):
+        with pytest.raises(E):
+            pkg._rows(ctx, "x", x, torch.bfloat16)
+    for x in (z(3, 1), z(6)[::2], z(4), z(3, dt=torch.float32), None):
+        with pytest.raises(E):
+            pkg._vector(ctx, "x", x, torch.bfloat16, 3)
+    other = types.SimpleNamespace(torch=torch, device=dev, index=-1)
+    with pytest.raises(E):
+        pkg.attn_decode(other, c, z(1, 512), z(1, 1, dt=torch.int32), z(1, dt=torch.int32))
+    with pytest.raises(E):
+        pkg.attn_prompt(ctx, z(3, 512), z(3, 256), z(3, 256), z(2, dt=torch.int32), head_dim=100)

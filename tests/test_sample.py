@@ -165,3 +165,28 @@ def test_defaults_and_frequencies(pkg, sctx):
     ids = pkg.sample(sctx, row.expand(m, 50).contiguous(), u)
     count = torch.bincount(ids.long(), minlength=50).double()
     assert ((count - torch.softmax(row.double(), 0) * m).abs() <= 1.0).all()
+
+
+@gpu
+def test_refusals(pkg, sctx):
+    E = pkg.DsufError
+    x, u = torch.zeros(3, 100, device=DEV), torch.zeros(3, device=DEV)
+    f, i = torch.zeros(3, device=DEV), torch.zeros(3, dtype=torch.int32, device=DEV)
+    pkg.sample(sctx, x, u)
+    for logits, uu, kw in [(x.half(), u, {}), (x.cpu(), u, {}), (x, u[:2], {}), (x, u.double(), {}), (x[0], u, {}), (x.t(), u, {}), (x, u, dict(temperature=i)), (x, u, dict(top_k=f)),
+                           (x, u, dict(top_p=f[:2])), (x, u, dict(min_p=f.cpu())), (x, u, dict(ids=f)), (x, u, dict(logprobs=i)), (x[:, :0], u, {}), (None, u, {})]:
+        with pytest.raises(E):
+            pkg.sample(sctx, logits, uu, **kw)
+    assert pkg.sample(sctx, x[:0], u[:0]).shape == (0,)
+
+
+@gpu
+def test_head_and_sampler_together(pkg, sctx):
+    """The output head's logits, their padding columns included, straight into the sampler; greedy rows agree with the head's records."""
+    g = torch.Generator(device=DEV).manual_seed(2)
+    w = torch.empty(1024, 256, device=DEV).normal_(0, 0.1, generator=g).bfloat16()
+    h = torch.empty(9, 256, device=DEV).normal_(0, 1, generator=g).bfloat16()
+    logits, rec = pkg.lm_head(sctx, w, h, temperature=1.0)
+    ids = pkg.sample(sctx, logits, torch.zeros(9, device=DEV), temperature=torch.zeros(9, device=DEV))
+    best = rec[:, :, 0].argmax(1)
+    assert torch.equal(ids, rec[torch.arange(9), best, 11].contiguous().view(torch.int32))
