@@ -24,8 +24,9 @@
 //
 // Softmax: base-2 exponentials against a reference point that only moves when a score exceeds it by 2^15 (exact: the sum and the
 // output share it); it is set 7 below the maximum so that p <= 2^15 and p's fp16 form keeps full precision down to 2^-21 of
-// the largest.  Scores, sums and outputs are fp32; p is rounded once, to bf16 (bf16 cache) or fp16 (e4m3 cache), as operand of
-// the second product.  e4m3 codes are widened exactly to fp16; the query is scaled by a power of two into fp16's range first.
+// the largest.  Scores, sums and outputs are fp32.  As operand of the second product p is rounded to fp16
+// (e4m3 cache), or split into two bf16 numbers (bf16 cache, whose values fix the operands' type): one alone would make the output's error 1.4 times
+// that of its own rounding, the second costs 1 % of the time.  e4m3 codes are widened exactly to fp16; the query is scaled by a power of two into fp16's range first.
 #include "internal.h"
 
 namespace dsuf {
@@ -542,7 +543,7 @@ __global__ void __launch_bounds__(AD_THREADS, 2) attn_decode_kernel(const Decode
                             }
                         }
                 }
-                uint32_t pf[NT][2];
+                uint32_t pf[NT][2], pr[NT][2];     // pr: what rounding to bf16 leaves
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float p[4];
@@ -550,8 +551,13 @@ __global__ void __launch_bounds__(AD_THREADS, 2) attn_decode_kernel(const Decode
                     for (int e = 0; e < 4; ++e) p[e] = exp2_approx(st[nt][e] - ref[nt][e & 1]);
                     sum[nt][0] += p[0] + p[2];
                     sum[nt][1] += p[1] + p[3];
-                    pf[nt][0] = transpose8x8(pack2<FP8>(p[0], p[1]));
-                    pf[nt][1] = transpose8x8(pack2<FP8>(p[2], p[3]));
+                    const uint32_t w0 = pack2<FP8>(p[0], p[1]), w1 = pack2<FP8>(p[2], p[3]);
+                    pf[nt][0] = transpose8x8(w0);
+                    pf[nt][1] = transpose8x8(w1);
+                    if constexpr (!FP8) {
+                        pr[nt][0] = transpose8x8(pack2<false>(p[0] - __uint_as_float(w0 << 16), p[1] - __uint_as_float(w0 & 0xffff0000u)));
+                        pr[nt][1] = transpose8x8(pack2<false>(p[2] - __uint_as_float(w1 << 16), p[3] - __uint_as_float(w1 & 0xffff0000u)));
+                    }
                 }
                 // O^T (D x heads) += V^T (D x 16 tokens) P^T
                 if constexpr (!FP8) {
@@ -560,7 +566,10 @@ __global__ void __launch_bounds__(AD_THREADS, 2) attn_decode_kernel(const Decode
                         uint32_t vf[4];
                         ldsm4t(vf, vst + ring_at<S::ROW>(s * 16 + (lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)));
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) mma_16816<false>(o[ks][nt], vf, pf[nt][0], pf[nt][1]);
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma_16816<false>(o[ks][nt], vf, pf[nt][0], pf[nt][1]);
+                            mma_16816<false>(o[ks][nt], vf, pr[nt][0], pr[nt][1]);
+                        }
                     }
                 } else {
 #pragma unroll
