@@ -698,6 +698,7 @@ static int decode_launch(dsuf_ctx* ctx, cudaStream_t stream, DecodeArgs& a) {
     // no more CTAs than units that the block table could hold (their number is only known on the device)
     const long long cap = (long long)a.b * a.kv_heads * a.blocks * ((((long long)a.max_pages << a.page_shift) + 15 + S::UNIT - 1) / S::UNIT);
     DSUF_REQUIRE(ctx, cap < (1ll << 31), "attn_decode: b * kv_heads * positions of the block table is too large (%lld units of work)", cap);
+    DSUF_REQUIRE_DEVICE(ctx, "attn_decode");
     const int grid = (int)(cap < decode_ctas(ctx) ? cap : decode_ctas(ctx));
     return launch(ctx, stream, attn_decode_kernel<D, FP8, NT>, dim3(grid), dim3(AD_THREADS), (size_t)S::SMEM, a);
 }

@@ -576,6 +576,7 @@ extern "C" int32_t dsuf_attn_prompt(dsuf_ctx* ctx, void* stream, uint64_t q, int
     if (t == 0 || n_seqs == 0) return DSUF_OK;
     DSUF_REQUIRE(ctx, q && k && v && out && cu_seqlens && (q & 15) == 0 && (k & 15) == 0 && (v & 15) == 0 && (out & 15) == 0 && (cu_seqlens & 3) == 0 &&
                  (lse & 3) == 0, "attn_prompt: null or misaligned pointer (q, k, v, out 16 bytes, cu_seqlens and lse 4)");
+    DSUF_REQUIRE_DEVICE(ctx, "attn_prompt");
     PromptArgs a;
     memset(&a, 0, sizeof(a));
     int rc = encode_heads(ctx, &a.tm_q, (const void*)q, (long long)q_heads * head_dim, ldq, t);

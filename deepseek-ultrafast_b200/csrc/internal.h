@@ -65,6 +65,13 @@ inline int cuda_fail(dsuf_ctx* ctx, cudaError_t e, const char* what) {
 #define DSUF_REQUIRE(ctx, cond, ...) \
     do { if (!(cond)) return ::dsuf::fail(ctx, DSUF_E_BADARG, __VA_ARGS__); } while (0)
 
+// The default stream's handle names the current device's: a launch with another one current would run there, on this context's pointers.
+#define DSUF_REQUIRE_DEVICE(ctx, who) \
+    do { int dev_ = -1; \
+         cudaError_t err_ = cudaGetDevice(&dev_); \
+         if (err_ != cudaSuccess) return ::dsuf::cuda_fail(ctx, err_, who); \
+         if (dev_ != (ctx)->device) return ::dsuf::fail(ctx, DSUF_E_BADARG, "%s: device %d is current, the context's is %d", who, dev_, (ctx)->device); } while (0)
+
 // One launch path for every kernel: asynchronous on the caller's stream, optional PDL attribute, no
 // allocation and no synchronisation (safe inside stream capture).
 // `cluster_x` > 1 launches thread-block clusters of that many CTAs along x (the grid must be a multiple of it).

@@ -205,6 +205,7 @@ extern "C" int32_t dsuf_kv_append(dsuf_ctx* ctx, void* stream, const dsuf_kv_cac
     DSUF_REQUIRE(ctx, k && v && pos && block_table && (k & 15) == 0 && (v & 15) == 0 && (pos & 3) == 0 && (seq & 3) == 0 && (block_table & 3) == 0,
                  "kv_append: null or misaligned pointer (k, v 16 bytes, indexes 4)");
     DSUF_REQUIRE(ctx, !q_heads || (q && q_out && (q & 15) == 0 && (q_out & 15) == 0), "kv_append: q and q_out must be 16-byte aligned");
+    DSUF_REQUIRE_DEVICE(ctx, "kv_append");
     AppendArgs a;
     memset(&a, 0, sizeof(a));
     a.q = (const bf16*)q; a.k = (const bf16*)k; a.v = (const bf16*)v; a.q_out = (bf16*)q_out; a.k_out = (bf16*)k_out;

@@ -774,6 +774,7 @@ extern "C" int32_t dsuf_sample(dsuf_ctx* ctx, void* stream, uint64_t logits, int
     if (m == 0) return DSUF_OK;
     DSUF_REQUIRE(ctx, logits && u && ids_out && ((logits | u | ids_out | logprobs_out | temperature | top_k | top_p | min_p) & 3) == 0,
                  "sample: null or misaligned pointer");
+    DSUF_REQUIRE_DEVICE(ctx, "sample");
     SampleArgs a;
     memset(&a, 0, sizeof(a));
     a.logits = (const float*)logits; a.ld = ld; a.n = n;

@@ -4,6 +4,7 @@ with experts, and a decode step from hidden states to sampled tokens, eager and 
 Tolerances of the attention as in test_kv_attention.py; the projections around it are compared bit for bit with the same kernels
 called by themselves."""
 import math
+import os
 
 import pytest
 import torch
@@ -18,7 +19,7 @@ DEV = "cuda"
 def lctx(pkg, request):
     if not torch.cuda.is_available():
         pytest.skip("no GPU")
-    c = pkg.Ctx(0, tcgen05=request.param)
+    c = pkg.Ctx(0, tcgen05=request.param, pdl=os.environ.get("DSUF_TEST_PDL", "0") == "1")
     yield c
     c.close()
 

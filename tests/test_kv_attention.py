@@ -5,6 +5,7 @@ The softmax weights enter the second product rounded to bf16 (2^-8 each, at wors
 2^-8 of its own magnitude plus 2^-8 of sum_j p_j |v_j|, the sum of its terms' magnitudes; fp32 sums and base-2 exponentials add
 less than 2^-12 of that sum (a score s has an absolute error of about d 2^-24 sum |q k| scale, below 2^-14 for these inputs)."""
 import math
+import os
 
 import pytest
 import torch
@@ -17,7 +18,7 @@ DEV = "cuda"
 def actx(pkg):
     if not torch.cuda.is_available():
         pytest.skip("no GPU")
-    c = pkg.Ctx(0)
+    c = pkg.Ctx(0, pdl=os.environ.get("DSUF_TEST_PDL", "0") == "1")
     yield c
     c.close()
 
@@ -450,3 +451,22 @@ def test_refusals(pkg, actx):
     assert pkg.attn_prompt(actx, z(0, 4 * d), z(0, 2 * d), z(0, 2 * d), i(1)).shape == (0, 4 * d)
     assert pkg.kv_append(actx, cache, z(0, 2 * d), z(0, 2 * d), i(0), i(0, 1)) is None
     assert actx.status().code == 0
+
+
+@gpu
+def test_another_current_device_is_refused(pkg, actx):
+    """The context says device 0; a copy of it that says 5 stands for a caller that has another device current."""
+    import ctypes as C
+    other = C.create_string_buffer(64 << 10)
+    C.memmove(other, actx.h, 64)
+    C.cast(other, C.POINTER(C.c_int32))[0] = 5
+    L, cache = pkg.lib(), pkg.KvCache.empty(actx, 2, 16, 1, 64)
+    x, i, f = bf16(gen(1), 2, 64), torch.zeros(2, dtype=torch.int32, device=DEV), torch.zeros(2, 64, device=DEV)
+    p, s = x.data_ptr(), actx.stream()
+    assert L.dsuf_kv_append(other, s, cache.ref, p, 64, p, 64, 1, i.data_ptr(), 0, i.data_ptr(), 1, 1, None, 0, 0, 0, 0, 0, 0, 0) == -1
+    assert L.dsuf_attn_decode(other, s, cache.ref, p, 64, 1, 1, i.data_ptr(), 1, i.data_ptr(), 1.0, 0, p, 64, 0, actx.attn_workspace.data_ptr()) == -1
+    assert L.dsuf_attn_prompt(other, s, p, 64, p, 64, p, 64, 2, 1, 1, 64, i.data_ptr(), 1, 1.0, 0, p, 64, 0) == -1
+    assert L.dsuf_sample(other, s, f.data_ptr(), 64, 2, 64, 0, 0, 0, 0, f.data_ptr(), i.data_ptr(), 0) == -1
+    buf = C.create_string_buffer(512)
+    L.dsuf_last_error(other, buf, 512)
+    assert b"device 0 is current" in buf.value

@@ -6,6 +6,7 @@ worst), so a border moves by at most 2^-21 of the row's weight against u times t
 from the borders of the chosen token, and the limits' distance from theirs, is above that (the inputs are drawn by
 seed; how many rows that leaves out is bounded below)."""
 import math
+import os
 
 import numpy as np
 import pytest
@@ -20,7 +21,7 @@ NEAR = 2.0 ** -21
 def sctx(pkg):
     if not torch.cuda.is_available():
         pytest.skip("no GPU")
-    c = pkg.Ctx(0)
+    c = pkg.Ctx(0, pdl=os.environ.get("DSUF_TEST_PDL", "0") == "1")
     yield c
     c.close()
 
