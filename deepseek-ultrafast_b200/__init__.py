@@ -760,8 +760,7 @@ def attn_decode(ctx, cache, q, block_table, seq_lens, scale=None, window=0, out=
 def attn_prompt(ctx, q, k, v, cu_seqlens, head_dim=128, scale=None, window=0, out=None, lse=None, return_lse=False):
     """dsuf_attn_prompt: causal attention over packed prompts, q bf16 [t][q_heads * head_dim], k / v bf16 [t][kv_heads * head_dim] (their
     rows may be parts of a merged projection's), ``cu_seqlens`` i32 [sequences + 1]; ``window`` > 0: a row sees that many rows, itself
-    included.  ``scale`` None: head_dim ** -0.5.  Rows behind the last sequence are not written.  The values of a sequence's tokens must be finite (one
-    that is not may reach every row of its block of 128).  Returns out bf16
+    included.  ``scale`` None: head_dim ** -0.5.  Rows behind the last sequence are not written.  Returns out bf16
     [t][q_heads * head_dim], or (out, lse f32 [t][q_heads]) with ``return_lse``."""
     t = ctx.torch
     _need(head_dim in (64, 128), "attn_prompt: head_dim is 64 or 128")

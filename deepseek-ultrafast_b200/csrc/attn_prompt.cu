@@ -46,11 +46,13 @@ struct PromptShape {
 
 struct PromptArgs {
     CUtensorMap tm_q, tm_k, tm_v;
+    const bf16 *q, *k, *v;          // the same rows, for the seldom path of prompt_repair
+    int ldq, ldk, ldv;
     bf16* out;
     float* lse;
     int ldo, t, q_heads, kv_heads, group, n_seqs, window;
     const int* cu;
-    float scale_log2;
+    float scale, scale_log2;
     DevStatus* status;
 };
 
@@ -196,6 +198,11 @@ DSUF_DEV void pa_chunks(uint32_t tS, F f) {
         f(c, s[c & 1]);
     }
 }
+DSUF_DEV float pa_total(unsigned long long two) {
+    float x, y;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(two));
+    return x + y;
+}
 DSUF_DEV bool pa_seen(int col, int upper, int lower) { return col <= upper && col > lower; }
 // p = 2^(s sl2 - ref) of a row, packed to bf16 in w, and their sum.  MASK 0: all columns are visible, 1: those up to `upper`, 2: those above
 // `lower` as well.
@@ -221,9 +228,60 @@ DSUF_DEV float pa_weights(uint32_t tS, float sl2, float ref, int upper, int lowe
             w[c * 16 + e / 2] = pa_pack(x, y);
         }
     });
-    float x, y;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(sum2));
-    return x + y;
+    return pa_total(sum2);
+}
+
+// In the tiles that the diagonal or the window cuts, the tensor core multiplies hidden values with p = 0, and 0 x infinity is NaN.  A warp that finds
+// rows (bits of `rows`, the first at sequence row row0) with an output that is not finite comes here: where a hidden value of those tiles is not finite in
+// a column and no visible one of them is, the row is computed again from its visible rows alone, one key at a time.
+template <int D>
+__device__ __noinline__ void prompt_repair(const PromptArgs& a, unsigned rows, int row0, int start, int len, int head, int kvh, int lo) {
+    constexpr int V = D / 32;                        // columns of a lane
+    const int lane = threadIdx.x & 31;
+    const bf16* kb = a.k + (size_t)start * a.ldk + (size_t)kvh * D + lane * V;
+    const bf16* vb = a.v + (size_t)start * a.ldv + (size_t)kvh * D + lane * V;
+    for (; rows; rows &= rows - 1) {
+        const int i = row0 + __ffs(rows) - 1;
+        if (i >= len) continue;
+        const int from = a.window > 0 ? max(0, i - a.window + 1) : 0;
+        bf16* out = a.out + (size_t)(start + i) * a.ldo + (size_t)head * D + lane * V;
+        bool hidden[V], seen[V], wrong = false;
+#pragma unroll
+        for (int e = 0; e < V; ++e) hidden[e] = seen[e] = false;
+        const int tile0 = i / PA_BM * PA_BM;
+        for (int j = lo * PA_BM; j < min(len, tile0 + PA_BM); ++j) {
+            if (j == max(lo * PA_BM, (from / PA_BM + 1) * PA_BM) && j < tile0) j = tile0;      // (uncut tiles hide nothing)
+            const bool sees = j >= from && j <= i;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float x = __bfloat162float(vb[(size_t)j * a.ldv + e]);
+                if (!(fabsf(x) < INFINITY)) (sees ? seen[e] : hidden[e]) = true;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) wrong |= hidden[e] && !seen[e] && !(fabsf(__bfloat162float(out[e])) < INFINITY);
+        if (!__any_sync(0xffffffffu, wrong)) continue;
+        float q[V], o[V], top = PA_UNSET, sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            q[e] = __bfloat162float(a.q[(size_t)(start + i) * a.ldq + (size_t)head * D + lane * V + e]) * a.scale_log2;
+            o[e] = 0.f;
+        }
+        for (int j = from; j <= i; ++j) {
+            float s = 0.f;
+#pragma unroll
+            for (int e = 0; e < V; ++e) s += q[e] * __bfloat162float(kb[(size_t)j * a.ldk + e]);
+#pragma unroll
+            for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+            const float to = fmaxf(top, s), by = pa_exp2(top - to), w = pa_exp2(s - to);
+            top = to;
+            sum = sum * by + w;
+#pragma unroll
+            for (int e = 0; e < V; ++e) o[e] = o[e] * by + w * __bfloat162float(vb[(size_t)j * a.ldv + e]);
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) out[e] = __float2bfloat16(sum == 0.f ? 0.f : o[e] / sum);
+    }
 }
 
 template <int D>
@@ -509,12 +567,16 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
             // through shared memory, so that a store instruction writes four rows of 128 bytes instead of 32 pieces of 16
             const int row0 = q.qb * PA_BM + (warp & 3) * 32;      // the warp's first row
             bf16* dst = a.out + (size_t)(p.start + row0) * a.ldo + (size_t)q.head * D;
+            unsigned long long odd = pack_f32x2(0.f, 0.f);       // NaN once an output is not finite
 #pragma unroll
             for (int c = 0; c < D; c += 64) {
                 float o[64];
                 tmem_ld_issue<32>(tO + c, o);
                 tmem_ld_issue<32>(tO + c + 32, o + 32);
                 tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 64; e += 2)
+                    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(odd) : "l"(pack_f32x2(o[e], o[e + 1])), "l"(pack_f32x2(0.f, 0.f)));
 #pragma unroll
                 for (int e = 0; e < 64; e += 8)
                     *reinterpret_cast<uint4*>(stage + lane * 128 + (((e / 8) ^ (lane & 7)) << 4)) =
@@ -531,6 +593,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
                 }
                 __syncwarp();
             }
+            const unsigned again = __ballot_sync(0xffffffffu, live && !(pa_total(odd) == 0.f));
+            if (again) prompt_repair<D>(a, again, row0, p.start, p.len, q.head, p.kvh, q.lo);
             if (live && a.lse) a.lse[(size_t)(p.start + row) * a.q_heads + q.head] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
             tc_fence_before();
         }
@@ -586,7 +650,10 @@ extern "C" int32_t dsuf_attn_prompt(dsuf_ctx* ctx, void* stream, uint64_t q, int
     a.out = (bf16*)out; a.lse = (float*)lse; a.ldo = ldo; a.t = t;
     a.q_heads = q_heads; a.kv_heads = kv_heads; a.group = q_heads / kv_heads; a.n_seqs = n_seqs; a.window = window;
     a.cu = (const int*)cu_seqlens;
+    a.scale = scale;
     a.scale_log2 = scale * 1.4426950408889634f;
+    a.q = (const bf16*)q; a.k = (const bf16*)k; a.v = (const bf16*)v;
+    a.ldq = ldq; a.ldk = ldk; a.ldv = ldv;
     a.status = ctx->dev_status;
     // no more CTAs than pairs there can be (the lengths are only known on the device)
     const long long blocks = (long long)(t / PA_BM) + (t < n_seqs ? t : n_seqs);

@@ -440,8 +440,7 @@ int32_t dsuf_attn_decode(dsuf_ctx* ctx, void* stream, const dsuf_kv_cache* cache
  * of q, k, v, out are sequence i; row r of a sequence sees its rows max(0, r - window + 1) .. r (window 0: all up to r).
  * q / out bf16 [t][q_heads * head_dim], k / v bf16 [t][kv_heads * head_dim] (row strides ld*, so the parts of one merged projection can be
  * passed as they lie), lse f32 [t][q_heads] or 0.  Rows that belong to no sequence are left as they were, and nothing of them is
- * read into a result.  Inside a sequence the values must be finite: an infinity or NaN in v may reach every row of its 128-row block
- * (those of q and k stay with the rows that see them).  q_heads a multiple of kv_heads, head_dim 64 or 128. */
+ * read into a result; an infinity or NaN inside a sequence reaches the rows that see it, no others.  q_heads a multiple of kv_heads, head_dim 64 or 128. */
 int32_t dsuf_attn_prompt(dsuf_ctx* ctx, void* stream, uint64_t q, int32_t ldq, uint64_t k, int32_t ldk, uint64_t v, int32_t ldv, int32_t t,
                          int32_t q_heads, int32_t kv_heads, int32_t head_dim, uint64_t cu_seqlens, int32_t n_seqs, float scale,
                          int32_t window, uint64_t out, int32_t ldo, uint64_t lse);

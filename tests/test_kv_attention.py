@@ -470,3 +470,35 @@ def test_another_current_device_is_refused(pkg, actx):
     buf = C.create_string_buffer(512)
     L.dsuf_last_error(other, buf, 512)
     assert b"device 0 is current" in buf.value
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("window", [0, 70, 200])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_hidden_values_that_are_not_finite(pkg, actx, d, window, bad):
+    """Values of later tokens of the same sequence, and of tokens that the window has left behind, do not reach a row, whatever they are; those that
+    it sees do."""
+    g = gen(31)
+    lens, hq, hkv = [300, 131], 6, 2
+    t = sum(lens)
+    q, k, v = bf16(g, t, hq * d), bf16(g, t, hkv * d), bf16(g, t, hkv * d)
+    where = [(100, 0, 3), (290, 1, d - 1), (300 + 128, 0, 0), (5, 1, 7)]        # (row, kv head, column)
+    for r, h, c in where:
+        v[r, h * d + c] = bad
+    cu = torch.tensor([0, 300, t], dtype=torch.int32, device=DEV)
+    out = pkg.attn_prompt(actx, q, k, v, cu, head_dim=d, window=window)
+    clean = v.clone()
+    for r, h, c in where:
+        clean[r, h * d + c] = 0
+    want, _, size = prompt64(q, k, clean, lens, hq, hkv, d, window, d ** -0.5)
+    hit = torch.zeros(t, hq * d, dtype=torch.bool, device=DEV)
+    for r, h, c in where:
+        start, n = (0, 300) if r < 300 else (300, 131)
+        last = start + n if window == 0 else min(start + n, r + window)
+        for head in range(h * 3, h * 3 + 3):
+            hit[r:last, head * d + c] = True
+    assert torch.equal(~torch.isfinite(out), hit)
+    within(torch.where(hit, torch.zeros_like(out), out), torch.where(hit, 0.0, want), size, terms=2 ** -8 + 2 ** -12)
+    # and nothing changes where nothing is hidden: the clean input gives the same bits as before in rows without
+    assert actx.status().code == 0
