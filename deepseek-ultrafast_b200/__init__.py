@@ -169,6 +169,29 @@ def lib():
     return _LIB
 
 
+HOSTCALL_PATH = os.path.join(_HERE, "dsuf_hostcall.so")
+_HOSTCALL = None
+
+
+def hostcall():
+    """The module csrc/hostcall.cc: checks of the tensors, new results and the C call of kv_append, attn_decode, attn_prompt and sample in native code.
+    Raises if it has not been built."""
+    global _HOSTCALL
+    if _HOSTCALL is None:
+        import importlib.machinery
+        import importlib.util
+        import torch  # noqa: F401 - its libraries resolve the module's
+        if not os.path.exists(HOSTCALL_PATH):
+            raise DsufError(-2, f"{HOSTCALL_PATH} is missing: build it with `python deepseek-ultrafast_b200/build.py`")
+        spec = importlib.util.spec_from_file_location("dsuf_hostcall", HOSTCALL_PATH, loader=importlib.machinery.ExtensionFileLoader("dsuf_hostcall", HOSTCALL_PATH))
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        entries = ("dsuf_kv_append", "dsuf_attn_decode", "dsuf_attn_prompt", "dsuf_sample", "dsuf_last_error", "dsuf_attn_workspace_bytes")
+        mod.bind(DsufError, *(C.cast(getattr(lib(), n), C.c_void_p).value for n in entries))
+        _HOSTCALL = mod
+    return _HOSTCALL
+
+
 def _np_ptr(a):
     return None if a is None else a.ctypes.data_as(C.c_void_p)
 
@@ -300,7 +323,7 @@ class Ctx:
         rc = lib().dsuf_ctx_create(device, C.byref(h))
         if rc:
             raise DsufError(rc, "dsuf_ctx_create failed (needs an sm_100 GPU)")
-        self.h = h
+        self.h, self.address = h, h.value
         if pdl:
             self.check(lib().dsuf_ctx_set_pdl(self.h, 1))
         self.set_decode_path(tcgen05)
@@ -356,7 +379,7 @@ class Ctx:
     def close(self):
         if self.h:
             lib().dsuf_ctx_destroy(self.h)
-            self.h = None
+            self.h, self.address = None, 0
 
 
 class Weight:
@@ -614,38 +637,6 @@ def _need(cond, msg):
         raise DsufError(-1, msg)
 
 
-def _refuse(ctx, name, x, dtype, shape, rows):
-    if not isinstance(x, ctx.torch.Tensor) or x.device != ctx.device or x.dtype != dtype:
-        raise DsufError(-1, f"{name}: a {dtype} tensor on {ctx.device} is wanted")
-    raise DsufError(-1, f"{name}: shape {tuple(x.shape)} with strides {x.stride()}; wanted {shape}, " +
-                    ("rows contiguous and not overlapping" if rows else "contiguous"))
-
-
-def _vector(ctx, name, x, dtype, n=None):
-    """x is a contiguous vector (of n elements) of this type on the context's device."""
-    try:
-        ok = x.dtype is dtype and x.get_device() == ctx.index and x.dim() == 1 and (n is None or x.shape[0] == n) and x.is_contiguous()
-    except AttributeError:
-        ok = False
-    if not ok:
-        _refuse(ctx, name, x, dtype, (n,), False)
-
-
-def _rows(ctx, name, x, dtype, n=None, width=None):
-    """x is a matrix [n][width] of this type on the context's device whose rows may lie apart; returns its row stride."""
-    try:
-        m, w = x.shape
-        ld, one = x.stride()
-        if x.dtype is dtype and x.get_device() == ctx.index and (n is None or m == n) and (width is None or w == width):
-            if m < 2 or w == 0:
-                ld = w          # (a single row's stride says nothing)
-            if (one == 1 or w < 2 or m == 0) and ld >= w:
-                return ld
-    except (AttributeError, ValueError):
-        pass
-    _refuse(ctx, name, x, dtype, (n, width), True)
-
-
 class KvCache:
     """dsuf_kv_cache: one layer's paged cache over tensors k, v [n_pages][kv_heads][page_size][head_dim], bf16 or (uint8 codes)
     e4m3 with optional f32 scales per kv head.  The pages may lie apart (a slice of a tensor that holds all layers)."""
@@ -659,13 +650,14 @@ class KvCache:
             _need(x.stride()[1:] == (p * d, d, 1) and x.stride(0) == k.stride(0), f"KvCache: {name}: the heads of a page must be contiguous, k's and v's pages equally far apart")
         for name, x in (("k_scale", k_scale), ("v_scale", v_scale)):
             if x is not None:
-                _vector(ctx, "KvCache: " + name, x, t.float32, h)
+                _need(isinstance(x, t.Tensor) and x.device == ctx.device and x.dtype == t.float32 and x.shape == (h,) and x.is_contiguous(),
+                      f"KvCache: {name}: a contiguous f32 [kv_heads] is wanted")
         self.ctx, self.k, self.v, self.k_scale, self.v_scale = ctx, k, v, k_scale, v_scale   # (keeps the tensors alive)
         self.n_pages, self.kv_heads, self.page_size, self.head_dim = n, h, p, d
         self.c = KvCacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if k_scale is not None else 0,
                                v_scale.data_ptr() if v_scale is not None else 0, max(k.stride(0), h * p * d) if n > 1 else h * p * d,
                                KV_BF16 if k.dtype == t.bfloat16 else KV_E4M3, n, p, h, d)
-        self.ref = C.byref(self.c)
+        self.ref, self.address = C.byref(self.c), C.addressof(self.c)
 
     @staticmethod
     def empty(ctx, n_pages, page_size, kv_heads, head_dim, fp8=False, k_scale=None, v_scale=None):
@@ -676,13 +668,6 @@ class KvCache:
         return KvCache(ctx, k, v, k_scale, v_scale)
 
 
-def _table(ctx, who, table):
-    """(sequences, pages) of a contiguous block table."""
-    if _rows(ctx, who + ": block_table", table, ctx.torch.int32) != table.shape[1]:
-        raise DsufError(-1, who + ": block_table must be contiguous")
-    return table.shape
-
-
 def kv_append(ctx, cache, k, v, pos, block_table, seq=None, rope=None, rope_half=False, q=None, q_out=None, k_out=None):
     """dsuf_kv_append: writes the tokens' keys (rotated) and values bf16 [t][kv_heads * head_dim] into the cache at positions
     ``pos`` i32 [t] of sequences ``seq`` i32 [t] (None: token i is sequence i), pages from ``block_table`` i32 [seqs][pages]; a
@@ -690,39 +675,9 @@ def kv_append(ctx, cache, k, v, pos, block_table, seq=None, rope=None, rope_half
     (even, odd) pairs or with ``rope_half`` in pairs rot/2 apart.  ``q`` bf16 [t][q_heads * head_dim]: rotated as well, into
     ``q_out`` (None: a new tensor; q itself: in place).  ``k_out``: receives the rotated keys as rows, for attn_prompt over these tokens (k
     itself: in place).  Returns q_out."""
-    t = ctx.torch
-    _need(cache.ctx is ctx, "kv_append: the cache belongs to another context")
-    d = cache.head_dim
-    ldk = _rows(ctx, "kv_append: k", k, t.bfloat16, None, cache.kv_heads * d)
-    n = k.shape[0]
-    ldv = _rows(ctx, "kv_append: v", v, t.bfloat16, n, cache.kv_heads * d)
-    _vector(ctx, "kv_append: pos", pos, t.int32, n)
-    n_seqs, pages = _table(ctx, "kv_append", block_table)
-    if seq is not None:
-        _vector(ctx, "kv_append: seq", seq, t.int32, n)
-    r = None
-    if rope is not None:
-        cos, sin, off = rope
-        _need(_rows(ctx, "kv_append: cos", cos, t.float32) == cos.shape[1] == _rows(ctx, "kv_append: sin", sin, t.float32, *cos.shape),
-              "kv_append: cos and sin must be contiguous")
-        r = C.byref(RopeStruct(cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1], off, 1 if rope_half else 0))
-    heads = ldq = ldo = qp = op = 0
-    if q is not None:
-        ldq = _rows(ctx, "kv_append: q", q, t.bfloat16, n)
-        width = q.shape[1]
-        heads = width // d
-        _need(heads > 0 and heads * d == width, "kv_append: q's rows must hold whole heads")
-        if q_out is None:
-            q_out = q.new_empty((n, width))
-        ldo = _rows(ctx, "kv_append: q_out", q_out, t.bfloat16, n, width)
-        qp, op = q.data_ptr(), q_out.data_ptr()
-    kp = ldko = 0
-    if k_out is not None:
-        ldko = _rows(ctx, "kv_append: k_out", k_out, t.bfloat16, n, cache.kv_heads * d)
-        kp = k_out.data_ptr()
-    ctx.check(lib().dsuf_kv_append(ctx.h, ctx.stream(), cache.ref, k.data_ptr(), ldk, v.data_ptr(), ldv, n, pos.data_ptr(),
-                                   seq.data_ptr() if seq is not None else 0, block_table.data_ptr(), n_seqs, pages, r, qp, ldq, heads, op, ldo, kp, ldko))
-    return q_out
+    if cache.ctx is not ctx:
+        raise DsufError(-1, "kv_append: the cache belongs to another context")
+    return hostcall().kv_append(ctx.address, ctx.index, cache.address, k, v, pos, block_table, seq, rope, rope_half, q, q_out, k_out)
 
 
 def attn_decode(ctx, cache, q, block_table, seq_lens, scale=None, window=0, out=None, lse=None, return_lse=False, workspace=None):
@@ -730,31 +685,10 @@ def attn_decode(ctx, cache, q, block_table, seq_lens, scale=None, window=0, out=
     [max(0, len - window), len) with len = ``seq_lens`` i32 [b] (the new token included, its key already appended); ``scale`` None:
     head_dim ** -0.5.  Returns out bf16 [b][q_heads * head_dim], or (out, lse f32 [b][q_heads]) with ``return_lse``.
     ``workspace``: one of ctx.new_attn_workspace() for calls that may overlap others of this context."""
-    t = ctx.torch
-    _need(cache.ctx is ctx, "attn_decode: the cache belongs to another context")
-    d = cache.head_dim
-    ldq = _rows(ctx, "attn_decode: q", q, t.bfloat16)
-    b, width = q.shape
-    heads = width // d
-    _need(width > 0 and width % (d * cache.kv_heads) == 0, "attn_decode: q's rows must hold a multiple of kv_heads heads")
-    n_seqs, pages = _table(ctx, "attn_decode", block_table)
-    _need(n_seqs == b, "attn_decode: block_table holds one row per row of q")
-    _vector(ctx, "attn_decode: seq_lens", seq_lens, t.int32, b)
-    if out is None:
-        out = q.new_empty((b, width))
-    ldo = _rows(ctx, "attn_decode: out", out, t.bfloat16, b, width)
-    if lse is None and return_lse:
-        lse = q.new_empty((b, heads), dtype=t.float32)
-    if lse is not None:
-        _need(_rows(ctx, "attn_decode: lse", lse, t.float32, b, heads) == heads, "attn_decode: lse must be contiguous")
-    if workspace is None:
-        workspace = ctx.attn_workspace
-    else:
-        _vector(ctx, "attn_decode: workspace", workspace, t.uint8, ctx.attn_workspace.shape[0])
-    ctx.check(lib().dsuf_attn_decode(ctx.h, ctx.stream(), cache.ref, q.data_ptr(), ldq, heads, b, block_table.data_ptr(), pages, seq_lens.data_ptr(),
-                                     d ** -0.5 if scale is None else scale, window, out.data_ptr(), ldo, lse.data_ptr() if lse is not None else 0,
-                                     workspace.data_ptr()))
-    return (out, lse) if return_lse else out
+    if cache.ctx is not ctx:
+        raise DsufError(-1, "attn_decode: the cache belongs to another context")
+    return hostcall().attn_decode(ctx.address, ctx.index, cache.address, q, block_table, seq_lens, scale, window, out, lse, return_lse,
+                                  ctx.attn_workspace if workspace is None else workspace)
 
 
 def attn_prompt(ctx, q, k, v, cu_seqlens, head_dim=128, scale=None, window=0, out=None, lse=None, return_lse=False):
@@ -762,54 +696,14 @@ def attn_prompt(ctx, q, k, v, cu_seqlens, head_dim=128, scale=None, window=0, ou
     rows may be parts of a merged projection's), ``cu_seqlens`` i32 [sequences + 1]; ``window`` > 0: a row sees that many rows, itself
     included.  ``scale`` None: head_dim ** -0.5.  Rows behind the last sequence are not written.  Returns out bf16
     [t][q_heads * head_dim], or (out, lse f32 [t][q_heads]) with ``return_lse``."""
-    t = ctx.torch
-    _need(head_dim in (64, 128), "attn_prompt: head_dim is 64 or 128")
-    ldq = _rows(ctx, "attn_prompt: q", q, t.bfloat16)
-    n, width = q.shape
-    ldk = _rows(ctx, "attn_prompt: k", k, t.bfloat16, n)
-    ldv = _rows(ctx, "attn_prompt: v", v, t.bfloat16, n, k.shape[1])
-    heads, kv_heads = width // head_dim, k.shape[1] // head_dim
-    _need(heads * head_dim == width and kv_heads * head_dim == k.shape[1], "attn_prompt: rows hold whole heads")
-    _vector(ctx, "attn_prompt: cu_seqlens", cu_seqlens, t.int32)
-    _need(cu_seqlens.shape[0] >= 1, "attn_prompt: cu_seqlens holds at least one entry")
-    if out is None:
-        out = q.new_empty((n, width))
-    ldo = _rows(ctx, "attn_prompt: out", out, t.bfloat16, n, width)
-    if lse is None and return_lse:
-        lse = q.new_empty((n, heads), dtype=t.float32)
-    if lse is not None:
-        _need(_rows(ctx, "attn_prompt: lse", lse, t.float32, n, heads) == heads, "attn_prompt: lse must be contiguous")
-    ctx.check(lib().dsuf_attn_prompt(ctx.h, ctx.stream(), q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, n, heads, kv_heads, head_dim,
-                                     cu_seqlens.data_ptr(), cu_seqlens.shape[0] - 1, head_dim ** -0.5 if scale is None else scale, window,
-                                     out.data_ptr(), ldo, lse.data_ptr() if lse is not None else 0))
-    return (out, lse) if return_lse else out
+    return hostcall().attn_prompt(ctx.address, ctx.index, q, k, v, cu_seqlens, head_dim, scale, window, out, lse, return_lse)
 
 
 def sample(ctx, logits, u, temperature=None, top_k=None, top_p=None, min_p=None, ids=None, logprobs=None, return_logprobs=False):
     """dsuf_sample: one token per row of fp32 ``logits`` [m][n] (lm_head's) from the given uniform numbers ``u`` f32 [m] in [0, 1), after
     temperature, top-k, top-p and min-p (tensors of one value per row; None: off; see include/dsuf_qmm.h for the order and ties).
     Returns ids i32 [m], or (ids, logprobs f32 [m]) with ``return_logprobs``: the raw log-probabilities of the drawn tokens."""
-    t = ctx.torch
-    ld = _rows(ctx, "sample: logits", logits, t.float32)
-    m, n = logits.shape
-    _vector(ctx, "sample: u", u, t.float32, m)
-    ptrs = []
-    for name, x, dtype in (("sample: temperature", temperature, t.float32), ("sample: top_k", top_k, t.int32), ("sample: top_p", top_p, t.float32),
-                           ("sample: min_p", min_p, t.float32)):
-        if x is not None:
-            _vector(ctx, name, x, dtype, m)
-        ptrs.append(0 if x is None else x.data_ptr())
-    if ids is None:
-        ids = u.new_empty(m, dtype=t.int32)
-    else:
-        _vector(ctx, "sample: ids", ids, t.int32, m)
-    if logprobs is None and return_logprobs:
-        logprobs = u.new_empty(m)
-    if logprobs is not None:
-        _vector(ctx, "sample: logprobs", logprobs, t.float32, m)
-    ctx.check(lib().dsuf_sample(ctx.h, ctx.stream(), logits.data_ptr(), ld, m, n, *ptrs, u.data_ptr(), ids.data_ptr(),
-                                logprobs.data_ptr() if logprobs is not None else 0))
-    return (ids, logprobs) if return_logprobs else ids
+    return hostcall().sample(ctx.address, ctx.index, logits, u, temperature, top_k, top_p, min_p, ids, logprobs, return_logprobs)
 
 
 def probe_tensor_rate(ctx, n_cols=128, a_is_e2m1=False, iters=20000, reps=5):

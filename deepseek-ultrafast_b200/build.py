@@ -1,4 +1,4 @@
-"""In-tree build of libdsuf_qmm.so (nvcc, sm_100a only).
+"""In-tree build of libdsuf_qmm.so (nvcc, sm_100a only) and of the Python module dsuf_hostcall.so (g++).
 
 ``python deepseek-ultrafast_b200/build.py`` or ``build()`` from Python.  Objects are cached under
 ``csrc/build/`` and rebuilt when a source or header is newer.
@@ -11,6 +11,7 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libdsuf_qmm.so")
+HOSTCALL = os.path.join(HERE, "dsuf_hostcall.so")
 SOURCES = ["abi.cu", "quant.cu", "moe_aux.cu", "stream_launch.cu", "noalloc.cu", "ep_comm.cu", "peak_probe.cu", "lm_head.cu", "kv_cache.cu", "attn_decode.cu", "attn_prompt.cu", "sample.cu", "pack.cc", "loader.cc"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC",
@@ -33,6 +34,27 @@ def _compile(src, obj, log):
         f.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)
     if r.returncode != 0:
         raise RuntimeError(f"nvcc failed on {src}:\n{r.stdout}\n{r.stderr}")
+
+
+def build_hostcall():
+    """dsuf_hostcall.so: the Python entries that check tensors and call the library in native code (csrc/hostcall.cc), against the torch and Python
+    that run this."""
+    import sysconfig
+    import torch
+    src, header = os.path.join(CSRC, "hostcall.cc"), os.path.join(HERE, "..", "include", "dsuf_qmm.h")
+    if os.path.exists(HOSTCALL) and os.path.getmtime(HOSTCALL) >= max(os.path.getmtime(src), os.path.getmtime(header)):
+        return HOSTCALL
+    root = os.path.dirname(torch.__file__)
+    includes = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include")]
+    cuda = os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", cuda,
+           "-I", sysconfig.get_paths()["include"], *[x for d in includes for x in ("-isystem", d)], src, "-o", HOSTCALL + ".tmp",
+           "-L", os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("g++ failed on hostcall.cc:\n" + r.stderr)
+    os.replace(HOSTCALL + ".tmp", HOSTCALL)
+    return HOSTCALL
 
 
 def build(verbose=False):
@@ -58,6 +80,7 @@ def build(verbose=False):
         if r.returncode != 0:
             raise RuntimeError("link failed:\n" + r.stdout + r.stderr)
         os.replace(OUT + ".tmp", OUT)
+    build_hostcall()
     if verbose:
         for s, _, log in jobs:
             print(open(log).read())

@@ -502,3 +502,15 @@ def test_hidden_values_that_are_not_finite(pkg, actx, d, window, bad):
     within(torch.where(hit, torch.zeros_like(out), out), torch.where(hit, 0.0, want), size, terms=2 ** -8 + 2 ** -12)
     # and nothing changes where nothing is hidden: the clean input gives the same bits as before in rows without
     assert actx.status().code == 0
+
+
+@gpu
+def test_a_closed_context_is_refused(pkg, actx):
+    c = pkg.Ctx(0)
+    cache = pkg.KvCache.empty(c, 2, 16, 1, 64)
+    q, i = bf16(gen(1), 1, 64), torch.zeros(1, dtype=torch.int32, device=DEV)
+    c.close()
+    for call in (lambda: pkg.kv_append(c, cache, q, q, i, i.reshape(1, 1)), lambda: pkg.attn_decode(c, cache, q, i.reshape(1, 1), i),
+                 lambda: pkg.attn_prompt(c, q, q, q, torch.zeros(2, dtype=torch.int32, device=DEV), head_dim=64), lambda: pkg.sample(c, q.float(), q[0, :1].float())):
+        with pytest.raises(pkg.DsufError):
+            call()

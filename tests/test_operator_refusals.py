@@ -102,28 +102,57 @@ def test_sample_refuses(pkg, cctx):
     assert call(m=0, logits=0, u=0, ids=0) == 0
 
 
-def test_the_mirror_refuses(pkg):
+def test_the_mirror_refuses(pkg, cctx):
     """Shapes, types, devices and strides, on CPU tensors with a stand-in for the context."""
     dev = torch.device("cpu")
-    ctx = types.SimpleNamespace(torch=torch, device=dev, index=-1)
+    address = C.addressof(cctx)
+    space = torch.zeros(16, dtype=torch.uint8)
+    ctx = types.SimpleNamespace(torch=torch, device=dev, index=-1, address=address, attn_workspace=space)
     E = pkg.DsufError
     z = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt)   # noqa: E731
+    i = lambda *s: z(*s, dt=torch.int32)   # noqa: E731
     for a in [(z(4, 2, 16),) * 2, (z(4, 2, 16, 128, dt=torch.float32),) * 2, (z(4, 2, 16, 128), z(4, 2, 16, 64)), (z(4, 16, 2, 128).transpose(1, 2),) * 2,
               (z(4, 2, 16, 128), z(8, 2, 16, 128)[::2]), (z(4, 2, 16, 128, dt=torch.uint8),) * 2 + (z(2),)]:
         with pytest.raises(E):
             pkg.KvCache(ctx, *a)
     c = pkg.KvCache(ctx, z(8, 2, 16, 128)[::2], z(8, 2, 16, 128)[::2])
     assert c.c.page_stride == 2 * 2 * 16 * 128 and (c.n_pages, c.kv_heads, c.page_size, c.head_dim) == (4, 2, 16, 128)
-    assert pkg._rows(ctx, "x", z(3, 10)[:, :8], torch.bfloat16, 3, 8) == 10
-    assert pkg._rows(ctx, "x", z(1, 8).as_strided((1, 8), (3, 1)), torch.bfloat16) == 8
-    for x in (z(3, 8).t(), z(3), z(2, 8).as_strided((2, 8), (4, 1)), z(3, 8, dt=torch.float16), None, 3):
+    good = (z(3, 256), z(3, 256), i(3), i(3, 1))
+    for at, bad in [(0, z(3, 256, dt=torch.float16)), (0, z(256, 3).t()), (0, z(3, 128)), (0, z(768)), (0, z(2, 256).as_strided((2, 256), (128, 1))), (0, None), (0, 3), (1, z(2, 256)),
+                    (2, i(4)), (2, i(6)[::2]), (2, i(3, 1)), (2, z(3, dt=torch.int64)), (3, i(3)), (3, i(3, 4)[:, :2]), (3, z(3, 1))]:
+        with pytest.raises(E, match="kv_append"):
+            pkg.kv_append(ctx, c, *(bad if n == at else x for n, x in enumerate(good)))
+    for kw in [dict(seq=i(2)), dict(rope=(1, 2)), dict(rope=3), dict(rope=(z(4, 64), z(4, 64), 0)), dict(rope=(z(4, 64, dt=torch.float32), z(4, 32, dt=torch.float32), 0)),
+               dict(rope=(z(4, 64, dt=torch.float32),) * 2 + ("x",)), dict(rope=(z(4, 64, dt=torch.float32),) * 2 + (1 << 40,)), dict(q=z(3, 100)), dict(q=z(3, 0)), dict(q=z(3, 256), q_out=z(3, 128)),
+               dict(k_out=z(2, 256))]:
         with pytest.raises(E):
-            pkg._rows(ctx, "x", x, torch.bfloat16)
-    for x in (z(3, 1), z(6)[::2], z(4), z(3, dt=torch.float32), None):
-        with pytest.raises(E):
-            pkg._vector(ctx, "x", x, torch.bfloat16, 3)
-    other = types.SimpleNamespace(torch=torch, device=dev, index=-1)
-    with pytest.raises(E):
-        pkg.attn_decode(other, c, z(1, 512), z(1, 1, dt=torch.int32), z(1, dt=torch.int32))
-    with pytest.raises(E):
-        pkg.attn_prompt(ctx, z(3, 512), z(3, 256), z(3, 256), z(2, dt=torch.int32), head_dim=100)
+            pkg.kv_append(ctx, c, *good, **kw)
+    other = types.SimpleNamespace(**vars(ctx))
+    with pytest.raises(E, match="another context"):
+        pkg.attn_decode(other, c, z(1, 512), i(1, 1), i(1))
+    with pytest.raises(E, match="another context"):
+        pkg.kv_append(other, c, *good)
+    for a, kw in [((z(1, 384), i(1, 1), i(1)), {}), ((z(1, 512), i(2, 1), i(1)), {}), ((z(1, 512), i(1, 1), i(2)), {}), ((z(1, 512), i(1, 1), i(1)), dict(scale="x")),
+                  ((z(1, 512), i(1, 1), i(1)), dict(window=1.5)), ((z(1, 512), i(1, 1), i(1)), dict(window=1 << 40)), ((z(1, 512), i(1, 1), i(1)), dict(workspace=z(3)))]:
+        with pytest.raises(E, match="attn_decode"):
+            pkg.attn_decode(ctx, c, *a, **kw)
+    for a, kw in [((z(3, 512), z(3, 256), z(3, 256), i(2)), dict(head_dim=100)), ((z(3, 500), z(3, 256), z(3, 256), i(2)), {}), ((z(3, 512), z(3, 256), z(3, 128), i(2)), {}),
+                  ((z(3, 512), z(3, 256), z(3, 256), i(0)), {}), ((z(3, 512), z(3, 256), z(3, 256), i(2)), dict(out=z(3, 256))),
+                  ((z(3, 512), z(3, 256), z(3, 256), i(2)), dict(lse=z(3, 4))), ((z(3, 512), z(3, 256), z(3, 256), i(2)), dict(head_dim="a"))]:
+        with pytest.raises(E, match="attn_prompt"):
+            pkg.attn_prompt(ctx, *a, **kw)
+    f = z(3, dt=torch.float32)
+    for a, kw in [((z(3, 9), f), {}), ((z(3, 9, dt=torch.float32), f[:2]), {}), ((z(9, 3, dt=torch.float32).t(), f), {}), ((z(3, 9, dt=torch.float32), f), dict(top_k=f)),
+                  ((z(3, 9, dt=torch.float32), f), dict(ids=f)), ((z(3, 9, dt=torch.float32), f), dict(logprobs=i(3)))]:
+        with pytest.raises(E, match="sample"):
+            pkg.sample(ctx, *a, **kw)
+    with pytest.raises(TypeError):
+        pkg.hostcall().sample(1, 2)
+    # a single row's stride says nothing; an empty batch is no error and touches nothing
+    assert pkg.kv_append(ctx, c, z(0, 256), z(0, 256), i(0), i(0, 1), q=z(0, 512)).shape == (0, 512)
+    out, lse = pkg.attn_prompt(ctx, z(0, 512), z(0, 256), z(0, 256), i(1), return_lse=True)
+    assert out.shape == (0, 512) and lse.shape == (0, 4)
+    ids, lp = pkg.sample(ctx, z(0, 9, dt=torch.float32), f[:0], return_logprobs=True)
+    assert ids.dtype == torch.int32 and lp.shape == (0,)
+    mine = z(0, 512)
+    assert pkg.attn_prompt(ctx, z(0, 512), z(0, 256), z(0, 256), i(1), out=mine) is mine
