@@ -10,7 +10,10 @@
 // known on the host (a captured graph replays with new ones).  A piece inside one CTA is finished there; a piece cut by range
 // ends leaves fp32 partials (output, reference point, sum) in the workspace and the CTA that arrives last adds them in CTA order,
 // so the result does not depend on timing.  Where there are few units, segments of four of one piece are dealt instead of units (8 contexts
-// of 1000 tokens, 56 / 8 heads of 128: 12.8 us instead of 14.5; one of 16000, one kv head: 14.0 instead of 24.6).
+// of 1000 tokens, 56 / 8 heads of 128: 12.8 us instead of 14.5; one of 16000, one kv head: 14.0 instead of 24.6).  Where every piece is short (four
+// units at most) and there is one for each CTA, a warp takes whole pieces alone and writes them itself: no barrier and no other warp's part to add
+// (56 / 8 heads of 128; 512 contexts of 128 tokens: 56 us instead of 68; 256 of 1 to 256: 37 instead of 61; 64 of 40: 7.6 instead of 10; with half as many pieces
+// as CTAs it would lose: 32 of 100 tokens 9.6 instead of 7.6).
 //
 // Inside a CTA every warp runs alone: a private ring of three stages (4 KB keys + 4 KB values each, cp.async, zero-filled
 // outside the visible range so that stale values behind a sequence cannot reach the sums), no barrier until the end of a
@@ -40,6 +43,7 @@ constexpr int AD_RING = AD_WARPS * AD_STAGES * 2 * AD_HALF;
 constexpr int AD_PART = 16 * 128;                          // floats of one partial output
 constexpr int AD_JOIN = 16;                                // partials whose loads are in flight together when a piece is joined
 constexpr int AD_SEGMENT_SHIFT = 2;                        // log2 of the units of a segment when there are few
+constexpr unsigned AD_SOLO_UNITS = 4, AD_SOLO_PIECES = 1;    // a warp per piece: pieces of at most so many units, at least so many per CTA
 constexpr float AD_UNSET = -1e30f;
 constexpr float AD_TRIGGER = 15.f, AD_HEADROOM = 7.f;
 
@@ -111,7 +115,9 @@ struct DecodeShape {
     static constexpr int ROW = D * (FP8 ? 1 : 2);          // bytes of a token's key
     static constexpr int CH = AD_HALF / ROW;               // tokens of a warp's stage
     static constexpr int SUBS = CH / 16;
+    static constexpr int CH_SHIFT = CH == 16 ? 4 : CH == 32 ? 5 : 6;
     static constexpr int UNIT = AD_WARPS * CH;
+    static_assert(CH == 1 << CH_SHIFT && AD_WARPS == 4, "units are powers of two");
     static constexpr int PIECES = ROW / 16;                // 16-byte columns of a row
     static constexpr int ROWS = 8 * NT;                    // query heads of a block
     static constexpr int SMEM = AD_RING + AD_WARPS * 8 * D * 4;
@@ -131,23 +137,22 @@ struct UnitAt {
     int seq, hb, u, nu, beg, len;
 };
 
-template <int UNIT>
-DSUF_DEV void visible_range(const DecodeArgs& a, int seq, int& beg, int& len, int& nu) {
+// (units of 2^unit tokens)
+DSUF_DEV void visible_range(const DecodeArgs& a, int seq, int unit, int& beg, int& len, int& nu) {
     len = seq < a.b ? __ldg(a.lens + seq) : 0;
     const int cap = a.max_pages << a.page_shift;
     len = min(max(len, 0), cap);
     beg = a.window > 0 ? max(0, len - a.window) : 0;
-    nu = len > 0 ? (len - (beg & ~15) + UNIT - 1) / UNIT : 0;
+    nu = len > 0 ? (len - (beg & ~15) + (1 << unit) - 1) >> unit : 0;
 }
-template <int UNIT>
-DSUF_DEV void next_unit(const DecodeArgs& a, UnitAt& p) {
+DSUF_DEV void next_unit(const DecodeArgs& a, UnitAt& p, int unit) {
     if (++p.u < p.nu) return;
     p.u = 0;
     if (++p.hb < a.kv_heads * a.blocks) return;
     p.hb = 0;
     do {
         ++p.seq;
-        visible_range<UNIT>(a, p.seq, p.beg, p.len, p.nu);
+        visible_range(a, p.seq, unit, p.beg, p.len, p.nu);
     } while (p.seq < a.b && p.nu == 0);
 }
 
@@ -255,17 +260,20 @@ __global__ void __launch_bounds__(AD_THREADS, 2) attn_decode_kernel(const Decode
     pdl_wait();
     pdl_launch_dependents();
 
-    // What is dealt are segments of 2^seg units (1, or 2^AD_SEGMENT_SHIFT where the GPU would get fewer than that many units per CTA: then a piece's parts
-    // begin with the CTAs, few have to be joined, and a short piece stays whole).  Every warp finds the CTA's range by itself: the lanes sum up
-    // a share of the sequences each.  (All numbers of units are below 2^31: the host has seen to that.)
+    // What is dealt are segments of 2^seg units: of one unit; of 2^AD_SEGMENT_SHIFT where the GPU would get fewer than that many units per CTA (then a
+    // piece's parts begin with the CTAs, few have to be joined, and a short piece stays whole); of whole pieces, and to warps instead of CTAs
+    // (`solo`: a unit is then the CH tokens of one warp), where all pieces are short and many.  Every warp finds its range by itself: the lanes sum
+    // up a share of the sequences each.  (All numbers of units are below 2^31: the host has seen to that.)
     const int HB = a.kv_heads * a.blocks;
     const int share = (a.b + 31) / 32, i0 = min(a.b, lane * share), i1 = min(a.b, i0 + share);
-    auto sum_up = [&](int seg, unsigned& mine) {
-        mine = 0;
+    unsigned mine, longest;
+    auto sum_up = [&](int unit, int seg) {
+        mine = longest = 0;
         for (int i = i0; i < i1; ++i) {
             int beg, len, nu;
-            visible_range<S::UNIT>(a, i, beg, len, nu);
+            visible_range(a, i, unit, beg, len, nu);
             mine += (unsigned)(((nu + (1 << seg) - 1) >> seg) * HB);
+            longest = max(longest, (unsigned)nu);
         }
         unsigned upto = mine;
 #pragma unroll
@@ -275,19 +283,35 @@ __global__ void __launch_bounds__(AD_THREADS, 2) attn_decode_kernel(const Decode
         }
         return upto;
     };
-    unsigned mine, upto = sum_up(0, mine);
+    int unit = S::CH_SHIFT + 2, seg = 0;
+    unsigned upto = sum_up(unit, 0);
     const bool few = __shfl_sync(0xffffffffu, upto, 31) < gridDim.x << AD_SEGMENT_SHIFT;
-    const int seg = few ? AD_SEGMENT_SHIFT : 0;
-    if (few) upto = sum_up(seg, mine);
+    bool solo = (unsigned)(a.b * HB) >= AD_SOLO_PIECES * gridDim.x && __reduce_max_sync(0xffffffffu, longest) <= AD_SOLO_UNITS;
+    if (solo) {
+        const unsigned pieces = sum_up(unit, 20);
+        solo = __shfl_sync(0xffffffffu, pieces, 31) >= AD_SOLO_PIECES * gridDim.x;
+        upto = pieces;
+    }
+    if (solo) {
+        unit = S::CH_SHIFT;
+        seg = 20;
+    } else if (few) {
+        seg = AD_SEGMENT_SHIFT;
+        upto = sum_up(unit, seg);
+    } else {
+        upto = sum_up(unit, 0);
+    }
+    const int own = solo ? 0 : warp * S::CH;            // the warp's tokens inside a unit
     const unsigned total = __shfl_sync(0xffffffffu, upto, 31);
-    const unsigned used = min(gridDim.x, total);        // CTAs that get work
-    if (blockIdx.x >= used) {
+    const unsigned worker = solo ? warp * gridDim.x + blockIdx.x : blockIdx.x, workers = solo ? gridDim.x * AD_WARPS : gridDim.x;
+    const unsigned used = min(workers, total);          // CTAs, or warps, that get work
+    if (worker >= used) {
         empty_rows<D>(a);
         return;
     }
     // the first `more` CTAs take base + 1 segments, the others base
     const unsigned base = total / used, more = total % used;
-    const unsigned s0 = base * blockIdx.x + min(blockIdx.x, more), s1 = s0 + base + (blockIdx.x < more ? 1 : 0);
+    const unsigned s0 = base * worker + min(worker, more), s1 = s0 + base + (worker < more ? 1 : 0);
     auto cta_of = [&](unsigned segment) {
         const unsigned cut = more * (base + 1);
         return segment < cut ? segment / (base + 1) : more + (segment - cut) / base;
@@ -301,7 +325,7 @@ __global__ void __launch_bounds__(AD_THREADS, 2) attn_decode_kernel(const Decode
             at.seq = i0;
             unsigned n;
             for (;;) {
-                visible_range<S::UNIT>(a, at.seq, at.beg, at.len, at.nu);
+                visible_range(a, at.seq, unit, at.beg, at.len, at.nu);
                 n = (unsigned)((at.nu + (1 << seg) - 1) >> seg);
                 if (left < n * HB) break;
                 left -= n * HB;
@@ -327,14 +351,14 @@ __global__ void __launch_bounds__(AD_THREADS, 2) attn_decode_kernel(const Decode
     struct Pages { int id[S::SUBS]; };
     auto look_up = [&](const UnitAt& p) {
         Pages r;
-        const int t0 = (p.beg & ~15) + p.u * S::UNIT + warp * S::CH;
+        const int t0 = (p.beg & ~15) + (p.u << unit) + own;
 #pragma unroll
         for (int s = 0; s < S::SUBS; ++s)
             r.id[s] = t0 + 16 * s < p.len ? __ldg(a.table + (size_t)p.seq * a.max_pages + ((t0 + 16 * s) >> a.page_shift)) : 0;
         return r;
     };
     auto issue = [&](const UnitAt& p, int stage, const Pages& pages) {
-        const int t0 = (p.beg & ~15) + p.u * S::UNIT + warp * S::CH;
+        const int t0 = (p.beg & ~15) + (p.u << unit) + own;
         const int kvh = p.hb / a.blocks;
         const uint32_t kdst = ring + stage * 2 * AD_HALF, vdst = kdst + AD_HALF;
 #pragma unroll
@@ -366,7 +390,7 @@ __global__ void __launch_bounds__(AD_THREADS, 2) attn_decode_kernel(const Decode
     unsigned to_load = s1 - s0, to_do = to_load;
     auto step = [&](UnitAt& p) {
         const bool ends = p.u + 1 == p.nu || ((p.u + 1) & ((1 << seg) - 1)) == 0;
-        next_unit<S::UNIT>(a, p);
+        next_unit(a, p, unit);
         return ends ? 1u : 0u;
     };
     int fill = 0, use = 0;
@@ -453,8 +477,8 @@ __global__ void __launch_bounds__(AD_THREADS, 2) attn_decode_kernel(const Decode
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[ks][nt][e] = 0.f;
         }
-        int t0 = (at.beg & ~15) + at.u * S::UNIT + warp * S::CH;
-        for (int f = 0; f < frag; ++f, t0 += S::UNIT) {
+        int t0 = (at.beg & ~15) + (at.u << unit) + own;
+        for (int f = 0; f < frag; ++f, t0 += 1 << unit) {
             cp_async_wait<AD_STAGES - 2>();
             __syncwarp();   // the stage is full, and every lane is through with the stage that is filled next
             if (to_load > 0) {
@@ -589,13 +613,52 @@ __global__ void __launch_bounds__(AD_THREADS, 2) attn_decode_kernel(const Decode
             }
         }
 
+        const float out_scale = FP8 && a.v_scale ? __ldg(a.v_scale + kvh) : 1.f;
+        if (solo) {
+            // ---------------- the warp's own piece ----------------
+            float* mw = merge + warp * 8 * D;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                if (nt * 8 >= heads) break;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float l = sum[nt][e];
+                    l += __shfl_xor_sync(0xffffffffu, l, 4);
+                    l += __shfl_xor_sync(0xffffffffu, l, 8);
+                    l += __shfl_xor_sync(0xffffffffu, l, 16);
+                    const float inv = l == 0.f ? 0.f : out_scale / l;
+                    const int h = nt * 8 + 2 * quad + e;
+                    if (a.lse && row8 == 0 && h < heads) a.lse[(size_t)at.seq * a.q_heads + head0 + h] = l == 0.f ? -INFINITY : (ref[nt][e] + log2f(l)) * 0.6931471805599453f;
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            const int col = FP8 ? ks * 16 + 2 * row8 + half : ks * 16 + row8 + 8 * half;
+                            mw[(2 * quad + e) * D + col] = o[ks][nt][e + 2 * half] * inv;
+                        }
+                }
+                __syncwarp();
+#pragma unroll
+                for (int i = lane; i < 8 * D / 4; i += 32) {
+                    const int r = i / (D / 4), c = (i % (D / 4)) * 4;
+                    const float4 v = *reinterpret_cast<const float4*>(mw + r * D + c);
+                    if (nt * 8 + r < heads)
+                        *reinterpret_cast<uint2*>(a.out + (size_t)at.seq * a.ldo + (size_t)(head0 + nt * 8 + r) * D + c) =
+                            make_uint2(pack2<false>(v.x, v.y), pack2<false>(v.z, v.w));
+                }
+                __syncwarp();
+            }
+            to_do -= segs;
+            at.u += frag - 1;
+            next_unit(a, at, unit);
+            continue;
+        }
         // ---------------- the four warps' parts of the piece ----------------
         const bool whole = frag == at.nu;
         const bool leads = at.u + frag < at.nu && at.u == 0;     // first CTA of a cut piece: its second slot
         const unsigned piece0 = s1 - to_do - seg_at;             // the piece's first segment
         float* part = a.part + ((size_t)blockIdx.x * 2 + (leads ? 1 : 0)) * AD_PART;
         float* part_ml = a.part_ml + ((size_t)blockIdx.x * 2 + (leads ? 1 : 0)) * 32;
-        const float out_scale = FP8 && a.v_scale ? __ldg(a.v_scale + kvh) : 1.f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             if (nt * 8 >= heads) break;
@@ -665,7 +728,7 @@ __global__ void __launch_bounds__(AD_THREADS, 2) attn_decode_kernel(const Decode
         }
         to_do -= segs;
         at.u += frag - 1;
-        next_unit<S::UNIT>(a, at);
+        next_unit(a, at, unit);
     }
     cp_async_wait<0>();
     empty_rows<D>(a);

@@ -349,6 +349,42 @@ def test_many_sequences(pkg, actx):
 
 
 @gpu
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("d,hq,hkv,window", [(128, 56, 8, 0), (128, 12, 1, 0), (64, 34, 2, 70), (64, 3, 3, 1)])
+@pytest.mark.parametrize("most", [1, 17, 65, 256])
+def test_many_short_sequences(pkg, actx, fp8, d, hq, hkv, window, most):
+    """Enough short contexts for every SM: each of 0 to `most` tokens."""
+    lens = [(37 * i) % (most + 1) for i in range(600)]
+    cache, q, table, n = decode_inputs(pkg, actx, 21 + most, lens, hq, hkv, d, 16, fp8)
+    out, lse = pkg.attn_decode(actx, cache, q, table, n, window=window, return_lse=True)
+    torch.cuda.synchronize()
+    assert actx.status().code == 0
+    want, wl, size = decode64(cache, q, table, lens, window, d ** -0.5)
+    within(out, want, size, terms=2 ** -8 + 2 ** -12)
+    live = wl > -math.inf
+    assert torch.equal(live, lse > -math.inf)
+    assert ((lse.double() - wl)[live].abs() <= 2 ** -12 + 2 ** -22 * wl[live].abs()).all()
+
+
+@gpu
+def test_every_bad_length_is_reported(pkg, actx):
+    """One length beyond its table among many short contexts, wherever it stands, is cut to the table and reported."""
+    lens = [5] * 600
+    cache, q, table, n = decode_inputs(pkg, actx, 31, lens, 7, 1, 64, 16, False)
+    want = pkg.attn_decode(actx, cache, q, table, n)
+    table = table[:, :1].contiguous()
+    for at in (0, 1, 299, 599):
+        n[at] = 17
+        got = pkg.attn_decode(actx, cache, q, table, n)
+        with pytest.raises(pkg.DsufError, match="status 2 from kernel 8"):
+            actx.status()
+        n[at] = 16
+        assert torch.equal(got, pkg.attn_decode(actx, cache, q, table, n)) and actx.status().code == 0
+        n[at] = 5
+    assert torch.equal(want, pkg.attn_decode(actx, cache, q, table, n))
+
+
+@gpu
 def test_bad_pages_and_lengths_are_reported(pkg, actx):
     cache, q, table, n = decode_inputs(pkg, actx, 12, [100, 40], 4, 2, 128, 16, False)
     good = pkg.attn_decode(actx, cache, q, table, n)
