@@ -561,8 +561,8 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleArgs 
         return;               // (all CTAs of the row alike, and nobody reads remote memory any more)
     }
     const double inv = greedy ? 1.0 : 1.4426950408889634 / (double)temp;
-    z.inv_temp = (float)inv;
-    z.inv_temp_rest = isinf(z.inv_temp) ? 0.f : (float)(inv - (double)z.inv_temp);
+    z.inv_temp = (float)fmin(inv, 3.4028234663852886e38);      // (finite, so that the top's weight is 1 at any temperature)
+    z.inv_temp_rest = inv > 3.4028234663852886e38 ? 0.f : (float)(inv - (double)z.inv_temp);
     const float span = fmaxf(24.f, 32.f * temp);
     z.inv_bin = span < INFINITY ? (float)(SA_BINS - 1) / span : 0.f;
 

@@ -157,6 +157,20 @@ def test_infinite_and_missing_logits(pkg, sctx):
 
 
 @gpu
+@pytest.mark.parametrize("temp", [1.4e-45, 1e-40, 4e-39, 1.2e-38, 1e-30])
+@pytest.mark.parametrize("kw", [{}, dict(top_k=3), dict(top_k=2000), dict(top_p=0.7), dict(min_p=0.5)])
+def test_temperatures_next_to_nothing(pkg, sctx, temp, kw):
+    """Only the largest logits are left, as likely as each other, down to the smallest temperature that fp32 has."""
+    x = torch.randn(4, 5000, generator=torch.Generator(device=DEV).manual_seed(3), device=DEV)
+    x[:, 700] = x[:, 4100] = 9.0
+    u = torch.tensor([0.0, 0.2, 0.9, 0.999], device=DEV)
+    full = lambda v: torch.full((4,), v, dtype=torch.int32 if isinstance(v, int) else torch.float32, device=DEV)
+    got = torch.full((4,), -7, dtype=torch.int32, device=DEV)
+    pkg.sample(sctx, x, u, temperature=full(temp), ids=got, **{k: full(v) for k, v in kw.items()})
+    assert got.tolist() == [700, 700, 4100, 4100]
+
+
+@gpu
 def test_defaults_and_frequencies(pkg, sctx):
     """Without settings the draw follows softmax(logits): one row drawn with a lattice of uniforms meets its expectation to one."""
     g = torch.Generator(device=DEV).manual_seed(1)
