@@ -20,7 +20,8 @@
 // from the list: ranks, both limits, min-p and the draw (129280 logits, top_k 50, top_p 0.9: 16 us instead of 38).
 // What the CTAs tell each other is pushed into everybody's shared memory before a barrier, not fetched after it: a remote load costs
 // about 250 cycles, and there are many.
-// With many rows the passes are bound by instructions (some 30 per logit and weight), not by bytes, so every pass computes no more than it needs.
+// With many rows the passes are bound by instructions, not by bytes (64 rows of 129280 flat logits, top_p 0.9, 67 us: the largest logit 5, weights and
+// histogram 16, list 8, kept weights 13; the histogram's atomics are 1 of it), so every pass computes no more than it needs.
 // The exponent is carried in two fp32 numbers ((l - M) / T rounded to one would be off by 1e-6 relative in a far token's weight).
 #include "internal.h"
 
@@ -106,8 +107,10 @@ struct Sampler {
 #pragma unroll
         for (int e = 0; e < 4; ++e) l[e] = i + e >= 0 && i + e < a.n ? clean(x[i + e]) : -INFINITY;
     }
-    // f(id, logit) for every element of this warp's part.  Lines that reach over the row's ends are read by elements.
-    template <typename F>
+    // f(id, logit) for every element of this warp's part.  Lines that reach over the row's ends are read by elements.  LIGHT: f is a few instructions, so
+    // four lines at a time; else one, with two more on their way (sixteen copies of a long f do not stay in the instruction cache: 64 rows
+    // of 129280 logits, top_p 0.9, 70 us instead of 67; 16 rows 58 instead of 48).
+    template <bool LIGHT = false, typename F>
     DSUF_DEV void each(F f) const {
         const int full0 = lead > 0 ? 1 : 0, full1 = (a.n + lead) >> 2;
         const float4* lines = reinterpret_cast<const float4*>(x - lead);
@@ -119,14 +122,22 @@ struct Sampler {
             f(4 * w - lead + 2, clean(q.z));
             f(4 * w - lead + 3, clean(q.w));
         };
-        for (; v + 96 < end; v += 128) {     // four lines in flight
-            float4 q[4];
+        if (LIGHT) {
+            for (; v + 96 < end; v += 128) {
+                float4 q[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) q[j] = lines[v + 32 * j];
+                for (int j = 0; j < 4; ++j) q[j] = lines[v + 32 * j];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) four(v + 32 * j, q[j]);
+                for (int j = 0; j < 4; ++j) four(v + 32 * j, q[j]);
+            }
         }
-        for (; v < end; v += 32) four(v, lines[v]);
+        float4 q0 = v < end ? lines[v] : float4{}, q1 = v + 32 < end ? lines[v + 32] : float4{};
+        for (; v < end; v += 32) {           // two lines ahead
+            const float4 q = q0;
+            q0 = q1;
+            if (v + 64 < end) q1 = lines[v + 64];
+            four(v, q);
+        }
         if (lane < 2) {                      // lane 0: a cut first line, lane 1: a cut last one
             const int w = lane ? full1 : 0;
             const bool cut = lane ? ((a.n + lead) & 3) != 0 && !(full1 == 0 && full0) : full0 != 0;
@@ -142,7 +153,7 @@ struct Sampler {
     DSUF_DEV float weight(float l) const {
         const float d = fminf(l - top, 0.f);          // (inf - inf is NaN: 0)
         const float v = d - l;
-        const float d_rest = top < INFINITY ? (l - (d - v)) + (-top - v) : 0.f;
+        const float d_rest = top < INFINITY ? (l - (d - v)) - (top + v) : 0.f;
         const float z = d * inv_temp;
         const float z_rest = fmaf(d, inv_temp, -z) + fmaf(d, inv_temp_rest, d_rest * inv_temp);
         float w;
@@ -151,15 +162,12 @@ struct Sampler {
     }
     // w * 2^40, truncated
     DSUF_DEV static u64 fixed(float w) {
-        const uint32_t b = __float_as_uint(w);
-        const int shift = (int)(b >> 23) - (127 + 23 - SA_FRACTION);
-        const uint32_t m = (b & 0x7fffffu) | 0x800000u;
-        return shift >= 0 ? (u64)m << shift : (u64)(m >> min(-shift, 31));
+        return __float2ull_rz(w * (float)(1ull << SA_FRACTION));
     }
     // (rounding to the nearest bin by the addition's own rounding: any map that never goes up with the logit will do)
     DSUF_DEV int bin(float l) const {
-        const float f = fminf((top - l) * inv_bin, (float)(SA_BINS - 1));
-        return l == top ? 0 : (int)(__float_as_uint(f + 8388608.f) & (SA_BINS - 1));
+        const float f = fminf(fmaxf((top - l) * inv_bin, 0.f), (float)(SA_BINS - 1));      // (inf - inf, inf * 0: NaN, so 0)
+        return (int)(__float_as_uint(f + 8388608.f) & (SA_BINS - 1));
     }
     DSUF_DEV u64 block_sum(u64 v) {     // over the CTA, the result in every thread
 #pragma unroll
@@ -371,7 +379,7 @@ struct Sampler {
 #pragma unroll
         for (int e = 0; e < SA_PER; ++e) {
             s.row_w[tid * SA_PER + e] = w[e];
-            if (w[e] && (double)ahead[e] < target && (f[e] >= min_p || l[e] == top))
+            if (w[e] && (double)ahead[e] < target && f[e] >= min_p)
                 s.row_at[atomicAdd(&s.n_list, 1u)] = ((u64)(0xffffffffu - id[e]) << 32) | (uint32_t)(tid * SA_PER + e);
         }
         __syncthreads();
@@ -534,12 +542,12 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleArgs 
     Sampler z{a, s, x, lead, (int)(lines * part / parts), (int)(lines * (part + 1) / parts), tid, warp, lane, rank, ctas, 0.f, 0.f, 0.f, 0.f};
     const float temp = a.temperature ? a.temperature[row] : 1.f;
     const int top_k = a.top_k ? a.top_k[row] : 0;
-    const float top_p = a.top_p ? a.top_p[row] : 1.f, min_p = a.min_p ? fminf(a.min_p[row], 1.f) : 0.f;
+    const float top_p = a.top_p ? a.top_p[row] : 1.f, min_p = a.min_p ? fminf(a.min_p[row], 1.f) : 0.f;      // (the top's weight is 1: it always stays)
     const bool greedy = !(temp > 0.f);
 
     // ---- the largest logit ----
     float hi = -INFINITY;
-    z.each([&](int id, float l) { hi = fmaxf(hi, l); });
+    z.each<true>([&](int id, float l) { hi = fmaxf(hi, l); });
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     if (lane == 0) s.warp_f[warp] = hi;
@@ -600,7 +608,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleArgs 
         if (want_lp)
             z.each([&](int id, float l) { add_lp(l); if (l == hi) at = min(at, id); });
         else
-            z.each([&](int id, float l) { if (l == hi) at = min(at, id); });
+            z.each<true>([&](int id, float l) { if (l == hi) at = min(at, id); });
         at = __reduce_min_sync(0xffffffffu, at);
         if (lane == 0) atomicMin(&s.own_first, at);
         if (want_lp) share_lp();
@@ -675,14 +683,14 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleArgs 
         z.each([&](int id, float l) {
             if (lim.holds(l, id)) {
                 const float w = z.weight(l);
-                if (w >= min_p || l == hi) sum += z.fixed(w);
+                if (w >= min_p) sum += z.fixed(w);
             }
         });
     } else {
         z.each([&](int id, float l) {
             if (want_lp) add_lp(l);
             const float w = z.weight(l);
-            sum += w >= min_p || l == hi ? z.fixed(w) : 0;
+            sum += w >= min_p ? z.fixed(w) : 0;
         });
         if (want_lp) share_lp();
     }
@@ -712,7 +720,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleArgs 
     auto mass = [&](int id, float l) {
         if (!lim.holds(l, id)) return (u64)0;
         const float w = z.weight(l);
-        return w >= min_p || l == hi ? z.fixed(w) : 0;
+        return w >= min_p ? z.fixed(w) : 0;
     };
     int holder = 0;
     while (before + s.warp_a[holder] <= draw) before += s.warp_a[holder++];
