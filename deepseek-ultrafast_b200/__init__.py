@@ -3,7 +3,8 @@
 The reference's host side is Rust (crates/engine/src/ops.rs); no Rust toolchain exists in this build
 environment, so the same operator surface is mirrored here in Python over ctypes.  Names follow the reference:
 ``gemv`` (ops.rs:331), ``moe_route_tokens`` / ``moe_perm`` / ``moe_gather_quant`` (cu/ops.cu:615, cu/tcmoe.cu:19,88),
-``moe_gemv`` (ops.rs:482), ``ffn`` (crates/engine/src/model.rs:3497).  PyTorch is used only to own device memory
+``moe_gemv`` (ops.rs:482), ``ffn`` (crates/engine/src/model.rs:3497).  The per-layer calls of a decode step (``kv_append``,
+``attn_decode``, ``attn_prompt``, ``sample``) check their tensors and call the library in C++ (csrc/hostcall.cc).  PyTorch is used only to own device memory
 and streams; every computation happens in the library's CUDA kernels.  There is no fallback: if the shared
 library is missing or the device is not sm_100, construction fails.
 """
