@@ -616,6 +616,14 @@ static int encode_heads(dsuf_ctx* ctx, CUtensorMap* tm, const void* base, long l
     return DSUF_OK;
 }
 
+// Whether t rows of `wo` bf16 columns at `out` share memory with t rows of `w` columns at `x`.  Parts of the columns of the same rows do not.
+static bool rows_overlap(uint64_t out, long long ldo, long long wo, uint64_t x, long long ld, long long w, long long t) {
+    if (out >= x + 2 * ((t - 1) * ld + w) || x >= out + 2 * ((t - 1) * ldo + wo)) return false;
+    if (ldo != ld) return true;
+    const long long apart = (((long long)(out - x) / 2) % ld + ld) % ld;
+    return apart < w || apart + wo > ld;
+}
+
 int attn_prompt_setup(dsuf_ctx* ctx) {
     cudaError_t e = cudaFuncSetAttribute(attn_prompt_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<64>::SMEM);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(attn_prompt_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<128>::SMEM);
@@ -640,12 +648,15 @@ extern "C" int32_t dsuf_attn_prompt(dsuf_ctx* ctx, void* stream, uint64_t q, int
     if (t == 0 || n_seqs == 0) return DSUF_OK;
     DSUF_REQUIRE(ctx, q && k && v && out && cu_seqlens && (q & 15) == 0 && (k & 15) == 0 && (v & 15) == 0 && (out & 15) == 0 && (cu_seqlens & 3) == 0 &&
                  (lse & 3) == 0, "attn_prompt: null or misaligned pointer (q, k, v, out 16 bytes, cu_seqlens and lse 4)");
+    const long long wq = (long long)q_heads * head_dim, wk = (long long)kv_heads * head_dim;
+    DSUF_REQUIRE(ctx, !rows_overlap(out, ldo, wq, q, ldq, wq, t) && !rows_overlap(out, ldo, wq, k, ldk, wk, t) && !rows_overlap(out, ldo, wq, v, ldv, wk, t),
+                 "attn_prompt: out must not share memory with q, k or v");
     DSUF_REQUIRE_DEVICE(ctx, "attn_prompt");
     PromptArgs a;
     memset(&a, 0, sizeof(a));
-    int rc = encode_heads(ctx, &a.tm_q, (const void*)q, (long long)q_heads * head_dim, ldq, t);
-    if (!rc) rc = encode_heads(ctx, &a.tm_k, (const void*)k, (long long)kv_heads * head_dim, ldk, t);
-    if (!rc) rc = encode_heads(ctx, &a.tm_v, (const void*)v, (long long)kv_heads * head_dim, ldv, t);
+    int rc = encode_heads(ctx, &a.tm_q, (const void*)q, wq, ldq, t);
+    if (!rc) rc = encode_heads(ctx, &a.tm_k, (const void*)k, wk, ldk, t);
+    if (!rc) rc = encode_heads(ctx, &a.tm_v, (const void*)v, wk, ldv, t);
     if (rc) return rc;
     a.out = (bf16*)out; a.lse = (float*)lse; a.ldo = ldo; a.t = t;
     a.q_heads = q_heads; a.kv_heads = kv_heads; a.group = q_heads / kv_heads; a.n_seqs = n_seqs; a.window = window;

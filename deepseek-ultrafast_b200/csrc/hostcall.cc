@@ -98,6 +98,14 @@ long whole(const Call& c, PyObject* o, const char* what) {
     if (v < -0x7fffffffl || v > 0x7fffffffl) refuse(c.name(what) + ": out of range");
     return v;
 }
+bool yes(const Call& c, PyObject* o, const char* what) {
+    const int v = PyObject_IsTrue(o);
+    if (v < 0) {
+        PyErr_Clear();
+        refuse(c.name(what) + ": true or false is wanted");
+    }
+    return v == 1;
+}
 float real(const Call& c, PyObject* o, const char* what) {
     const double v = PyFloat_AsDouble(o);
     if (v == -1.0 && PyErr_Occurred()) {
@@ -125,7 +133,7 @@ PyObject* kv_append(PyObject* const* a) {
         const at::Tensor& cos = c.dense(PyTuple_GET_ITEM(a[8], 0), "cos", at::kFloat, -1, -1);
         const at::Tensor& sin = c.dense(PyTuple_GET_ITEM(a[8], 1), "sin", at::kFloat, cos.size(0), cos.size(1));
         if (cos.size(1) > 4096) refuse("kv_append: cos and sin are wider than any head");
-        r = {at_(cos), at_(sin), (int32_t)cos.size(0), (int32_t)cos.size(1) * 2, (int32_t)whole(c, PyTuple_GET_ITEM(a[8], 2), "off"), PyObject_IsTrue(a[9]) == 1};
+        r = {at_(cos), at_(sin), (int32_t)cos.size(0), (int32_t)cos.size(1) * 2, (int32_t)whole(c, PyTuple_GET_ITEM(a[8], 2), "off"), yes(c, a[9], "rope_half")};
     }
     uint64_t qp = 0, qo = 0, ko = 0;
     at::Tensor q_out;
@@ -183,7 +191,7 @@ PyObject* attn_decode(PyObject* const* a) {
     const at::Tensor& lens = c.vector(a[5], "seq_lens", at::kInt, b);
     const float scale = given(a[6]) ? real(c, a[6], "scale") : (float)(1.0 / std::sqrt((double)d));
     const long window = whole(c, a[7], "window");
-    const bool want = PyObject_IsTrue(a[10]) == 1;
+    const bool want = yes(c, a[10], "return_lse");
     const at::Tensor& space = c.vector(a[11], "workspace", at::kByte, (int64_t)c_workspace_bytes(c.ctx));
     Results r(c, a[8], a[9], want, b, width, heads);
     c.run([&](void* s) {
@@ -209,7 +217,7 @@ PyObject* attn_prompt(PyObject* const* a) {
     if (cu.size(0) < 1) refuse("attn_prompt: cu_seqlens holds at least one entry");
     const float scale = given(a[7]) ? real(c, a[7], "scale") : (float)(1.0 / std::sqrt((double)d));
     const long window = whole(c, a[8], "window");
-    const bool want = PyObject_IsTrue(a[11]) == 1;
+    const bool want = yes(c, a[11], "return_lse");
     Results r(c, a[9], a[10], want, n, width, heads);
     c.run([&](void* s) {
         return c_attn_prompt(c.ctx, s, at_(q), ldq, at_(k), ldk, at_(v), ldv, (int)n, (int)heads, (int)kv_heads, (int)d, at_(cu), (int)cu.size(0) - 1, scale,
@@ -229,7 +237,7 @@ PyObject* sample(PyObject* const* a) {
     auto column = [&](int i, const char* what, at::ScalarType type) { return given(a[i]) ? at_(c.vector(a[i], what, type, m)) : 0; };
     const uint64_t temperature = column(4, "temperature", at::kFloat), top_k = column(5, "top_k", at::kInt), top_p = column(6, "top_p", at::kFloat),
                    min_p = column(7, "min_p", at::kFloat);
-    const bool want = PyObject_IsTrue(a[10]) == 1;
+    const bool want = yes(c, a[10], "return_logprobs");
     at::Tensor ids = given(a[8]) ? c.vector(a[8], "ids", at::kInt, m) : c.make({m}, at::kInt), lp;
     if (given(a[9])) lp = c.vector(a[9], "logprobs", at::kFloat, m);
     else if (want) lp = c.make({m}, at::kFloat);

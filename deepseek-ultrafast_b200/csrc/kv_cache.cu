@@ -197,7 +197,7 @@ extern "C" int32_t dsuf_kv_append(dsuf_ctx* ctx, void* stream, const dsuf_kv_cac
                  "kv_append: ldq and ldqo must be multiples of 8 and hold q_heads * head_dim elements");
     DSUF_REQUIRE(ctx, !k_out || (ldko >= cache->kv_heads * D && ldko % 8 == 0 && (k_out & 15) == 0),
                  "kv_append: k_out must be 16-byte aligned, ldko a multiple of 8 that holds kv_heads * head_dim elements");
-    DSUF_REQUIRE(ctx, !rope || (rope->rot >= 16 && rope->rot % 16 == 0 && rope->off >= 0 && rope->off % 8 == 0 && rope->off + rope->rot <= D),
+    DSUF_REQUIRE(ctx, !rope || (rope->rot >= 16 && rope->rot % 16 == 0 && rope->off >= 0 && rope->off % 8 == 0 && rope->off <= D - rope->rot),
                  "kv_append: rope needs rot a multiple of 16, off a multiple of 8, off + rot <= head_dim");
     DSUF_REQUIRE(ctx, !rope || (rope->cos && rope->sin && (rope->cos & 15) == 0 && (rope->sin & 15) == 0 && rope->positions >= 1),
                  "kv_append: rope tables must be 16-byte aligned and hold at least one position");

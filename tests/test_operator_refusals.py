@@ -93,6 +93,36 @@ def test_prompt_refuses(pkg, cctx):
     assert prompt(pkg, None) == BAD
 
 
+def test_prompt_refuses_an_output_in_its_inputs(pkg, cctx):
+    row = 512 + 256 + 256 + 512      # q, k, v and the output as columns of one row
+    base = dict(ldq=row, ldk=row, ldv=row, ldo=row, q=P, k=P + 1024, v=P + 1536, out=P + 2048)
+    text = C.create_string_buffer(512)
+
+    def refused(**kw):
+        assert prompt(pkg, cctx, **{**base, **kw}) != 0      # (without a GPU the device is what the good ones are refused for)
+        pkg.lib().dsuf_last_error(cctx, text, 512)
+        return b"share memory" in text.value
+    for kw in [dict(out=P), dict(out=P + 1024), dict(out=P + 1536), dict(out=P + 1024 + 496), dict(out=P + 2 * row), dict(out=P, ldo=512), dict(out=P + 16 * row, ldo=520),
+               dict(out=P - 16), dict(ldq=512, ldo=512, out=P + 1024 * 8)]:
+        assert refused(**kw), kw
+    for kw in [{}, dict(out=P + 2048 + 2 * row), dict(out=P + 2 * 9 * row), dict(out=P - 2 * 9 * row), dict(out=P - 1024, ldo=row), dict(ldq=512, out=P + (1 << 16), ldo=512)]:
+        assert not refused(**kw), kw
+
+
+def test_flags_and_offsets_are_refused(pkg, cctx):
+    assert append(pkg, cache(pkg), cctx, rope=rope(pkg, rot=16, off=0x7ffffff8)) == BAD      # (their sum passes 32 bits)
+
+    class Neither:
+        def __bool__(self):
+            raise ValueError("neither")
+    ctx = types.SimpleNamespace(torch=torch, device=torch.device("cpu"), index=-1, address=C.addressof(cctx))
+    z = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt)   # noqa: E731
+    with pytest.raises(pkg.DsufError, match="return_lse"):
+        pkg.attn_prompt(ctx, z(3, 512), z(3, 256), z(3, 256), z(2, dt=torch.int32), return_lse=Neither())
+    with pytest.raises(pkg.DsufError, match="return_logprobs"):
+        pkg.sample(ctx, z(3, 9, dt=torch.float32), z(3, dt=torch.float32), return_logprobs=Neither())
+
+
 def test_sample_refuses(pkg, cctx):
     def call(ctx=cctx, logits=P, ld=100, m=2, n=100, t=0, k=0, p=0, q=0, u=P, ids=P, lp=0):
         return pkg.lib().dsuf_sample(ctx, None, logits, ld, m, n, t, k, p, q, u, ids, lp)
