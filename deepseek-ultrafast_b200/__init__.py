@@ -340,6 +340,8 @@ class Ctx:
         nbytes = lib().dsuf_attn_workspace_bytes(self.h)
         w = t.empty(nbytes, dtype=t.uint8, device=self.device)
         self.check(lib().dsuf_attn_workspace_init(self.h, self.stream(), w.data_ptr(), nbytes))
+        if not t.cuda.is_current_stream_capturing():
+            t.cuda.current_stream(self.index).synchronize()     # (its first user may be another stream)
         return w
 
     def set_decode_path(self, tcgen05):

@@ -367,6 +367,43 @@ def test_many_short_sequences(pkg, actx, fp8, d, hq, hkv, window, most):
 
 
 @gpu
+@pytest.mark.parametrize("lens", [[3000, 5], [40] * 400])
+def test_decode_in_place_and_over_shared_pages(pkg, actx, lens):
+    """out = q, by ranges and by warps, and sequences that all read the first one's pages."""
+    cache, q, table, n = decode_inputs(pkg, actx, 51, lens, 16, 2, 128, 16, False)
+    want, lse = pkg.attn_decode(actx, cache, q, table, n, return_lse=True)
+    mine = q.clone()
+    assert pkg.attn_decode(actx, cache, mine, table, n, out=mine) is mine
+    assert torch.equal(mine, want)
+    first = table[:1].repeat(len(lens), 1)
+    n.fill_(lens[0])
+    got = pkg.attn_decode(actx, cache, q[:1].repeat(len(lens), 1), first, n)
+    torch.cuda.synchronize()
+    assert actx.status().code == 0
+    want, _, size = decode64(cache, q[:1].repeat(len(lens), 1), first, [lens[0]] * len(lens), 0, 128 ** -0.5)
+    within(got, want, size, terms=2 ** -8 + 2 ** -12)
+
+
+@gpu
+def test_a_new_workspace_is_ready_for_another_stream(pkg, actx):
+    cache, q, table, n = decode_inputs(pkg, actx, 53, [5000], 8, 1, 128, 16, False)
+    want = pkg.attn_decode(actx, cache, q, table, n)
+    junk = torch.full((64 << 20,), 255, dtype=torch.uint8, device=DEV)
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for _ in range(20):
+            junk.add_(0)                 # keeps the creating stream busy
+        w = torch.full_like(actx.attn_workspace, 255)
+        del w                            # (its memory is what the new one gets)
+        w = actx.new_attn_workspace()
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            got = pkg.attn_decode(actx, cache, q, table, n, workspace=w)
+        side.synchronize()
+        assert torch.equal(got, want)
+
+
+@gpu
 def test_every_bad_length_is_reported(pkg, actx):
     """One length beyond its table among many short contexts, wherever it stands, is cut to the table and reported."""
     lens = [5] * 600
