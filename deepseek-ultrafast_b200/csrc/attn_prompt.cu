@@ -32,8 +32,9 @@ namespace dsuf {
 constexpr int KID_PROMPT = 9;
 constexpr int PA_THREADS = 352;
 constexpr int PA_BM = 128;
-constexpr float PA_UNSET = -1e30f;
+constexpr float PA_UNSET = -3e38f;     // below every finite score
 constexpr float PA_TRIGGER = 16777216.f;
+constexpr float PA_FAR = 268435456.f;   // beyond this a reference's own rounding is an exponent of more than 8
 
 template <int D>
 struct PromptShape {
@@ -203,9 +204,10 @@ DSUF_DEV float pa_total(unsigned long long two) {
     asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(two));
     return x + y;
 }
+DSUF_DEV bool pa_far(float ref) { return fabsf(ref) > PA_FAR && ref > PA_UNSET; }
 DSUF_DEV bool pa_seen(int col, int upper, int lower) { return col <= upper && col > lower; }
 // p = 2^(s sl2 - ref) of a row, packed to bf16 in w, and their sum.  MASK 0: all columns are visible, 1: those up to `upper`, 2: those above
-// `lower` as well.
+// `lower` as well, 3: the same, and the product s sl2 is rounded as a far reference was.
 template <int MASK>
 DSUF_DEV float pa_weights(uint32_t tS, float sl2, float ref, int upper, int lower, uint32_t* w) {
     const unsigned long long scale2 = pack_f32x2(sl2, sl2), ref2 = pack_f32x2(-ref, -ref);
@@ -217,6 +219,10 @@ DSUF_DEV float pa_weights(uint32_t tS, float sl2, float ref, int upper, int lowe
             asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(pack_f32x2(s[e], s[e + 1])), "l"(scale2), "l"(ref2));
             float x, y;
             asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+            if (MASK == 3 && pa_far(ref)) {
+                x = __fsub_rn(__fmul_rn(s[e], sl2), ref);
+                y = __fsub_rn(__fmul_rn(s[e + 1], sl2), ref);
+            }
             if constexpr (MASK > 0) {
                 const int col = c * 32 + e;
                 x = pa_seen(col, upper, MASK > 1 ? lower : -1) ? x : -INFINITY;
@@ -523,8 +529,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
                 if (windowed) part = pa_weights<2>(tS, sl2, ref, upper, lower, w);
                 else if (diagonal) part = pa_weights<1>(tS, sl2, ref, upper, lower, w);
                 else part = pa_weights<0>(tS, sl2, ref, upper, lower, w);
-                if (!__all_sync(0xffffffffu, part <= PA_TRIGGER)) {
-                    // (seldom, or NaN) the reference moves up to the tile's largest score where that is larger; so do the sum and the output, which is
+                const bool fine = part <= PA_TRIGGER && !pa_far(ref);
+                if (!__all_sync(0xffffffffu, fine)) {
+                    // (seldom, or NaN, or scores of 2^28 and more) the reference moves up to the tile's largest score where that is larger; so do the sum and the output, which is
                     // complete: this step's scores were issued behind the last step's product
                     float top = PA_UNSET;
 #pragma unroll 1
@@ -532,9 +539,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
                         float s[16];
                         tmem_ld<16>(tS + c, s);
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) top = fmaxf(top, pa_seen(c + e, upper, lower) ? s[e] * sl2 : -INFINITY);
+                        for (int e = 0; e < 16; ++e) top = fmaxf(top, pa_seen(c + e, upper, lower) ? __fmul_rn(s[e], sl2) : -INFINITY);
                     }
-                    const float to = part <= PA_TRIGGER ? ref : fmaxf(ref, top);      // (a row's result does not depend on its neighbours)
+                    const float to = fine ? ref : fmaxf(ref, top);      // (a row's result does not depend on its neighbours)
                     const float by = pa_exp2(ref - to);
                     if (j > q.lo) {
 #pragma unroll 1
@@ -548,7 +555,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
                     }
                     ref = to;
                     sum *= by;
-                    part = pa_weights<2>(tS, sl2, ref, upper, lower, w);
+                    part = pa_weights<3>(tS, sl2, ref, upper, lower, w);
                 }
                 sum += part;
 #pragma unroll

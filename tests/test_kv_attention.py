@@ -463,6 +463,31 @@ def test_large_scores_move_the_reference(pkg, actx):
 
 
 @gpu
+@pytest.mark.parametrize("score", [-8e31, 8e31, -1e37, 1e37])
+def test_scores_near_the_ends_of_fp32(pkg, actx, score):
+    """All scores equal and huge: the plain mean of the visible values, with and without a window."""
+    g = gen(61)
+    d, n = 64, 300
+    q = torch.ones(n, 2 * d, dtype=torch.bfloat16, device=DEV)
+    k = torch.full((n, d), score / 8, dtype=torch.float32, device=DEV).bfloat16()      # (times 64 columns times the scale 1/8: the score)
+    v = bf16(g, n, d)
+    cu = torch.tensor([0, n], dtype=torch.int32, device=DEV)
+    for window in (0, 50):
+        out = pkg.attn_prompt(actx, q, k, v, cu, head_dim=d, window=window).double().reshape(n, 2, d)
+        for r in (0, 1, 49, 128, 299):
+            seen = v.double()[max(0, r + 1 - window) if window else 0: r + 1]
+            within(out[r], seen.mean(0).expand(2, d), seen.abs().mean(0).expand(2, d), terms=2 ** -8 + 2 ** -12)
+    cache = pkg.KvCache.empty(actx, 20, 16, 1, d)
+    pos = torch.arange(n, dtype=torch.int32, device=DEV)
+    table = torch.arange(19, dtype=torch.int32, device=DEV)[None]
+    pkg.kv_append(actx, cache, k, v, pos, table, seq=torch.zeros_like(pos))
+    for window in (0, 50):
+        seen = v.double()[n - window if window else 0:]
+        out = pkg.attn_decode(actx, cache, q[:1], table, pos[-1:] + 1, window=window).double().reshape(2, d)
+        within(out, seen.mean(0).expand(2, d), seen.abs().mean(0).expand(2, d), terms=2 ** -8 + 2 ** -12)
+
+
+@gpu
 def test_nan_stays_with_the_rows_that_see_it(pkg, actx):
     g = gen(22)
     d, lens = 64, [200, 60]
