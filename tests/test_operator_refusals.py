@@ -97,9 +97,10 @@ def test_prompt_refuses_an_output_in_its_inputs(pkg, cctx):
     row = 512 + 256 + 256 + 512      # q, k, v and the output as columns of one row
     base = dict(ldq=row, ldk=row, ldv=row, ldo=row, q=P, k=P + 1024, v=P + 1536, out=P + 2048)
     text = C.create_string_buffer(512)
+    C.c_int.from_buffer(cctx).value = 1 << 20      # (the context's device, never the current one: the good calls go no further than that check)
 
     def refused(**kw):
-        assert prompt(pkg, cctx, **{**base, **kw}) != 0      # (without a GPU the device is what the good ones are refused for)
+        assert prompt(pkg, cctx, **{**base, **kw}) != 0
         pkg.lib().dsuf_last_error(cctx, text, 512)
         return b"share memory" in text.value
     for kw in [dict(out=P), dict(out=P + 1024), dict(out=P + 1536), dict(out=P + 1024 + 496), dict(out=P + 2 * row), dict(out=P, ldo=512), dict(out=P + 16 * row, ldo=520),
