@@ -173,9 +173,11 @@ DSUF_DEV uint32_t cluster_num_ctas() {
 }
 // Hardware barrier over every thread of every CTA of the cluster; shared-memory writes made before it are visible to
 // the other CTAs' distributed-shared-memory reads after it.  Whole warps must call it together.
+DSUF_DEV void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" : : : "memory"); }
+DSUF_DEV void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" : : : "memory"); }
 DSUF_DEV void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" : : : "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" : : : "memory");
+    cluster_arrive();
+    cluster_wait();
 }
 // One fp32 from the same shared-memory location of CTA `rank` of this cluster.
 DSUF_DEV float ld_cluster_f32(const float* my_smem_ptr, uint32_t rank) {

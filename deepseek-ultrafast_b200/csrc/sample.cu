@@ -169,18 +169,6 @@ struct Sampler {
         const float f = fminf(fmaxf((top - l) * inv_bin, 0.f), (float)(SA_BINS - 1));      // (inf - inf, inf * 0: NaN, so 0)
         return (int)(__float_as_uint(f + 8388608.f) & (SA_BINS - 1));
     }
-    DSUF_DEV u64 block_sum(u64 v) {     // over the CTA, the result in every thread
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        __syncthreads();
-        if (lane == 0) s.warp_a[warp] = v;
-        __syncthreads();
-        u64 r = 0;
-#pragma unroll
-        for (int w = 0; w < SA_WARPS; ++w) r += s.warp_a[w];
-        return r;
-    }
-
     DSUF_DEV void clear_bins() {
         for (int i = tid; i < SA_BINS; i += SA_THREADS) s.lo[i] = s.hi[i] = 0;
         __syncthreads();
@@ -210,23 +198,22 @@ struct Sampler {
         }
         cluster_barrier();
     }
-    DSUF_DEV u64 bins_sum() {
-        u64 v = 0;
-        for (int i = tid; i < SA_BINS; i += SA_THREADS) v += s.all[i];
-        return block_sum(v);
-    }
     // Whether an amount that goes from `from` to `to` is where the limit falls: the first to reach `want` tokens, or the weight `target`.
     DSUF_DEV static bool reaches(bool by_mass, u64 want, double target, u64 from, u64 to) {
         return by_mass ? (double)from < target && target <= (double)to : from < want && want <= to;
     }
-    // The bin where the limit falls, counting from `start`, and the amount before it.
-    DSUF_DEV int find_bin(bool by_mass, u64 want, double target, u64& start) {
-        constexpr int PER = SA_BINS / SA_THREADS;
-        u64 c[PER], cs = 0;
+    // Running sums over the row's bins: this thread's, the amount before them, and that of all.
+    static constexpr int BINS_PER = SA_BINS / SA_THREADS;
+    struct Scan {
+        u64 c[BINS_PER], before, all;
+    };
+    DSUF_DEV Scan scan_bins() {
+        Scan r;
+        u64 cs = 0;
 #pragma unroll
-        for (int e = 0; e < PER; ++e) {
-            c[e] = s.all[tid * PER + e];
-            cs += c[e];
+        for (int e = 0; e < BINS_PER; ++e) {
+            r.c[e] = s.all[tid * BINS_PER + e];
+            cs += r.c[e];
         }
         u64 ci = cs;
 #pragma unroll
@@ -237,15 +224,26 @@ struct Sampler {
         __syncthreads();
         if (lane == 31) s.warp_a[warp] = ci;
         __syncthreads();
-        u64 cb = start + ci - cs;
-        for (int w = 0; w < warp; ++w) cb += s.warp_a[w];
+        r.before = ci - cs;
+        r.all = 0;
 #pragma unroll
-        for (int e = 0; e < PER; ++e) {
-            if (reaches(by_mass, want, target, cb, cb + c[e])) {
-                s.found_bin = tid * PER + e;
+        for (int w = 0; w < SA_WARPS; ++w) {
+            const u64 v = s.warp_a[w];
+            if (w < warp) r.before += v;
+            r.all += v;
+        }
+        return r;
+    }
+    // The bin where the limit falls, counting from `start`, and the amount before it.
+    DSUF_DEV int find_bin(const Scan& r, bool by_mass, u64 want, double target, u64& start) {
+        u64 cb = start + r.before;
+#pragma unroll
+        for (int e = 0; e < BINS_PER; ++e) {
+            if (reaches(by_mass, want, target, cb, cb + r.c[e])) {
+                s.found_bin = tid * BINS_PER + e;
                 s.found_before = cb;
             }
-            cb += c[e];
+            cb += r.c[e];
         }
         __syncthreads();
         const int b = s.found_bin;
@@ -472,7 +470,7 @@ struct Sampler {
                 if (mine(id, l)) add((k_hi - key(l)) >> shift, by_mass ? fixed(weight(l)) : 1);
             });
             share_bins(by_mass);
-            const uint32_t b = (uint32_t)find_bin(by_mass, want, target, before);
+            const uint32_t b = (uint32_t)find_bin(scan_bins(), by_mass, want, target, before);
             k_hi -= b << shift;
             k_lo = max(k_lo, k_hi - min(k_hi, (1u << shift) - 1u));
         }
@@ -635,15 +633,17 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleArgs 
         if (want_lp) share_lp();
         want_lp = false;
         z.share_bins(false);
-        cut = (u64)top_k < z.bins_sum();
+        const Sampler::Scan bins = z.scan_bins();
+        cut = (u64)top_k < bins.all;
         if (cut) {
             u64 before = 0;
-            const int b = z.find_bin(false, (u64)top_k, 0.0, before);
+            const int b = z.find_bin(bins, false, (u64)top_k, 0.0, before);
             if (before + s.all[b] <= SA_LIST) {
                 const uint32_t total = z.list([&](int id, float l) { return l > -INFINITY && z.bin(l) <= b; });
                 if (rank == 0) z.fetch_list();
-                cluster_barrier();
+                cluster_arrive();        // (the other CTAs stay until their lists have been read)
                 if (rank == 0) z.finish(total, (u64)top_k, top_p, 0, min_p, u, store);
+                cluster_wait();
                 return;
             }
             lim = z.limit(false, (u64)top_k, 0.0, lim, b, before);
@@ -659,10 +659,11 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleArgs 
         want_lp = false;
         z.share_bins(true);
         // the first token is always inside: a target below one unit of weight is reached by it
-        const u64 mass = z.bins_sum();
+        const Sampler::Scan bins = z.scan_bins();
+        const u64 mass = bins.all;
         const double target = fmax((double)top_p * (double)mass, 0.5);
         u64 before = 0;
-        const int b = z.find_bin(true, 0, target, before);
+        const int b = z.find_bin(bins, true, 0, target, before);
         // Every token down to bin b weighs at least what the bin's edge does, which bounds their number; of flat rows the bound is near the
         // truth and far above the list's size: they do not try.
         const float edge = z.weight(hi - (float)(b + 1) / z.inv_bin);
@@ -670,8 +671,9 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleArgs 
             const uint32_t total = z.list([&](int id, float l) { return l > -INFINITY && z.bin(l) <= b; });
             if (total <= SA_LIST) {
                 if (rank == 0) z.fetch_list();
-                cluster_barrier();
+                cluster_arrive();
                 if (rank == 0) z.finish(total, ~0ull, top_p, mass, min_p, u, store);
+                cluster_wait();
                 return;
             }
             cluster_barrier();    // (everybody has read the lists' lengths: the next ones may be written)
@@ -788,8 +790,12 @@ extern "C" int32_t dsuf_sample(dsuf_ctx* ctx, void* stream, uint64_t logits, int
     a.logits = (const float*)logits; a.ld = ld; a.n = n;
     a.temperature = (const float*)temperature; a.top_p = (const float*)top_p; a.min_p = (const float*)min_p; a.u = (const float*)u;
     a.top_k = (const int*)top_k; a.ids = (int*)ids_out; a.logprobs = (float*)logprobs_out;
-    // as many CTAs per row as the GPU holds at once (two per SM), each with at least 2048 logits: fewer are not worth the cluster's barriers
+    // As many CTAs per row as the GPU holds at once (two per SM), each with at least 2048 logits: fewer are not worth the cluster's barriers.
+    // Clusters of 16 only while four fifths of the SMs hold them all: a cluster lies inside one GPC, which has room for one of 16 and some rest, so
+    // with more of them CTAs share SMs (129280 logits, top_k 50, top_p 0.9; 16 against 8: 1 row 15.3 / 17.1 us, 7 rows 15.6 / 17.3, 8 rows
+    // 19.4 / 17.5, 16 rows 29.2 / 22.6; rows of mixed settings lose up to 5 % at 8 to 11 rows of that width and win as much or more elsewhere).
     int c = SA_MAX_CLUSTER;
-    while (c > 1 && ((long long)m * c > 2ll * ctx->sm_count || n < 2048 * c)) c >>= 1;
+    auto fits = [&](int cl) { return 5ll * m * cl <= (cl == SA_MAX_CLUSTER ? 4ll : 10ll) * ctx->sm_count; };
+    while (c > 1 && (!fits(c) || n < 2048 * c)) c >>= 1;
     return launch_cluster(ctx, (cudaStream_t)stream, sample_kernel, dim3(m * c), dim3(SA_THREADS), sizeof(SampleShared), c, a);
 }
