@@ -70,6 +70,7 @@ struct SampleShared {
     uint32_t n_list;
     uint32_t lists[SA_MAX_CLUSTER];
     float top[SA_MAX_CLUSTER], lp[SA_MAX_CLUSTER];
+    uint32_t tops[SA_MAX_CLUSTER], warp_tops[SA_WARPS];
     int first[SA_MAX_CLUSTER];
     u64 kept[SA_MAX_CLUSTER];
     uint32_t key_hi[SA_MAX_CLUSTER], key_lo[SA_MAX_CLUSTER], ties[SA_MAX_CLUSTER];
@@ -574,31 +575,47 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleArgs 
 
     // ---- the limits; the first pass over all tokens also sums for the log-probability (temperature 1) ----
     bool want_lp = a.logprobs != nullptr;
+    // (the largest logits are counted and the others summed: the logarithm of a sum next to 1 would lose what the others add to it)
     float lp = 0.f;
+    uint32_t tops = 0;
     auto add_lp = [&](float l) {
         float e;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fminf(l - hi, 0.f) * 1.4426950408889634f));
-        lp += e;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"((l - hi) * 1.4426950408889634f));
+        if (l == hi) ++tops;
+        else lp += e;
     };
     // this CTA's sum into everybody's table; visible behind the next cluster barrier
     auto share_lp = [&]() {
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) lp += __shfl_xor_sync(0xffffffffu, lp, o);
+        tops = __reduce_add_sync(0xffffffffu, tops);
         __syncthreads();
-        if (lane == 0) s.warp_f[warp] = lp;
+        if (lane == 0) {
+            s.warp_f[warp] = lp;
+            s.warp_tops[warp] = tops;
+        }
         __syncthreads();
         if (tid < ctas) {
             float t = 0.f;
-            for (int w = 0; w < SA_WARPS; ++w) t += s.warp_f[w];
+            uint32_t n = 0;
+            for (int w = 0; w < SA_WARPS; ++w) {
+                t += s.warp_f[w];
+                n += s.warp_tops[w];
+            }
             *in_cta(&s.lp[rank], tid) = t;
+            *in_cta(&s.tops[rank], tid) = n;
         }
     };
     auto store = [&](int token, float l) {
         a.ids[row] = token;
         if (a.logprobs) {
             float t = 0.f;
-            for (uint32_t r = 0; r < ctas; ++r) t += s.lp[r];
-            a.logprobs[row] = fminf(l - hi, 0.f) - logf(t);
+            uint32_t n = 0;
+            for (uint32_t r = 0; r < ctas; ++r) {
+                t += s.lp[r];
+                n += s.tops[r];
+            }
+            a.logprobs[row] = fminf(l - hi, 0.f) - log1pf((float)(n - 1) + t);
         }
     };
     if (greedy) {

@@ -157,6 +157,24 @@ def test_infinite_and_missing_logits(pkg, sctx):
 
 
 @gpu
+@pytest.mark.parametrize("gap,tied", [(2.0, 1), (9.0, 1), (14.0, 1), (9.0, 3)])
+@pytest.mark.parametrize("kw", [{}, dict(top_k=5), dict(top_p=0.5), dict(temperature=0.0)])
+def test_log_probability_of_a_near_certain_token(pkg, sctx, gap, tied, kw):
+    """log(1 / (1 + s)) keeps s's precision however small s is."""
+    x, u, _ = inputs(12, 3, 5000)
+    x = x.clone()
+    x[:, 100:100 + tied] = x.amax(1, keepdim=True) + gap
+    full = lambda v: torch.full((3,), v, dtype=torch.int32 if isinstance(v, int) else torch.float32, device=DEV)
+    ids, lp = pkg.sample(sctx, x, u * 0.1, return_logprobs=True, **{k: full(v) for k, v in kw.items()})
+    assert ids.tolist() == [100] * 3
+    others = torch.cat([x[:, :100], x[:, 101:]], 1).double() - x[:, 100:101].double()
+    want = -torch.log1p(others.exp().sum(1))
+    # l - top (below 32) and its product with log2(e) are rounded once each, the exponential is good to 2^-22, and a sum of at most 5 terms per thread,
+    # 5 shuffles, 16 warps and 2 CTAs rounds 28 times: 2^-20 + 2^-19 ln 2 + 2^-22 + 28 2^-24, and log1p
+    assert ((lp.double() - want).abs() <= 2 ** -18 * want.abs()).all()
+
+
+@gpu
 @pytest.mark.parametrize("temp", [1.4e-45, 1e-40, 4e-39, 1.2e-38, 1e-30])
 @pytest.mark.parametrize("kw", [{}, dict(top_k=3), dict(top_k=2000), dict(top_p=0.7), dict(min_p=0.5)])
 def test_temperatures_next_to_nothing(pkg, sctx, temp, kw):
