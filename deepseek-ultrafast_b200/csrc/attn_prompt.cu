@@ -16,7 +16,8 @@
 // issued before the last output is stored.  The two issuing warps take strict turns (P0 V, S0, P1 V, S1): issuing blocks while the tensor
 // core's short queue is full, so the barrier waits of one tile (100 cycles and more each, even when met) have to pass while the
 // other's products are issued; without turns the tiles fall into step, and both softmaxes share the exponential unit and then both wait.
-// (8192 tokens, 56 / 8 heads of 128: one issuing warp 867 us, two without turns 1022, two with turns 778.)
+// (8192 tokens, 56 / 8 heads of 128: one issuing warp 867 us, two without turns 1022, two with turns 778; now 765 = 1255 TFLOP/s
+// of visible pairs, with the tensor pipe and the exponential unit each 54 % busy.)
 // Tensor memory (512 columns): S0 S1 (128 fp32 columns each; P_t overwrites the first 64 of S_t as packed bf16), O0 O1 (D each).
 // The reference point of a row is the largest of its first 32 scores and only moves when a tile's weights add up to more than 2^24 (exact: the
 // sum and the output share the reference, and bf16's and fp32's precision does not depend on the magnitude), so usual tiles need no maximum at
