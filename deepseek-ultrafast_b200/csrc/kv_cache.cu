@@ -5,8 +5,8 @@
 // (or 1) out per element; the tables add 8 bytes per pair and token.  A CTA serves one token (or a share of its heads when
 // tokens are few), and a thread keeps the same 8 columns for all its heads, so the cosines, sines, page lookup and position
 // are fetched once per thread; the first three heads' loads are issued ahead of that chain of lookups.
-// 16384 tokens, 56 + 2 x 8 heads of 128 into an e4m3 cache: 104 us = 5.5 TB/s, 0.85 of the measured copy bandwidth (CTAs of 256 threads with four heads
-// per thread: 155 us; 64 threads with five: 101 us, but 0.3 us more for the 64 tokens of a decode step, which take 2.5 us).
+// 16384 tokens, 56 + 2 x 8 heads of 128 into an e4m3 cache: 97 us = 5.9 TB/s, 0.91 of the measured copy bandwidth (CTAs of 64 threads with
+// five heads per thread: 98 us, and 0.2 us more for the 64 tokens of a decode step, which take 2.3).
 #include "internal.h"
 
 namespace dsuf {
@@ -25,7 +25,7 @@ struct AppendArgs {
     const float *k_scale, *v_scale;
     long long page_stride;
     const float *cos, *sin;
-    int rope_rows, rot, off, half;
+    int rope_rows, rot, off;
     DevStatus* status;
 };
 
@@ -59,7 +59,8 @@ DSUF_DEV uint4 pack8(const float* x) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <int D, bool FP8>
+// HALF: pairs rot / 2 apart (a kernel of its own, as the exchange costs the other form 10 registers and with them resident CTAs: 104 us instead of 97).
+template <int D, bool FP8, bool HALF>
 __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(const AppendArgs a) {
     constexpr int LANES = D / 8;                 // threads of one head
     constexpr int HPC = AP_THREADS / LANES;      // heads a CTA handles at a time
@@ -99,8 +100,8 @@ __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(const AppendArgs 
     const bool second = turn && rel >= a.rot / 2;   // half form: the second member of the pairs
     float cs[8], sn[8];
     if (turn) {
-        const int i0 = a.half ? rel - (second ? a.rot / 2 : 0) : rel / 2;
-        const int n4 = a.half ? 2 : 1;
+        const int i0 = HALF ? rel - (second ? a.rot / 2 : 0) : rel / 2;
+        const int n4 = HALF ? 2 : 1;
         const float4* cp = reinterpret_cast<const float4*>(a.cos + (size_t)pos * (a.rot / 2) + i0);
         const float4* sp = reinterpret_cast<const float4*>(a.sin + (size_t)pos * (a.rot / 2) + i0);
 #pragma unroll
@@ -112,7 +113,7 @@ __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(const AppendArgs 
             }
         }
     }
-    const int partner = a.half ? (second ? -a.rot / 16 : a.rot / 16) : 0;   // lanes to the other member of the pair
+    const int partner = HALF ? (second ? -a.rot / 16 : a.rot / 16) : 0;   // lanes to the other member of the pair
     const size_t slot = (size_t)(pos & ((1 << a.page_shift) - 1));
     for (int h0 = blockIdx.y * HPC; h0 < H; h0 += gridDim.y * HPC * AP_BATCH) {
         if (h0 >= (int)(gridDim.y * HPC * AP_BATCH)) load(h0);
@@ -121,7 +122,7 @@ __global__ void __launch_bounds__(AP_THREADS) kv_append_kernel(const AppendArgs 
             const int h = h0 + j * gridDim.y * HPC + threadIdx.x / LANES;
             float x[8];
             unpack8(raw[j], x);
-            if (a.half) {
+            if constexpr (HALF) {
                 // every lane of the warp takes part; lanes outside the rotated columns read themselves
                 const int from = (threadIdx.x & 31) + (turn ? partner : 0);
                 uint4 o;
@@ -218,14 +219,18 @@ extern "C" int32_t dsuf_kv_append(dsuf_ctx* ctx, void* stream, const dsuf_kv_cac
     a.page_stride = cache->page_stride;
     if (rope) {
         a.cos = (const float*)rope->cos; a.sin = (const float*)rope->sin;
-        a.rope_rows = rope->positions; a.rot = rope->rot; a.off = rope->off; a.half = rope->half ? 1 : 0;
+        a.rope_rows = rope->positions; a.rot = rope->rot; a.off = rope->off;
     }
     a.status = ctx->dev_status;
     // few tokens: several CTAs share a token's heads, so that its loads are not queued behind one another in one CTA
     const int groups = ((q_heads + 2 * cache->kv_heads) * (D / 8) + AP_THREADS - 1) / AP_THREADS;
     int share = (2 * ctx->sm_count + t - 1) / t;
     if (share > groups) share = groups;
-    auto kern = cache->dtype == DSUF_KV_E4M3 ? (D == 64 ? kv_append_kernel<64, true> : kv_append_kernel<128, true>)
-                                             : (D == 64 ? kv_append_kernel<64, false> : kv_append_kernel<128, false>);
+    void (*kern)(AppendArgs);
+    const bool fp8 = cache->dtype == DSUF_KV_E4M3, half = rope && rope->half;
+    if (D == 64) kern = fp8 ? (half ? kv_append_kernel<64, true, true> : kv_append_kernel<64, true, false>)
+                            : (half ? kv_append_kernel<64, false, true> : kv_append_kernel<64, false, false>);
+    else kern = fp8 ? (half ? kv_append_kernel<128, true, true> : kv_append_kernel<128, true, false>)
+                    : (half ? kv_append_kernel<128, false, true> : kv_append_kernel<128, false, false>);
     return launch(ctx, (cudaStream_t)stream, kern, dim3(t, share), dim3(AP_THREADS), 0, a);
 }
