@@ -20,8 +20,9 @@
 // from the list: ranks, both limits, min-p and the draw (129280 logits, top_k 50, top_p 0.9: 16 us instead of 38).
 // What the CTAs tell each other is pushed into everybody's shared memory before a barrier, not fetched after it: a remote load costs
 // about 250 cycles, and there are many.
-// With many rows the passes are bound by instructions, not by bytes (64 rows of 129280 flat logits, top_p 0.9, 67 us: the largest logit 5, weights and
-// histogram 16, list 8, kept weights 13; the histogram's atomics are 1 of it), so every pass computes no more than it needs.
+// With many rows the passes are bound by instructions, not by bytes (64 rows of 129280 flat logits, top_p 0.9: 57 us, with the weights by scalar
+// instructions 66, of which the largest logit took 5, weights and histogram 16, the list 8 and the kept weights 13; the histogram's atomics are 1 of it),
+// so every pass computes no more than it needs.
 // The exponent is carried in two fp32 numbers ((l - M) / T rounded to one would be off by 1e-6 relative in a far token's weight).
 #include "internal.h"
 
@@ -108,20 +109,18 @@ struct Sampler {
 #pragma unroll
         for (int e = 0; e < 4; ++e) l[e] = i + e >= 0 && i + e < a.n ? clean(x[i + e]) : -INFINITY;
     }
-    // f(id, logit) for every element of this warp's part.  Lines that reach over the row's ends are read by elements.  LIGHT: f is a few instructions, so
-    // four lines at a time; else one, with two more on their way (sixteen copies of a long f do not stay in the instruction cache: 64 rows
-    // of 129280 logits, top_p 0.9, 70 us instead of 67; 16 rows 58 instead of 48).
+    // f(id, logit, the next id's logit) for all pairs of elements of this warp's part.  Lines that reach over the row's ends are read by elements (what
+    // lies outside is -inf).  LIGHT: f is a few instructions, so four lines at a time; else one, with two more on their way (sixteen copies of a long f
+    // do not stay in the instruction cache: 64 rows of 129280 logits, top_p 0.9, 70 us instead of 67; 16 rows 58 instead of 48).
     template <bool LIGHT = false, typename F>
-    DSUF_DEV void each(F f) const {
+    DSUF_DEV void each_pair(F f) const {
         const int full0 = lead > 0 ? 1 : 0, full1 = (a.n + lead) >> 2;
         const float4* lines = reinterpret_cast<const float4*>(x - lead);
         const int end = min(v1, full1);
         int v = max(v0, full0) + lane;
         auto four = [&](int w, float4 q) {
-            f(4 * w - lead, clean(q.x));
-            f(4 * w - lead + 1, clean(q.y));
-            f(4 * w - lead + 2, clean(q.z));
-            f(4 * w - lead + 3, clean(q.w));
+            f(4 * w - lead, clean(q.x), clean(q.y));
+            f(4 * w - lead + 2, clean(q.z), clean(q.w));
         };
         if (LIGHT) {
             for (; v + 96 < end; v += 128) {
@@ -145,22 +144,44 @@ struct Sampler {
             if (cut && w >= v0 && w < v1) {
                 float l[4];
                 line(w, l);
-                for (int e = 0; e < 4; ++e) f(4 * w - lead + e, l[e]);
+                for (int e = 0; e < 4; e += 2) f(4 * w - lead + e, l[e], l[e + 1]);
             }
         }
     }
-    // exp((l - top) / T).  The difference and the product are carried as unevaluated sums of two fp32 numbers (Knuth's two-sum, an fma for the
-    // product's rest), because a rounding of the exponent is a relative error of the weight; the rests enter as a factor 1 + rest.
-    DSUF_DEV float weight(float l) const {
-        const float d = fminf(l - top, 0.f);          // (inf - inf is NaN: 0)
-        const float v = d - l;
-        const float d_rest = top < INFINITY ? (l - (d - v)) - (top + v) : 0.f;
-        const float z = d * inv_temp;
-        const float z_rest = fmaf(d, inv_temp, -z) + fmaf(d, inv_temp_rest, d_rest * inv_temp);
-        float w;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(z));
-        return z > -100.f ? fmaf(w, z_rest * 0.6931471805599453f, w) : 0.f;
+    // f(id, logit)
+    template <bool LIGHT = false, typename F>
+    DSUF_DEV void each(F f) const {
+        each_pair<LIGHT>([&](int id, float l0, float l1) {
+            f(id, l0);
+            f(id + 1, l1);
+        });
     }
+    // exp((l - top) / T) of two logits, by packed instructions.  The difference and the product are carried as unevaluated sums of two fp32 numbers
+    // (Knuth's two-sum, an fma for the product's rest), because a rounding of the exponent is a relative error of the weight; the rests enter as a
+    // factor 1 + rest.
+    DSUF_DEV float2 weights(float l0, float l1) const {
+        if (top == INFINITY) return make_float2(l0 == top ? 1.f : 0.f, l1 == top ? 1.f : 0.f);
+        const u64 l = pack_f32x2(l0, l1), t = pack_f32x2(top, top), inv = pack_f32x2(inv_temp, inv_temp);
+        const u64 d = sub2(l, t), v = sub2(d, l);
+        const u64 rest = sub2(sub2(l, sub2(d, v)), add2(t, v));
+        const u64 minus_z = mul2(d, pack_f32x2(-inv_temp, -inv_temp));
+        const u64 z_rest = fma2(rest, inv, fma2(d, pack_f32x2(inv_temp_rest, inv_temp_rest), fma2(d, inv, minus_z)));
+        const float2 y = unpack(mul2(z_rest, pack_f32x2(0.6931471805599453f, 0.6931471805599453f))), z = unpack(minus_z);
+        float2 w;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w.x) : "f"(-z.x));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w.y) : "f"(-z.y));
+        return make_float2(z.x < 100.f ? fmaf(w.x, y.x, w.x) : 0.f, z.y < 100.f ? fmaf(w.y, y.y, w.y) : 0.f);
+    }
+    DSUF_DEV float weight(float l) const { return weights(l, l).x; }
+    DSUF_DEV static float2 unpack(u64 v) {
+        float2 r;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+        return r;
+    }
+    DSUF_DEV static u64 add2(u64 x, u64 y) { u64 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y)); return r; }
+    DSUF_DEV static u64 sub2(u64 x, u64 y) { u64 r; asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y)); return r; }
+    DSUF_DEV static u64 mul2(u64 x, u64 y) { u64 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y)); return r; }
+    DSUF_DEV static u64 fma2(u64 x, u64 y, u64 z) { u64 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z)); return r; }
     // w * 2^40, truncated
     DSUF_DEV static u64 fixed(float w) {
         return __float2ull_rz(w * (float)(1ull << SA_FRACTION));
@@ -666,12 +687,21 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleArgs 
             lim = z.limit(false, (u64)top_k, 0.0, lim, b, before);
         }
     }
+    const bool few = cut;                  // the limits leave so little of the row that most warps meet none of it: they skip the weights
     if (top_p < 1.f) {
         z.clear_bins();    // (the others read this CTA's histogram before the last barrier)
-        z.each([&](int id, float l) {
-            if (want_lp) add_lp(l);
-            if (!cut || lim.holds(l, id)) z.add(z.bin(l), z.fixed(z.weight(l)));
-        });
+        if (few)
+            z.each([&](int id, float l) { if (lim.holds(l, id)) z.add(z.bin(l), z.fixed(z.weight(l))); });
+        else
+            z.each_pair([&](int id, float l0, float l1) {
+                if (want_lp) {
+                    add_lp(l0);
+                    add_lp(l1);
+                }
+                const float2 w = z.weights(l0, l1);
+                z.add(z.bin(l0), z.fixed(w.x));
+                z.add(z.bin(l1), z.fixed(w.y));
+            });
         if (want_lp) share_lp();
         want_lp = false;
         z.share_bins(true);
@@ -698,18 +728,27 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleArgs 
         lim = z.limit(true, 0, target, lim, b, before);
         cut = true;
     }
-    if (cut) {
+    if (few) {
         z.each([&](int id, float l) {
             if (lim.holds(l, id)) {
                 const float w = z.weight(l);
                 if (w >= min_p) sum += z.fixed(w);
             }
         });
+    } else if (cut) {
+        z.each_pair([&](int id, float l0, float l1) {
+            const float2 w = z.weights(l0, l1);
+            if (lim.holds(l0, id) && w.x >= min_p) sum += z.fixed(w.x);
+            if (lim.holds(l1, id + 1) && w.y >= min_p) sum += z.fixed(w.y);
+        });
     } else {
-        z.each([&](int id, float l) {
-            if (want_lp) add_lp(l);
-            const float w = z.weight(l);
-            sum += w >= min_p ? z.fixed(w) : 0;
+        z.each_pair([&](int id, float l0, float l1) {
+            if (want_lp) {
+                add_lp(l0);
+                add_lp(l1);
+            }
+            const float2 w = z.weights(l0, l1);
+            sum += (w.x >= min_p ? z.fixed(w.x) : 0) + (w.y >= min_p ? z.fixed(w.y) : 0);
         });
         if (want_lp) share_lp();
     }
