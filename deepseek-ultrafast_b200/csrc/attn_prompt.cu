@@ -19,7 +19,7 @@
 // (8192 tokens, 56 / 8 heads of 128: one issuing warp 867 us, two without turns 1022, two with turns 778; now 765 = 1255 TFLOP/s
 // of visible pairs, with the tensor pipe and the exponential unit each 54 % busy.)
 // Tensor memory (512 columns): S0 S1 (128 fp32 columns each; P_t overwrites the first 64 of S_t as packed bf16), O0 O1 (D each).
-// The reference point of a row is the largest of its first 32 scores and only moves when a tile's weights add up to more than 2^24 (exact: the
+// The reference point of a row is the largest of 32 scores of its first tile and only moves when a tile's weights add up to more than 2^24 (exact: the
 // sum and the output share the reference, and bf16's and fp32's precision does not depend on the magnitude), so usual tiles need no maximum at
 // all.  p is rounded once to bf16 as operand; sums, statistics and outputs are fp32.
 //
@@ -291,7 +291,8 @@ __device__ __noinline__ void prompt_repair(const PromptArgs& a, unsigned rows, i
     }
 }
 
-template <int D>
+// WINDOW: with a sliding window (a kernel of its own: what only windows need costs the other 4 % of its time).
+template <int D, bool WINDOW>
 __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid_constant__ PromptArgs a) {
     using S = PromptShape<D>;
     constexpr int BOX = PA_BM * 128;                 // bytes of one box
@@ -515,19 +516,21 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
                 ++sn;
                 tc_fence_after();
                 const int upper = row - j * PA_BM;                                  // last visible column of the tile
-                const int lower = a.window > 0 ? upper - a.window : -1;             // last column hidden by the window
-                const bool windowed = a.window > 0 && q.qb * PA_BM + PA_BM - 1 - j * PA_BM >= a.window, diagonal = j == q.hi - 1;
+                const int lower = WINDOW ? upper - a.window : -1;             // last column hidden by the window
+                const bool windowed = WINDOW && q.qb * PA_BM + PA_BM - 1 - j * PA_BM >= a.window, diagonal = j == q.hi - 1;
                 uint32_t w[64];
-                if (j == q.lo) {
-                    // the first tile's reference: the largest of 32 scores (every row sees column 0, but for a window)
+                if (WINDOW ? __any_sync(0xffffffffu, ref == PA_UNSET) : j == q.lo) {
+                    // a row's first reference: the largest of 32 scores that it sees.  Without a window every row sees column 0; of a tile that only the
+                    // window cuts a row sees the last columns or none; where the diagonal cuts too, its own column.
+                    const int at = !WINDOW || !windowed ? 0 : diagonal ? (warp & 3) * 32 : 96;
                     float s[32], top = -INFINITY;
-                    tmem_ld<32>(tS, s);
+                    tmem_ld<32>(tS + at, s);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) top = fmaxf(top, pa_seen(e, upper, lower) ? s[e] : -INFINITY);
-                    ref = fmaxf(top * sl2, PA_UNSET);
+                    for (int e = 0; e < 32; ++e) top = fmaxf(top, pa_seen(at + e, upper, lower) ? s[e] : -INFINITY);
+                    if (!WINDOW || ref == PA_UNSET) ref = fmaxf(top * sl2, PA_UNSET);
                 }
                 float part;
-                if (windowed) part = pa_weights<2>(tS, sl2, ref, upper, lower, w);
+                if (WINDOW && windowed) part = pa_weights<2>(tS, sl2, ref, upper, lower, w);
                 else if (diagonal) part = pa_weights<1>(tS, sl2, ref, upper, lower, w);
                 else part = pa_weights<0>(tS, sl2, ref, upper, lower, w);
                 const bool fine = part <= PA_TRIGGER && !pa_far(ref);
@@ -632,9 +635,13 @@ static bool rows_overlap(uint64_t out, long long ldo, long long wo, uint64_t x, 
     return apart < w || apart + wo > ld;
 }
 
+template <int D, bool WINDOW>
+static cudaError_t prompt_attr() { return cudaFuncSetAttribute(attn_prompt_kernel<D, WINDOW>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<D>::SMEM); }
 int attn_prompt_setup(dsuf_ctx* ctx) {
-    cudaError_t e = cudaFuncSetAttribute(attn_prompt_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<64>::SMEM);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(attn_prompt_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<128>::SMEM);
+    cudaError_t e = prompt_attr<64, false>();
+    if (e == cudaSuccess) e = prompt_attr<64, true>();
+    if (e == cudaSuccess) e = prompt_attr<128, false>();
+    if (e == cudaSuccess) e = prompt_attr<128, true>();
     return e == cudaSuccess ? DSUF_OK : cuda_fail(ctx, e, "cudaFuncSetAttribute(attn_prompt)");
 }
 
@@ -678,6 +685,8 @@ extern "C" int32_t dsuf_attn_prompt(dsuf_ctx* ctx, void* stream, uint64_t q, int
     const long long blocks = (long long)(t / PA_BM) + (t < n_seqs ? t : n_seqs);
     const long long cap = (blocks * a.group + 1) * kv_heads;
     const int grid = (int)(cap < ctx->sm_count ? cap : ctx->sm_count);
-    if (head_dim == 64) return launch(ctx, (cudaStream_t)stream, attn_prompt_kernel<64>, dim3(grid), dim3(PA_THREADS), (size_t)PromptShape<64>::SMEM, a);
-    return launch(ctx, (cudaStream_t)stream, attn_prompt_kernel<128>, dim3(grid), dim3(PA_THREADS), (size_t)PromptShape<128>::SMEM, a);
+    const size_t smem = head_dim == 64 ? PromptShape<64>::SMEM : PromptShape<128>::SMEM;
+    void (*kern)(PromptArgs) = head_dim == 64 ? (window ? attn_prompt_kernel<64, true> : attn_prompt_kernel<64, false>)
+                                              : (window ? attn_prompt_kernel<128, true> : attn_prompt_kernel<128, false>);
+    return launch(ctx, (cudaStream_t)stream, kern, dim3(grid), dim3(PA_THREADS), smem, a);
 }

@@ -277,6 +277,23 @@ def test_prompt(pkg, actx, d, hq, hkv, lens, window):
 
 # ------------------------------------------------------------------ strides, streams, workspaces
 @gpu
+@pytest.mark.parametrize("d,window", [(128, 1024), (64, 1000), (128, 127), (64, 129), (128, 255), (64, 32)])
+def test_prompt_windows_over_many_tiles(pkg, actx, d, window):
+    """Windows that end on, before and behind a tile's border, with scores that differ by far more inside a row than in its first columns."""
+    lens, hq, hkv = [2300, 1, 700], 6, 2
+    g = gen(71 + window)
+    t = sum(lens)
+    q, k, v = bf16(g, t, hq * d, std=3.0), bf16(g, t, hkv * d, std=2.0), bf16(g, t, hkv * d)
+    cu = torch.tensor([0, 2300, 2301, 3001], dtype=torch.int32, device=DEV)
+    out, lse = pkg.attn_prompt(actx, q, k, v, cu, head_dim=d, window=window, return_lse=True)
+    torch.cuda.synchronize()
+    assert actx.status().code == 0
+    want, wl, size = prompt64(q, k, v, lens, hq, hkv, d, window, d ** -0.5)
+    within(out.reshape(want.shape), want, size, terms=2 ** -8 + 2 ** -12)
+    assert ((lse.double() - wl).abs() <= 2 ** -12 + 2 ** -20 * wl.abs()).all()
+
+
+@gpu
 @pytest.mark.parametrize("fp8", [False, True])
 def test_interleaved_layers_and_far_pages(pkg, actx, fp8):
     """Pages of two layers interleaved in one allocation (a page stride of its own), and a pool of more than 2^31 elements, so that an offset
