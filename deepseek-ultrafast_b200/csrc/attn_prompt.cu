@@ -19,7 +19,7 @@
 // (8192 tokens, 56 / 8 heads of 128: one issuing warp 867 us, two without turns 1022, two with turns 778; now 765 = 1255 TFLOP/s
 // of visible pairs, with the tensor pipe and the exponential unit each 54 % busy.)
 // Tensor memory (512 columns): S0 S1 (128 fp32 columns each; P_t overwrites the first 64 of S_t as packed bf16), O0 O1 (D each).
-// The reference point of a row is the largest of 32 scores of its first tile and only moves when a tile's weights add up to more than 2^24 (exact: the
+// The reference point of a row is the largest of 16 or 32 scores of its first tile and only moves when a tile's weights add up to more than 2^24 (exact: the
 // sum and the output share the reference, and bf16's and fp32's precision does not depend on the magnitude), so usual tiles need no maximum at
 // all.  p is rounded once to bf16 as operand; sums, statistics and outputs are fp32.
 //
@@ -520,13 +520,15 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
                 const bool windowed = WINDOW && q.qb * PA_BM + PA_BM - 1 - j * PA_BM >= a.window, diagonal = j == q.hi - 1;
                 uint32_t w[64];
                 if (WINDOW ? __any_sync(0xffffffffu, ref == PA_UNSET) : j == q.lo) {
-                    // a row's first reference: the largest of 32 scores that it sees.  Without a window every row sees column 0; of a tile that only the
+                    // a row's first reference: the largest of some scores that it sees (of 16 without a window, where every row sees column 0: of 32, 1 % more
+                    // of the kernel's time).  Of a tile that only the
                     // window cuts a row sees the last columns or none; where the diagonal cuts too, its own column.
                     const int at = !WINDOW || !windowed ? 0 : diagonal ? (warp & 3) * 32 : 96;
-                    float s[32], top = -INFINITY;
-                    tmem_ld<32>(tS + at, s);
+                    constexpr int FIRST = WINDOW ? 32 : 16;
+                    float s[FIRST], top = -INFINITY;
+                    tmem_ld<FIRST>(tS + at, s);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) top = fmaxf(top, pa_seen(at + e, upper, lower) ? s[e] : -INFINITY);
+                    for (int e = 0; e < FIRST; ++e) top = fmaxf(top, pa_seen(at + e, upper, lower) ? s[e] : -INFINITY);
                     if (!WINDOW || ref == PA_UNSET) ref = fmaxf(top * sl2, PA_UNSET);
                 }
                 float part;
