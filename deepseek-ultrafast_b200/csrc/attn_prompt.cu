@@ -16,15 +16,15 @@
 // issued before the last output is stored.  The two issuing warps take strict turns (P0 V, S0, P1 V, S1): issuing blocks while the tensor
 // core's short queue is full, so the barrier waits of one tile (100 cycles and more each, even when met) have to pass while the
 // other's products are issued; without turns the tiles fall into step, and both softmaxes share the exponential unit and then both wait.
-// (8192 tokens, 56 / 8 heads of 128: one issuing warp 867 us, two without turns 1022, two with turns 778; now 765 = 1255 TFLOP/s
+// (8192 tokens, 56 / 8 heads of 128: one issuing warp 867 us, two without turns 1022, two with turns 778; now 757 = 1270 TFLOP/s
 // of visible pairs, with the tensor pipe and the exponential unit each 54 % busy.)
 // Tensor memory (512 columns): S0 S1 (128 fp32 columns each; P_t overwrites the first 64 of S_t as packed bf16), O0 O1 (D each).
 // The reference point of a row is the largest of 16 or 32 scores of its first tile and only moves when a tile's weights add up to more than 2^24 (exact: the
 // sum and the output share the reference, and bf16's and fp32's precision does not depend on the magnitude), so usual tiles need no maximum at
 // all.  p is rounded once to bf16 as operand; sums, statistics and outputs are fp32.
 //
-// Pairs are ordered from the longest rows to the shortest inside a sequence and dealt to the CTAs back and forth, so that a CTA's
-// long and short pairs balance.  Values behind a sequence's end inside its last tile belong to another sequence (or nobody) and are
+// Pairs are ordered from the longest rows to the shortest, those of all sequences together, and dealt to the CTAs back and forth, which
+// leaves the CTAs within 1 or 2 % of one another (9 prompts of 900 to 2600 tokens: 332 us; sequence after sequence 8 % apart and 342; one of 2048 69 instead of 74).  Values behind a sequence's end inside its last tile belong to another sequence (or nobody) and are
 // zeroed in shared memory before use: p is 0 there, but 0 x NaN is not.
 #include "internal.h"
 
@@ -127,13 +127,22 @@ struct PromptPair {
     }
 };
 
-// Walks the pairs of one CTA: row r of the deal takes index r * grid + c, or counted from the other end in odd rows.  A whole warp calls
-// next() together: its lanes look at 32 sequences at a time.
+// Walks the pairs of one CTA: row r of the deal takes index r * grid + c, or counted from the other end in odd rows.  The indexes go by level, the number
+// of key tiles up to a pair's diagonal, from the highest down, and inside a level by sequence.  Of a sequence of T blocks of 128 rows, blocks h - 1 and
+// before have h group query tiles, so the pairs of level h are those from (h - 1) group / 2 to h group / 2 (T group / 2 rounded up, for the last): how many
+// pairs a level has follows from the numbers of sequences with T > h and T = h.  A whole warp calls next() together: its lanes look at 32 sequences at a time.
 struct PromptWalk {
     const PromptArgs& a;
-    int row = 0, seq = 0;        // seq: first of the 32 sequences looked at
-    long long before = 0;        // pairs of the sequences below it
-    DSUF_DEV explicit PromptWalk(const PromptArgs& a_) : a(a_) {}
+    int row = 0, seq = 0, level = 0;      // seq: first of the 32 sequences looked at
+    long long before = 0;                 // pairs of the levels above, and of the sequences below it in this one
+    DSUF_DEV explicit PromptWalk(const PromptArgs& a_) : a(a_) {
+        for (int s = 0; s < a.n_seqs; s += 32) {
+            int start, len;
+            bounds(s + (threadIdx.x & 31), start, len);
+            level = max(level, (len + PA_BM - 1) / PA_BM);
+        }
+        level = __reduce_max_sync(0xffffffffu, level);
+    }
     DSUF_DEV void bounds(int s, int& start, int& len) const {
         start = len = 0;
         if (s < a.n_seqs) {
@@ -151,30 +160,28 @@ struct PromptWalk {
     }
     DSUF_DEV PromptPair next() {
         const int lane = threadIdx.x & 31;
+        const unsigned below = (2u << lane) - 1u;      // the lanes up to this one
         PromptPair p;
         p.ok = false;
         const long long x = (long long)row * gridDim.x + ((row & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
         ++row;
-        for (; seq < a.n_seqs; seq += 32) {
-            int start, len;
-            bounds(seq + lane, start, len);
-            const long long mine = (long long)((((len + PA_BM - 1) / PA_BM) * a.group + 1) / 2) * a.kv_heads;
-            long long upto = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long v = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += v;
-            }
-            const unsigned past = __ballot_sync(0xffffffffu, before + upto > x);
-            if (past) {
-                const int owner = __ffs(past) - 1;
+        int start = 0, len = 0;
+        for (bool load = true; level > 0; load = a.n_seqs > 32) {
+            if (load) bounds(seq + lane, start, len);
+            const int blocks = (len + PA_BM - 1) / PA_BM;
+            const unsigned higher = __ballot_sync(0xffffffffu, blocks > level), here = __ballot_sync(0xffffffffu, blocks == level);
+            const int first = (level - 1) * a.group / 2, full = level * a.group / 2 - first, last = (level * a.group + 1) / 2 - first;      // pairs per kv head
+            const int all = (__popc(higher) * full + __popc(here) * last) * a.kv_heads;
+            if (x < before + all) {
+                const int upto = (__popc(higher & below) * full + __popc(here & below) * last) * a.kv_heads;
+                const int owner = __ffs(__ballot_sync(0xffffffffu, before + upto > x)) - 1;
+                const int mine = (blocks > level ? full : blocks == level ? last : 0) * a.kv_heads;
+                const int local = (int)(x - before) - __shfl_sync(0xffffffffu, upto - mine, owner);
                 p.start = __shfl_sync(0xffffffffu, start, owner);
                 p.len = __shfl_sync(0xffffffffu, len, owner);
-                const int local = (int)(x - before - __shfl_sync(0xffffffffu, upto - mine, owner));
                 const int tiles = ((p.len + PA_BM - 1) / PA_BM) * a.group;
-                const int rank = local / a.kv_heads;
+                const int pair = first + local / a.kv_heads;
                 p.kvh = local % a.kv_heads;
-                const int pair = (tiles + 1) / 2 - 1 - rank;
                 p.t0 = tile(2 * pair, tiles, p.kvh);
                 p.t1 = tile(2 * pair + 1, tiles, p.kvh);
                 p.jlo = p.t0.lo;                              // (the second tile's rows are the same or later ones)
@@ -182,7 +189,12 @@ struct PromptWalk {
                 p.ok = true;
                 return p;
             }
-            before += __shfl_sync(0xffffffffu, upto, 31);
+            before += all;
+            seq += 32;
+            if (seq >= a.n_seqs) {
+                seq = 0;
+                --level;
+            }
         }
         return p;
     }

@@ -277,6 +277,24 @@ def test_prompt(pkg, actx, d, hq, hkv, lens, window):
 
 # ------------------------------------------------------------------ strides, streams, workspaces
 @gpu
+@pytest.mark.parametrize("hq,hkv", [(3, 1), (4, 2), (5, 1)])
+@pytest.mark.parametrize("window", [0, 100])
+def test_prompt_of_many_sequences(pkg, actx, hq, hkv, window):
+    """More sequences than a warp looks at together, of all lengths, so that every level of the deal takes from several groups of 32."""
+    d = 64
+    lens = [(53 * i * i) % 700 if i % 5 else 0 for i in range(75)]
+    g = gen(81 + hq)
+    t = sum(lens)
+    q, k, v = bf16(g, t, hq * d), bf16(g, t, hkv * d), bf16(g, t, hkv * d)
+    cu = torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32, device=DEV)
+    out = pkg.attn_prompt(actx, q, k, v, cu, head_dim=d, window=window)
+    torch.cuda.synchronize()
+    assert actx.status().code == 0
+    want, _, size = prompt64(q, k, v, lens, hq, hkv, d, window, d ** -0.5)
+    within(out.reshape(want.shape), want, size, terms=2 ** -8 + 2 ** -12)
+
+
+@gpu
 @pytest.mark.parametrize("d,window", [(128, 1024), (64, 1000), (128, 127), (64, 129), (128, 255), (64, 32)])
 def test_prompt_windows_over_many_tiles(pkg, actx, d, window):
     """Windows that end on, before and behind a tile's border, with scores that differ by far more inside a row than in its first columns."""
