@@ -12,7 +12,7 @@
 // ends leaves fp32 partials (output, reference point, sum) in the workspace and the CTA that arrives last adds them in CTA order,
 // so the result does not depend on timing.  Where there are few units, segments of four of one piece are dealt instead of units (8 contexts
 // of 1000 tokens, 56 / 8 heads of 128: 12.8 us instead of 14.5; one of 16000, one kv head: 14.0 instead of 24.6).  Where every piece is short (four
-// units at most) and there is one for each CTA, a warp takes whole pieces alone and writes them itself: no barrier and no other warp's part to add
+// units at most) and there is one for each CTA that the GPU holds, a warp takes whole pieces alone and writes them itself: no barrier and no other warp's part to add
 // (56 / 8 heads of 128; 512 contexts of 128 tokens: 56 us instead of 68; 256 of 1 to 256: 37 instead of 61; 64 of 40: 7.6 instead of 10; with half as many pieces
 // as CTAs it would lose: 32 of 100 tokens 9.6 instead of 7.6).
 //
@@ -44,7 +44,7 @@ constexpr int AD_RING = AD_WARPS * AD_STAGES * 2 * AD_HALF;
 constexpr int AD_PART = 16 * 128;                          // floats of one partial output
 constexpr int AD_JOIN = 16;                                // partials whose loads are in flight together when a piece is joined
 constexpr int AD_SEGMENT_SHIFT = 2;                        // log2 of the units of a segment when there are few
-constexpr unsigned AD_SOLO_UNITS = 4, AD_SOLO_PIECES = 1;    // a warp per piece: pieces of at most so many units, at least so many per CTA
+constexpr unsigned AD_SOLO_UNITS = 4;                      // a warp per piece: pieces of at most so many units, and one for every CTA that the GPU holds
 constexpr float AD_UNSET = -3e38f;                        // below every finite score
 constexpr float AD_TRIGGER = 15.f, AD_HEADROOM = 7.f;
 
@@ -61,6 +61,7 @@ struct DecodeArgs {
     float scale_log2;
     float *part, *part_ml;                                 // [CTA][2][16][128] and [CTA][2][16][2]
     int* counter;                                          // [CTA]
+    unsigned solo_from;                                    // pieces
     DevStatus* status;
 };
 
@@ -287,10 +288,10 @@ __global__ void __launch_bounds__(AD_THREADS, 2) attn_decode_kernel(const Decode
     int unit = S::CH_SHIFT + 2, seg = 0;
     unsigned upto = sum_up(unit, 0);
     const bool few = __shfl_sync(0xffffffffu, upto, 31) < gridDim.x << AD_SEGMENT_SHIFT;
-    bool solo = (unsigned)(a.b * HB) >= AD_SOLO_PIECES * gridDim.x && __reduce_max_sync(0xffffffffu, longest) <= AD_SOLO_UNITS;
+    bool solo = (unsigned)(a.b * HB) >= a.solo_from && __reduce_max_sync(0xffffffffu, longest) <= AD_SOLO_UNITS;
     if (solo) {
         const unsigned pieces = sum_up(unit, 20);
-        solo = __shfl_sync(0xffffffffu, pieces, 31) >= AD_SOLO_PIECES * gridDim.x;
+        solo = __shfl_sync(0xffffffffu, pieces, 31) >= a.solo_from;
         upto = pieces;
     }
     if (solo) {
@@ -819,6 +820,7 @@ int32_t dsuf_attn_decode(dsuf_ctx* ctx, void* stream, const dsuf_kv_cache* cache
     a.part = (float*)workspace;
     a.part_ml = a.part + (size_t)n * 2 * AD_PART;
     a.counter = (int*)(a.part_ml + (size_t)n * 2 * 32);
+    a.solo_from = (unsigned)n;
     a.status = ctx->dev_status;
     cudaStream_t s = (cudaStream_t)stream;
     if (a.group <= 8) {   // one column block of 8 heads holds the group; larger groups go by 16 (half the passes over the cache)
