@@ -651,6 +651,7 @@ class KvCache:
         for name, x in (("k", k), ("v", v)):
             _need(isinstance(x, t.Tensor) and x.device == ctx.device and x.dtype == k.dtype and x.shape == k.shape, f"KvCache: {name}: type, shape or device")
             _need(x.stride()[1:] == (p * d, d, 1) and x.stride(0) == k.stride(0), f"KvCache: {name}: the heads of a page must be contiguous, k's and v's pages equally far apart")
+            _need(n < 2 or x.stride(0) >= h * p * d, f"KvCache: {name}: pages must not overlap")
         for name, x in (("k_scale", k_scale), ("v_scale", v_scale)):
             if x is not None:
                 _need(isinstance(x, t.Tensor) and x.device == ctx.device and x.dtype == t.float32 and x.shape == (h,) and x.is_contiguous(),
@@ -658,7 +659,7 @@ class KvCache:
         self.ctx, self.k, self.v, self.k_scale, self.v_scale = ctx, k, v, k_scale, v_scale   # (keeps the tensors alive)
         self.n_pages, self.kv_heads, self.page_size, self.head_dim = n, h, p, d
         self.c = KvCacheStruct(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if k_scale is not None else 0,
-                               v_scale.data_ptr() if v_scale is not None else 0, max(k.stride(0), h * p * d) if n > 1 else h * p * d,
+                               v_scale.data_ptr() if v_scale is not None else 0, k.stride(0) if n > 1 else h * p * d,
                                KV_BF16 if k.dtype == t.bfloat16 else KV_E4M3, n, p, h, d)
         self.ref, self.address = C.byref(self.c), C.addressof(self.c)
 

@@ -1,0 +1,40 @@
+"""Calls at the edges of what the cache, attention and sampling entries document: what they refuse before anything reaches the GPU (on CPU tensors, with a
+zeroed block in the context's place), and rows, values and streams that the larger tests do not meet."""
+import ctypes as C
+import math
+import os
+import types
+
+import pytest
+import torch
+
+gpu = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.fixture()
+def hctx():
+    """A stand-in for a context, on the CPU: the entries check their arguments against it and get no further."""
+    block = C.create_string_buffer(64 << 10)
+    return types.SimpleNamespace(torch=torch, device=torch.device("cpu"), index=-1, address=C.addressof(block), block=block,
+                                 attn_workspace=torch.zeros(16, dtype=torch.uint8))
+
+
+def z(*shape, dt=torch.bfloat16):
+    return torch.zeros(*shape, dtype=dt)
+
+
+# ------------------------------------------------------------------ the cache's description
+def test_pages_that_overlap_are_refused(pkg, hctx):
+    """A page stride below a page's size would make the pages' addresses run past the tensor."""
+    page = 2 * 16 * 128
+    for k in (z(1, 2, 16, 128).expand(1000, 2, 16, 128), z(4 * page).as_strided((4, 2, 16, 128), (page - 16, 2048, 128, 1)),
+              z(4 * page).as_strided((4, 2, 16, 128), (2048, 2048, 128, 1))):
+        with pytest.raises(pkg.DsufError, match="KvCache"):
+            pkg.KvCache(hctx, k, k)
+    with pytest.raises(pkg.DsufError, match="KvCache"):
+        pkg.KvCache(hctx, z(4, 2, 16, 128), z(1, 2, 16, 128).expand(4, 2, 16, 128))
+    # one page has no stride; pages that touch or lie apart are theirs
+    one = pkg.KvCache(hctx, z(1, 2, 16, 128).expand(1, 2, 16, 128), z(1, 2, 16, 128))
+    assert one.c.page_stride == page and one.c.n_pages == 1
+    assert pkg.KvCache(hctx, z(3, 2, 16, 128), z(3, 2, 16, 128)).c.page_stride == page
