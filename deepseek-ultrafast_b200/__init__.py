@@ -648,6 +648,7 @@ class KvCache:
         t = ctx.torch
         _need(isinstance(k, t.Tensor) and k.dim() == 4 and k.dtype in (t.bfloat16, t.uint8), "KvCache: k must be bf16 or uint8 [pages][kv_heads][page][head_dim]")
         n, h, p, d = k.shape
+        _need(k.numel() > 0, "KvCache: k is empty")
         for name, x in (("k", k), ("v", v)):
             _need(isinstance(x, t.Tensor) and x.device == ctx.device and x.dtype == k.dtype and x.shape == k.shape, f"KvCache: {name}: type, shape or device")
             _need(x.stride()[1:] == (p * d, d, 1) and x.stride(0) == k.stride(0), f"KvCache: {name}: the heads of a page must be contiguous, k's and v's pages equally far apart")

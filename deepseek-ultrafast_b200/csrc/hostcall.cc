@@ -69,6 +69,12 @@ struct Call {
     at::Tensor make(at::IntArrayRef size, at::ScalarType type) const {
         return at::empty(size, at::TensorOptions().dtype(type).device(device < 0 ? at::Device(at::kCPU) : at::Device(at::kCUDA, (c10::DeviceIndex)device)));
     }
+    // The cache's description, as far as sizes are worked out from it here (the C entry checks the rest).
+    const dsuf_kv_cache* cache(PyObject* o) const {
+        const dsuf_kv_cache* k = (const dsuf_kv_cache*)PyLong_AsVoidPtr(o);
+        if ((k->head_dim != 64 && k->head_dim != 128) || k->kv_heads < 1) refuse(name("the cache has heads of 64 or 128 columns, and at least one"));
+        return k;
+    }
     void* stream() const { return device < 0 ? nullptr : (void*)c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream(); }
     template <typename F>
     void run(F f) const {
@@ -118,7 +124,7 @@ float real(const Call& c, PyObject* o, const char* what) {
 // (ctx, device, cache, k, v, pos, block_table, seq, rope, rope_half, q, q_out, k_out)
 PyObject* kv_append(PyObject* const* a) {
     Call c("kv_append", a[0], a[1]);
-    const dsuf_kv_cache* cache = (const dsuf_kv_cache*)PyLong_AsVoidPtr(a[2]);
+    const dsuf_kv_cache* cache = c.cache(a[2]);
     const int64_t d = cache->head_dim, kv = cache->kv_heads * d;
     int ldk, ldv, ldq = 0, ldqo = 0, ldko = 0, heads = 0;
     const at::Tensor& k = c.rows(a[3], "k", at::kBFloat16, -1, kv, ldk);
@@ -181,7 +187,7 @@ struct Results {
 // (ctx, device, cache, q, block_table, seq_lens, scale, window, out, lse, return_lse, workspace)
 PyObject* attn_decode(PyObject* const* a) {
     Call c("attn_decode", a[0], a[1]);
-    const dsuf_kv_cache* cache = (const dsuf_kv_cache*)PyLong_AsVoidPtr(a[2]);
+    const dsuf_kv_cache* cache = c.cache(a[2]);
     const int64_t d = cache->head_dim;
     int ldq;
     const at::Tensor& q = c.rows(a[3], "q", at::kBFloat16, -1, -1, ldq);

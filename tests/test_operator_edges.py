@@ -38,3 +38,37 @@ def test_pages_that_overlap_are_refused(pkg, hctx):
     one = pkg.KvCache(hctx, z(1, 2, 16, 128).expand(1, 2, 16, 128), z(1, 2, 16, 128))
     assert one.c.page_stride == page and one.c.n_pages == 1
     assert pkg.KvCache(hctx, z(3, 2, 16, 128), z(3, 2, 16, 128)).c.page_stride == page
+
+
+@pytest.mark.parametrize("shape", [(4, 0, 16, 128), (4, 2, 16, 0), (0, 2, 16, 128), (4, 2, 0, 128)])
+def test_empty_caches_are_refused(pkg, shape):
+    """In a process of its own: a division by the number of heads or columns would end it."""
+    import subprocess
+    import sys
+    code = f"""
+import ctypes as C, types, torch, sys
+sys.path.insert(0, {os.path.dirname(os.path.dirname(os.path.abspath(__file__)))!r})
+from __graft_entry__ import load_package
+pkg = load_package()
+block = C.create_string_buffer(64 << 10)
+ctx = types.SimpleNamespace(torch=torch, device=torch.device("cpu"), index=-1, address=C.addressof(block), attn_workspace=torch.zeros(16, dtype=torch.uint8))
+b, i = torch.bfloat16, torch.int32
+n, h, p, d = {shape}
+try:
+    pkg.KvCache(ctx, torch.zeros(n, h, p, d, dtype=b), torch.zeros(n, h, p, d, dtype=b))
+except pkg.DsufError:
+    print("cache refused")
+# the native entries by themselves, over a description that has not been checked
+c = types.SimpleNamespace(ctx=ctx, s=pkg.KvCacheStruct(1 << 20, 1 << 20, 0, 0, n * h * p * d, 0, n, p, h, d))
+c.address = C.addressof(c.s)
+for call in (lambda: pkg.attn_decode(ctx, c, torch.zeros(1, 512, dtype=b), torch.zeros(1, 1, dtype=i), torch.zeros(1, dtype=i)),
+             lambda: pkg.kv_append(ctx, c, torch.zeros(1, h * d, dtype=b), torch.zeros(1, h * d, dtype=b), torch.zeros(1, dtype=i), torch.zeros(1, 1, dtype=i),
+                                   q=torch.zeros(1, 512, dtype=b))):
+    try:
+        call()
+    except pkg.DsufError:
+        print("call refused")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, (r.returncode, r.stderr[-2000:])
+    assert r.stdout.split("\n")[:3] == ["cache refused", "call refused", "call refused"], r.stdout
