@@ -550,6 +550,7 @@ struct Sampler {
 __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleArgs a) {
     extern __shared__ __align__(16) uint8_t smem[];
     SampleShared& s = *reinterpret_cast<SampleShared*>(smem);
+    cluster_arrive();        // (waited for before the first write into a peer's shared memory: the peer has to have started)
     pdl_wait();
     pdl_launch_dependents();
     const uint32_t rank = cluster_cta_rank(), ctas = cluster_num_ctas();
@@ -573,6 +574,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) sample_kernel(const SampleArgs 
     if (lane == 0) s.warp_f[warp] = hi;
     if (tid == 0) s.own_first = 0x7fffffff;
     __syncthreads();
+    cluster_wait();
     if (tid < ctas) {
         for (int w = 0; w < SA_WARPS; ++w) hi = fmaxf(hi, s.warp_f[w]);
         *in_cta(&s.top[rank], tid) = hi;

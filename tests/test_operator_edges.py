@@ -72,3 +72,16 @@ for call in (lambda: pkg.attn_decode(ctx, c, torch.zeros(1, 512, dtype=b), torch
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, (r.returncode, r.stderr[-2000:])
     assert r.stdout.split("\n")[:3] == ["cache refused", "call refused", "call refused"], r.stdout
+
+
+# ------------------------------------------------------------------ the sampler's clusters
+def test_no_peer_memory_before_the_cluster_has_started(pkg):
+    """A CTA may touch another's shared memory only once that one is known to run, and whether it was is no result that a test could see: the kernel's
+    text has a completed cluster barrier ahead of the first such access."""
+    import re
+    with open(os.path.join(os.path.dirname(pkg.__file__), "csrc", "sample.cu")) as f:
+        text = re.sub(r"//[^\n]*", "", f.read())
+    body = text[text.index("sample_kernel(const SampleArgs"):]
+    touches = re.search(r"in_cta\(|ld_cluster_u32\(|share_bins\(|\.list\(|\.limit\(|fetch_list\(", body).start()
+    assert re.search(r"cluster_wait\(\)|cluster_barrier\(\)", body).start() < touches
+    assert body.index("cluster_arrive()") < touches or body.index("cluster_barrier()") < touches
