@@ -569,7 +569,11 @@ __global__ void __launch_bounds__(AD_THREADS, 2) attn_decode_kernel(const Decode
                             }
                         }
                 }
-                uint32_t pf[NT][2], pr[NT][2];     // pr: what rounding to bf16 leaves
+                // bf16: p as its leading bits and the rest, which gets 2^-23 p on top so that both parts are positive where p is: a visible infinity times
+                // them is infinite (0 x infinity, or infinity - infinity, would be NaN)
+                uint32_t pf[NT][2], pr[NT][2];
+                auto front = [](float x, float y) { return __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632); };
+                auto rest = [](float x) { return fmaf(x, 1.f + 0x1p-23f, -__uint_as_float(__float_as_uint(x) & 0xffff0000u)); };
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float p[4];
@@ -577,12 +581,14 @@ __global__ void __launch_bounds__(AD_THREADS, 2) attn_decode_kernel(const Decode
                     for (int e = 0; e < 4; ++e) p[e] = exp2_approx(st[nt][e] - ref[nt][e & 1]);
                     sum[nt][0] += p[0] + p[2];
                     sum[nt][1] += p[1] + p[3];
-                    const uint32_t w0 = pack2<FP8>(p[0], p[1]), w1 = pack2<FP8>(p[2], p[3]);
-                    pf[nt][0] = transpose8x8(w0);
-                    pf[nt][1] = transpose8x8(w1);
-                    if constexpr (!FP8) {
-                        pr[nt][0] = transpose8x8(pack2<false>(p[0] - __uint_as_float(w0 << 16), p[1] - __uint_as_float(w0 & 0xffff0000u)));
-                        pr[nt][1] = transpose8x8(pack2<false>(p[2] - __uint_as_float(w1 << 16), p[3] - __uint_as_float(w1 & 0xffff0000u)));
+                    if constexpr (FP8) {
+                        pf[nt][0] = transpose8x8(pack2<true>(p[0], p[1]));
+                        pf[nt][1] = transpose8x8(pack2<true>(p[2], p[3]));
+                    } else {
+                        pf[nt][0] = transpose8x8(front(p[0], p[1]));
+                        pf[nt][1] = transpose8x8(front(p[2], p[3]));
+                        pr[nt][0] = transpose8x8(pack2<false>(rest(p[0]), rest(p[1])));
+                        pr[nt][1] = transpose8x8(pack2<false>(rest(p[2]), rest(p[3])));
                     }
                 }
                 // O^T (D x heads) += V^T (D x 16 tokens) P^T

@@ -8,6 +8,8 @@ import types
 import pytest
 import torch
 
+import test_kv_attention as A
+
 gpu = pytest.mark.gpu
 DEV = "cuda"
 
@@ -18,6 +20,19 @@ def hctx():
     block = C.create_string_buffer(64 << 10)
     return types.SimpleNamespace(torch=torch, device=torch.device("cpu"), index=-1, address=C.addressof(block), block=block,
                                  attn_workspace=torch.zeros(16, dtype=torch.uint8))
+
+
+@pytest.fixture(scope="module")
+def ectx(pkg):
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    c = pkg.Ctx(0, pdl=os.environ.get("DSUF_TEST_PDL", "0") == "1")
+    yield c
+    c.close()
+
+
+def i32(*v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
 
 
 def z(*shape, dt=torch.bfloat16):
@@ -85,3 +100,24 @@ def test_no_peer_memory_before_the_cluster_has_started(pkg):
     touches = re.search(r"in_cta\(|ld_cluster_u32\(|share_bins\(|\.list\(|\.limit\(|fetch_list\(", body).start()
     assert re.search(r"cluster_wait\(\)|cluster_barrier\(\)", body).start() < touches
     assert body.index("cluster_arrive()") < touches or body.index("cluster_barrier()") < touches
+
+
+# ------------------------------------------------------------------ values that are not finite
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq,hkv,lens", [(7, 1, [500, 1, 33, 9]), (12, 1, [2600, 70, 17, 5]), (2, 2, [40] * 400)])
+def test_decode_over_infinite_values(pkg, ectx, d, hq, hkv, lens):
+    """A visible infinity makes its column infinite, infinities of both signs or a NaN make it NaN, and no other column changes."""
+    cache, q, table, n = A.decode_inputs(pkg, ectx, 91 + d, lens, hq, hkv, d, 16, False)
+    q = (q * 0.25).contiguous()                # (weights between 2^-20 and 1: none is rounded to nothing)
+    clean = pkg.attn_decode(ectx, cache, q, table, n)
+    place = lambda i, j: (table[i, j // 16].long(), 0, j % 16)   # noqa: E731
+    want = clean.clone().reshape(len(lens), hq, d)
+    heads = hq // hkv
+    for i, j, c, x in ((0, 3, 5, math.inf), (0, 8, 6, -math.inf), (2, 3, 0, -math.inf), (2, 16, 0, -math.inf), (2, 4, d - 1, math.inf), (2, 5, d - 1, -math.inf), (3, 2, 9, math.nan)):
+        cache.v[(*place(i, j), c)] = x
+        want[i, :heads, c] = x if x != -math.inf or c != d - 1 else math.nan
+    out = pkg.attn_decode(ectx, cache, q, table, n).reshape(want.shape)
+    torch.cuda.synchronize()
+    assert ectx.status().code == 0
+    assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(out.nan_to_num(0, 1e38, -1e38), want.nan_to_num(0, 1e38, -1e38))
