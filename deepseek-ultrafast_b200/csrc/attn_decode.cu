@@ -45,7 +45,7 @@ constexpr int AD_PART = 16 * 128;                          // floats of one part
 constexpr int AD_JOIN = 16;                                // partials whose loads are in flight together when a piece is joined
 constexpr int AD_SEGMENT_SHIFT = 2;                        // log2 of the units of a segment when there are few
 constexpr unsigned AD_SOLO_UNITS = 4;                      // a warp per piece: pieces of at most so many units, and one for every CTA that the GPU holds
-constexpr float AD_UNSET = -3e38f;                        // below every finite score
+constexpr float AD_UNSET = -3.4028234663852886e38f;         // no finite score is below it
 constexpr float AD_TRIGGER = 15.f, AD_HEADROOM = 7.f;
 
 struct DecodeArgs {

@@ -33,7 +33,7 @@ namespace dsuf {
 constexpr int KID_PROMPT = 9;
 constexpr int PA_THREADS = 352;
 constexpr int PA_BM = 128;
-constexpr float PA_UNSET = -3e38f;     // below every finite score
+constexpr float PA_UNSET = -3.4028234663852886e38f;     // no finite score is below it
 constexpr float PA_TRIGGER = 16777216.f;
 constexpr float PA_FAR = 268435456.f;   // beyond this a reference's own rounding is an exponent of more than 8
 

@@ -121,3 +121,37 @@ def test_decode_over_infinite_values(pkg, ectx, d, hq, hkv, lens):
     torch.cuda.synchronize()
     assert ectx.status().code == 0
     assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(out.nan_to_num(0, 1e38, -1e38), want.nan_to_num(0, 1e38, -1e38))
+
+
+@gpu
+@pytest.mark.parametrize("fp8", [False, True])
+def test_scores_below_all_others(pkg, ectx, fp8):
+    """Scores that, times log2(e), lie between -3.4e38 and -3e38: equal ones give the plain mean of the visible values, and their own lse."""
+    g = A.gen(62)
+    d, n = 64, 300
+    c = -3.46e36                               # (times 64 columns: -2.21e38, times log2(e): -3.19e38)
+    q = torch.ones(n, 2 * d, dtype=torch.bfloat16, device=DEV)
+    k, v = torch.full((n, d), c, dtype=torch.float32, device=DEV).bfloat16(), A.bf16(g, n, d)
+    score = 64 * float(k[0, 0])
+    assert -3.4e38 < score * math.log2(math.e) < -3e38
+    mean = lambda rows: (rows.mean(0).expand(2, d), rows.abs().mean(0).expand(2, d))   # noqa: E731
+    if not fp8:
+        for window in (0, 50):
+            out, lse = pkg.attn_prompt(ectx, q, k, v, i32(0, n), head_dim=d, scale=1.0, window=window, return_lse=True)
+            for r in (0, 1, 49, 128, 299):
+                want, size = mean(v.double()[max(0, r + 1 - window) if window else 0: r + 1])
+                A.within(out[r].reshape(2, d), want, size, terms=2 ** -8 + 2 ** -12)
+            # three fp32 roundings: of the sum of 64 equal terms, none; of its product with log2(e) and of that with ln(2), and of both constants
+            assert ((lse.double() - score).abs() <= 2 ** -21 * abs(score)).all()
+    scale = torch.tensor([float(k[0, 0]) / -448], device=DEV)
+    cache = pkg.KvCache.empty(ectx, 20, 16, 1, d, fp8, *((scale, scale * 0 + 0.05) if fp8 else ()))
+    pos = torch.arange(n, dtype=torch.int32, device=DEV)
+    table = torch.arange(19, dtype=torch.int32, device=DEV)[None]
+    pkg.kv_append(ectx, cache, k, v, pos, table, seq=torch.zeros_like(pos))
+    seen = A.cache64(cache)[1][:19].transpose(1, 2).reshape(-1, d)[:n]
+    for window in (0, 50):
+        want, size = mean(seen[n - window if window else 0:])
+        out, lse = pkg.attn_decode(ectx, cache, q[:1], table, pos[-1:] + 1, scale=1.0, window=window, return_lse=True)
+        A.within(out.reshape(2, d), want, size, terms=2 ** -8 + 2 ** -12)
+        assert ((lse.double() - score).abs() <= 2 ** -20 * abs(score)).all()
+    assert ectx.status().code == 0
