@@ -48,7 +48,7 @@ struct PromptShape {
 
 struct PromptArgs {
     CUtensorMap tm_q, tm_k, tm_v;
-    const bf16 *q, *k, *v;          // the same rows, for the seldom path of prompt_repair
+    const bf16 *q, *k, *v;          // the same rows, for prompt_repair, which is seldom needed
     int ldq, ldk, ldv;
     bf16* out;
     float* lse;
@@ -250,56 +250,141 @@ DSUF_DEV float pa_weights(uint32_t tS, float sl2, float ref, int upper, int lowe
     return pa_total(sum2);
 }
 
-// In the tiles that the diagonal or the window cuts, the tensor core multiplies hidden values with p = 0, and 0 x infinity is NaN.  A warp that finds
-// rows (bits of `rows`, the first at sequence row row0) with an output that is not finite comes here: where a hidden value of those tiles is not finite in
-// a column and no visible one of them is, the row is computed again from its visible rows alone, one key at a time.
+// Which of 32 consecutive bf16 at `p` (16-byte aligned) are not finite, and which are NaN, a bit for each.
+DSUF_DEV void pa_odd32(const bf16* p, uint32_t& odd, uint32_t& nan) {
+    odd = nan = 0;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+        const uint4 x = reinterpret_cast<const uint4*>(p)[v];
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t m = (w[e / 2] >> (16 * (e & 1))) & 0x7fffu;
+            odd |= (m >= 0x7f80u ? 1u : 0u) << (v * 8 + e);
+            nan |= (m > 0x7f80u ? 1u : 0u) << (v * 8 + e);
+        }
+    }
+}
+
+DSUF_DEV void pa_mma_sync(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// In the tiles that the diagonal or the window cuts, the tensor core multiplies hidden values with p = 0, and 0 x infinity is NaN.  A softmax warp that
+// has met outputs that are not finite comes here when the CTA is done otherwise (nobody waits for it then, however long its rows are), walks its tiles
+// again, and where an output is NaN, a value of its column that is hidden from the row is not finite in those tiles, and no visible one there is NaN, the
+// output is computed again from the row's visible keys alone: a row per lane and 32 columns at a time (8192 tokens, 56 / 8 heads of 128, one NaN in the
+// last tile: 2.0 ms more; a row of NaN in every head: 7.8).
+constexpr int PA_KEYS = 16;
+constexpr int PA_REPAIR = 32 * (PA_KEYS + 1) * 4 + PA_KEYS * 32 * 4;     // bytes of shared memory of a warp: scores and values
 template <int D>
-__device__ __noinline__ void prompt_repair(const PromptArgs& a, unsigned rows, int row0, int start, int len, int head, int kvh, int lo) {
-    constexpr int V = D / 32;                        // columns of a lane
-    const int lane = threadIdx.x & 31;
-    const bf16* kb = a.k + (size_t)start * a.ldk + (size_t)kvh * D + lane * V;
-    const bf16* vb = a.v + (size_t)start * a.ldv + (size_t)kvh * D + lane * V;
-    for (; rows; rows &= rows - 1) {
-        const int i = row0 + __ffs(rows) - 1;
-        if (i >= len) continue;
+__device__ __noinline__ void prompt_repair(const PromptArgs& a) {
+    extern __shared__ uint8_t smem_raw[];      // (its address and the tile worked out here: as arguments they cost the caller registers, and 2 % of its time)
+    const int t = threadIdx.x >> 7;
+    float* scores = reinterpret_cast<float*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u) + (threadIdx.x >> 5) * PA_REPAIR);
+    static_assert(PA_REPAIR % 16 == 0 && (32 * (PA_KEYS + 1) * 4) % 16 == 0 && 8 * PA_REPAIR <= PromptShape<D>::SMEM - 1024, "scores and values fit");
+    float* values = scores + 32 * (PA_KEYS + 1);
+    const int lane = threadIdx.x & 31, first = ((threadIdx.x >> 5) & 3) * 32;
+    PromptWalk walk(a);
+    for (;;) {
+        const PromptPair p = walk.next();
+        if (!p.ok) break;
+        const PromptTile q = p.tile(t);
+        const int tile0 = q.qb * PA_BM, row0 = tile0 + first, i = row0 + lane;
+        if (q.hi == 0 || row0 >= p.len) continue;
+        const bool live = i < p.len;
         const int from = a.window > 0 ? max(0, i - a.window + 1) : 0;
-        bf16* out = a.out + (size_t)(start + i) * a.ldo + (size_t)head * D + lane * V;
-        bool hidden[V], seen[V], wrong = false;
-#pragma unroll
-        for (int e = 0; e < V; ++e) hidden[e] = seen[e] = false;
-        const int tile0 = i / PA_BM * PA_BM;
-        for (int j = lo * PA_BM; j < min(len, tile0 + PA_BM); ++j) {
-            if (j == max(lo * PA_BM, (from / PA_BM + 1) * PA_BM) && j < tile0) j = tile0;      // (uncut tiles hide nothing)
-            const bool sees = j >= from && j <= i;
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float x = __bfloat162float(vb[(size_t)j * a.ldv + e]);
-                if (!(fabsf(x) < INFINITY)) (sees ? seen[e] : hidden[e]) = true;
+        const int end = min(p.len, tile0 + PA_BM);                                    // of the diagonal tile
+        const int lower = a.window > 0 ? min(tile0, row0 + 32 - a.window) : 0;        // of the keys that the window hides from one of the rows
+        bf16* out = a.out + (size_t)(p.start + (live ? i : row0)) * a.ldo + (size_t)q.head * D;
+        const bf16* kb = a.k + (size_t)p.start * a.ldk + (size_t)p.kvh * D;
+        const bf16* vb = a.v + (size_t)p.start * a.ldv + (size_t)p.kvh * D;
+        for (int c = 0; c < D; c += 32) {
+            uint32_t nan, hidden = 0, seen = 0;
+            pa_odd32(out + c, hidden, nan);
+            if (!live) nan = 0;
+            if (!__any_sync(0xffffffffu, nan != 0)) continue;
+            hidden = 0;
+            for (int j0 = q.lo * PA_BM; j0 < end; j0 += 32) {
+                if (j0 >= lower && j0 < tile0) j0 = tile0;                            // (uncut tiles hide nothing)
+                uint32_t odd_here = 0, nan_here = 0;
+                if (j0 + lane < end) pa_odd32(vb + (size_t)(j0 + lane) * a.ldv + c, odd_here, nan_here);
+                if (!__any_sync(0xffffffffu, odd_here != 0)) continue;
+                for (int m = 0; m < 32; ++m) {
+                    const uint32_t o = __shfl_sync(0xffffffffu, odd_here, m), n = __shfl_sync(0xffffffffu, nan_here, m);
+                    if (j0 + m >= from && j0 + m <= i) seen |= n;
+                    else hidden |= o;
+                }
             }
+            const uint32_t wrong = nan & hidden & ~seen;
+            if (!__any_sync(0xffffffffu, wrong != 0)) continue;
+            // scores of 32 rows and 16 keys by mma.sync, through shared memory to a row per lane.  Its sums over the head's columns may take these in any order:
+            // of each 32 a lane has 8 beside each other, as the operands of two steps.
+            uint4 qf[4][D / 32];                     // rows lane / 4 + 8 r
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int v = 0; v < D / 32; ++v)
+                    qf[r][v] = reinterpret_cast<const uint4*>(a.q + (size_t)(p.start + min(row0 + r * 8 + lane / 4, p.len - 1)) * a.ldq + (size_t)q.head * D)[v * 4 + lane % 4];
+            float o[32], top = PA_UNSET, sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0.f;
+            const int j_from = __reduce_min_sync(0xffffffffu, wrong ? from : 0x7fffffff), j_to = __reduce_max_sync(0xffffffffu, wrong ? i : -1);
+            for (int j0 = j_from; j0 <= j_to; j0 += PA_KEYS) {
+                uint4 y[PA_KEYS / 8];
+#pragma unroll
+                for (int v = 0; v < PA_KEYS / 8; ++v) y[v] = __ldg(reinterpret_cast<const uint4*>(vb + (size_t)min(j0 + v * 8 + lane / 4, j_to) * a.ldv + c) + lane % 4);
+                __syncwarp();                        // (the last scores and values have been read)
+#pragma unroll
+                for (int n = 0; n < PA_KEYS / 8; ++n) {
+                    const uint4* kr = reinterpret_cast<const uint4*>(kb + (size_t)min(j0 + n * 8 + lane / 4, j_to) * a.ldk) + lane % 4;
+                    float s[2][4] = {};
+#pragma unroll
+                    for (int v = 0; v < D / 32; ++v) {
+                        const uint4 x = __ldg(kr + v * 4);
+#pragma unroll
+                        for (int m = 0; m < 2; ++m) {
+                            pa_mma_sync(s[m], qf[2 * m][v].x, qf[2 * m + 1][v].x, qf[2 * m][v].y, qf[2 * m + 1][v].y, x.x, x.y);
+                            pa_mma_sync(s[m], qf[2 * m][v].z, qf[2 * m + 1][v].z, qf[2 * m][v].w, qf[2 * m + 1][v].w, x.z, x.w);
+                        }
+                    }
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) scores[(m * 16 + (e >> 1) * 8 + lane / 4) * (PA_KEYS + 1) + n * 8 + lane % 4 * 2 + (e & 1)] = s[m][e];
+                }
+#pragma unroll
+                for (int v = 0; v < PA_KEYS / 8; ++v) {
+                    const uint32_t w[4] = {y[v].x, y[v].y, y[v].z, y[v].w};
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2)
+                        *reinterpret_cast<float4*>(values + (v * 32 + lane) * 8 + 2 * e) = make_float4(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u),
+                                                                                                   __uint_as_float(w[e + 1] << 16), __uint_as_float(w[e + 1] & 0xffff0000u));
+                }
+                __syncwarp();
+#pragma unroll 4
+                for (int m = 0; m < PA_KEYS; ++m) {
+                    const float s = scores[lane * (PA_KEYS + 1) + m] * a.scale_log2;
+                    if (!wrong || j0 + m < from || j0 + m > i) continue;
+                    if (s > top) {
+                        const float by = pa_exp2(top - s);
+                        top = s;
+                        sum *= by;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] *= by;
+                    }
+                    const float w = pa_exp2(s - top);
+                    sum += w;
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = fmaf(w, values[m * 32 + e], o[e]);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+                if ((wrong >> e) & 1) out[c + e] = __float2bfloat16(sum == 0.f ? 0.f : o[e] / sum);
         }
-#pragma unroll
-        for (int e = 0; e < V; ++e) wrong |= hidden[e] && !seen[e] && !(fabsf(__bfloat162float(out[e])) < INFINITY);
-        if (!__any_sync(0xffffffffu, wrong)) continue;
-        float q[V], o[V], top = PA_UNSET, sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            q[e] = __bfloat162float(a.q[(size_t)(start + i) * a.ldq + (size_t)head * D + lane * V + e]) * a.scale_log2;
-            o[e] = 0.f;
-        }
-        for (int j = from; j <= i; ++j) {
-            float s = 0.f;
-#pragma unroll
-            for (int e = 0; e < V; ++e) s += q[e] * __bfloat162float(kb[(size_t)j * a.ldk + e]);
-#pragma unroll
-            for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-            const float to = fmaxf(top, s), by = pa_exp2(top - to), w = pa_exp2(s - to);
-            top = to;
-            sum = sum * by + w;
-#pragma unroll
-            for (int e = 0; e < V; ++e) o[e] = o[e] * by + w * __bfloat162float(vb[(size_t)j * a.ldv + e]);
-        }
-#pragma unroll
-        for (int e = 0; e < V; ++e) out[e] = __float2bfloat16(sum == 0.f ? 0.f : o[e] / sum);
     }
 }
 
@@ -313,6 +398,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
     uint8_t* ring = base + 2 * S::TILE;
     __shared__ __align__(8) uint64_t q_full[2], q_empty[2], kv_full[S::STAGES], kv_empty[S::STAGES], s_full[2], p_full[2], o_full[2];
     __shared__ uint32_t s_tmem;
+    __shared__ int s_odd[8];         // softmax warps that have met outputs which are not finite
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     bool dead = false;
 
@@ -320,6 +406,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
         tmem_alloc(&s_tmem, 512);
         tmem_relinquish();
     }
+    if (tid < 8) s_odd[tid] = 0;
     if (tid == 0) {
         for (int t = 0; t < 2; ++t) {
             mbar_init(&q_full[t], 1);
@@ -618,8 +705,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
                 }
                 __syncwarp();
             }
-            const unsigned again = __ballot_sync(0xffffffffu, live && !(pa_total(odd) == 0.f));
-            if (again) prompt_repair<D>(a, again, row0, p.start, p.len, q.head, p.kvh, q.lo);
+            if (live && !(pa_total(odd) == 0.f)) s_odd[warp] = 1;
             if (live && a.lse) a.lse[(size_t)(p.start + row) * a.q_heads + q.head] = sum == 0.f ? -INFINITY : (ref + log2f(sum)) * 0.6931471805599453f;
             tc_fence_before();
         }
@@ -628,6 +714,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
     __syncthreads();
     tc_fence_after();
     if (warp == 8) tmem_dealloc(tm, 512);
+    if (warp < 8 && s_odd[warp]) prompt_repair<D>(a);
 }
 
 static int encode_heads(dsuf_ctx* ctx, CUtensorMap* tm, const void* base, long long width, long long ld, long long rows) {

@@ -155,3 +155,66 @@ def test_scores_below_all_others(pkg, ectx, fp8):
         A.within(out.reshape(2, d), want, size, terms=2 ** -8 + 2 ** -12)
         assert ((lse.double() - score).abs() <= 2 ** -20 * abs(score)).all()
     assert ectx.status().code == 0
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("window", [0, 3000])
+def test_hidden_values_in_a_long_prompt(pkg, ectx, d, window):
+    """Values that are not finite near a long prompt's end: the rows of their tile that do not see them are computed from what they see, every other output keeps
+    its bits."""
+    n, hq, hkv = 20000, 4, 2
+    g = A.gen(131)
+    q, k, v = A.bf16(g, n, hq * d), A.bf16(g, n, hkv * d), A.bf16(g, n, hkv * d)
+    cu = i32(0, n)
+    clean = pkg.attn_prompt(ectx, q, k, v, cu, head_dim=d, window=window).reshape(n, hq, d)
+    bad = v.clone()
+    where = [(19990, 0, 3, math.nan), (19990, 1, d - 1, math.inf), (19969, 1, 0, -math.inf), (10000, 1, 40, math.nan)]         # the last tile begins at 19968
+    want = clean.clone()
+    by_other_means = torch.zeros(n, hq, d, dtype=torch.bool, device=DEV)
+    for r, h, c, x in where:
+        bad[r, h * d + c] = x
+        last = min(n, r + window) if window else n
+        heads = slice(2 * h, 2 * h + 2)
+        want[r:last, heads, c] = x
+        by_other_means[r // 128 * 128: r, heads, c] = True
+        if window and last < n:      # (up to the last tile of rows whose first row still sees a key of this key's tile, and so meets the whole tile)
+            by_other_means[last: ((r // 128 * 128 + 127 + window - 1) // 128 + 1) * 128, heads, c] = True
+    out = pkg.attn_prompt(ectx, q, k, bad, cu, head_dim=d, window=window).reshape(n, hq, d)
+    torch.cuda.synchronize()
+    assert ectx.status().code == 0
+    same = lambda x: torch.where(by_other_means, torch.zeros_like(x), x).nan_to_num(7e30, 8e30, 9e30)   # noqa: E731
+    assert torch.equal(same(out), same(want))
+    for r in sorted(set(by_other_means.any(2).any(1).nonzero().flatten().tolist())):
+        lo = max(0, r + 1 - window) if window else 0
+        for h in range(hq):
+            cols = by_other_means[r, h].nonzero().flatten()
+            if len(cols) == 0:
+                continue
+            kk, vv = (x[lo: r + 1].double().reshape(-1, hkv, d)[:, h // 2] for x in (k, v))
+            p = torch.softmax(kk @ q[r].double().reshape(hq, d)[h] * d ** -0.5, 0)
+            A.within(out[r, h, cols], (p @ vv)[cols], (p @ vv.abs())[cols], terms=2 ** -8 + 2 ** -12)
+
+
+@gpu
+@pytest.mark.parametrize("window", [0, 70])
+def test_hidden_nan_beside_a_visible_infinity(pkg, ectx, window):
+    """The rows that see the infinity and not the NaN in the same column have an infinity there."""
+    d, n = 64, 300
+    g = A.gen(132)
+    q, k, v = A.bf16(g, n, 2 * d), A.bf16(g, n, d), A.bf16(g, n, d)
+    for r, c, x in ((130, 5, math.inf), (200, 5, math.nan), (129, 6, -math.inf), (250, 6, math.inf), (10, 7, math.inf), (40, 7, math.nan)):
+        v[r, c] = x
+    out = pkg.attn_prompt(ectx, q, k, v, i32(0, n), head_dim=d, window=window).reshape(n, 2, d)
+    for c in (5, 6, 7):
+        for r in range(n):
+            seen = v[max(0, r + 1 - window) if window else 0: r + 1, c].float()
+            odd = seen[~torch.isfinite(seen)].tolist()
+            for x in out[r, :, c].tolist():
+                if not odd:
+                    assert math.isfinite(x), (r, c, x)
+                elif len(set(odd)) > 1 or math.isnan(odd[0]):
+                    assert math.isnan(x), (r, c, x)
+                else:
+                    assert x == odd[0], (r, c, x)
+    assert ectx.status().code == 0
