@@ -728,14 +728,6 @@ static int encode_heads(dsuf_ctx* ctx, CUtensorMap* tm, const void* base, long l
     return DSUF_OK;
 }
 
-// Whether t rows of `wo` bf16 columns at `out` share memory with t rows of `w` columns at `x`.  Parts of the columns of the same rows do not.
-static bool rows_overlap(uint64_t out, long long ldo, long long wo, uint64_t x, long long ld, long long w, long long t) {
-    if (out >= x + 2 * ((t - 1) * ld + w) || x >= out + 2 * ((t - 1) * ldo + wo)) return false;
-    if (ldo != ld) return true;
-    const long long apart = (((long long)(out - x) / 2) % ld + ld) % ld;
-    return apart < w || apart + wo > ld;
-}
-
 template <int D, bool WINDOW>
 static cudaError_t prompt_attr() { return cudaFuncSetAttribute(attn_prompt_kernel<D, WINDOW>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<D>::SMEM); }
 int attn_prompt_setup(dsuf_ctx* ctx) {

@@ -111,6 +111,17 @@ int launch(dsuf_ctx* ctx, cudaStream_t stream, void (*kernel)(KArgs...), dim3 gr
     return launch_cluster(ctx, stream, kernel, grid, block, smem, 1, std::forward<Args>(args)...);
 }
 
+// Whether t rows of `wo` bf16 columns at `out` share memory with t rows of `w` columns at `x`.  Parts of the columns of the same rows do not.
+inline bool rows_overlap(uint64_t out, long long ldo, long long wo, uint64_t x, long long ld, long long w, long long t) {
+    if (out >= x + 2 * ((t - 1) * ld + w) || x >= out + 2 * ((t - 1) * ldo + wo)) return false;
+    if (ldo != ld) return true;
+    const long long apart = (((long long)(out - x) / 2) % ld + ld) % ld;
+    return apart < w || apart + wo > ld;
+}
+
+// The same rows written in place: each element is read by the thread that writes it, or before it is written.
+inline bool rows_in_place(uint64_t out, long long ldo, uint64_t x, long long ld, long long t) { return out == x && (ldo == ld || t == 1); }
+
 // per-file launchers
 int launch_act_quant(dsuf_ctx* ctx, cudaStream_t stream, int mode, const void* x, int ldx, int rows_in, int k, void* q,
                      void* scales, const int* pair_row, int fanout, const void* norm_w = nullptr,

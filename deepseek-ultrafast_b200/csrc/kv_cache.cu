@@ -206,6 +206,13 @@ extern "C" int32_t dsuf_kv_append(dsuf_ctx* ctx, void* stream, const dsuf_kv_cac
     DSUF_REQUIRE(ctx, k && v && pos && block_table && (k & 15) == 0 && (v & 15) == 0 && (pos & 3) == 0 && (seq & 3) == 0 && (block_table & 3) == 0,
                  "kv_append: null or misaligned pointer (k, v 16 bytes, indexes 4)");
     DSUF_REQUIRE(ctx, !q_heads || (q && q_out && (q & 15) == 0 && (q_out & 15) == 0), "kv_append: q and q_out must be 16-byte aligned");
+    const long long wq = (long long)q_heads * D, wk = (long long)cache->kv_heads * D;
+    DSUF_REQUIRE(ctx, !q_heads || ((rows_in_place(q_out, ldqo, q, ldq, t) || !rows_overlap(q_out, ldqo, wq, q, ldq, wq, t)) &&
+                 !rows_overlap(q_out, ldqo, wq, k, ldk, wk, t) && !rows_overlap(q_out, ldqo, wq, v, ldv, wk, t)),
+                 "kv_append: q_out must be q itself, row for row, or share no memory with q, k and v");
+    DSUF_REQUIRE(ctx, !k_out || ((rows_in_place(k_out, ldko, k, ldk, t) || !rows_overlap(k_out, ldko, wk, k, ldk, wk, t)) && !rows_overlap(k_out, ldko, wk, v, ldv, wk, t) &&
+                 (!q_heads || (!rows_overlap(k_out, ldko, wk, q, ldq, wq, t) && !rows_overlap(k_out, ldko, wk, q_out, ldqo, wq, t)))),
+                 "kv_append: k_out must be k itself, row for row, or share no memory with k, v, q and q_out");
     DSUF_REQUIRE_DEVICE(ctx, "kv_append");
     AppendArgs a;
     memset(&a, 0, sizeof(a));

@@ -417,8 +417,9 @@ typedef struct {
     int32_t positions, rot, off, half;
 } dsuf_rope;
 /* Writes t tokens' keys (rotated to their positions when rope is given) and values into the cache and, with q_heads > 0, the
- * rotated queries to q_out (q_out = q: in place).  k_out (or 0) receives the rotated keys as bf16 rows, for dsuf_attn_prompt over the same
- * tokens (k_out = k: in place).  k, v bf16 [t][kv_heads * head_dim] (row strides ldk, ldv), q / q_out bf16
+ * rotated queries to q_out (q_out = q with ldqo = ldq: in place).  k_out (or 0) receives the rotated keys as bf16 rows, for dsuf_attn_prompt over
+ * the same tokens (k_out = k with ldko = ldk: in place).  Otherwise q_out and k_out share no memory with q, k, v or each other (columns of their own
+ * in the same rows are no sharing).  k, v bf16 [t][kv_heads * head_dim] (row strides ldk, ldv), q / q_out bf16
  * [t][q_heads * head_dim]; pos i32 [t], seq i32 [t] (0: token i belongs to sequence i, t <= n_seqs).  A token with a negative
  * pos or seq is padding: nothing of it is written.  The (seq, pos) pairs of one call must be distinct, and distinct sequences must not
  * share the pages that are written: which of two writes to one slot lands is undefined. */

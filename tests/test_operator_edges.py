@@ -218,3 +218,41 @@ def test_hidden_nan_beside_a_visible_infinity(pkg, ectx, window):
                 else:
                     assert x == odd[0], (r, c, x)
     assert ectx.status().code == 0
+
+
+# ------------------------------------------------------------------ outputs that lie in inputs
+P = 1 << 24          # an aligned address that nothing follows
+
+
+def shares(pkg, block, rc):
+    text = C.create_string_buffer(512)
+    pkg.lib().dsuf_last_error(block, text, 512)
+    assert rc != 0           # (the calls that pass the check end at the next one: the stand-in's device is never the current one)
+    return b"share no memory" in text.value
+
+
+@pytest.fixture()
+def cblock():
+    block = C.create_string_buffer(64 << 10)
+    C.c_int.from_buffer(block).value = 1 << 20
+    return block
+
+
+ROW = 4 * 128 + 2 * 128 + 2 * 128        # q, k and v of a token beside each other
+
+
+def test_append_refuses_outputs_in_its_inputs(pkg, cblock):
+    cache = pkg.KvCacheStruct(P >> 4, P >> 4, 0, 0, 2 * 16 * 128, 0, 4, 16, 2, 128)
+
+    def refused(t=9, q=P, k=P + 1024, v=P + 1536, ld=ROW, q_out=P + (1 << 20), ldqo=512, k_out=0, ldko=0):
+        return shares(pkg, cblock, pkg.lib().dsuf_kv_append(cblock, None, C.byref(cache), k, ld, v, ld, t, P - 4096, P - 4096, P - 4096, 2, 4, None, q, ld, 4, q_out, ldqo,
+                                                           k_out, ldko))
+    for kw in [dict(q_out=P + 16, ldqo=ROW), dict(q_out=P, ldqo=512), dict(q_out=P + 2 * ROW, ldqo=ROW), dict(q_out=P + 1024, ldqo=ROW), dict(q_out=P + 1536, ldqo=ROW),
+               dict(q_out=P - 1008, ldqo=512, t=1), dict(q_out=P + 1024 * 4, ldqo=520),
+               dict(k_out=P + 1024 + 16, ldko=ROW), dict(k_out=P + 1024, ldko=256), dict(k_out=P + 1536, ldko=ROW), dict(k_out=P, ldko=ROW), dict(k_out=P + 1024 + 2 * ROW, ldko=ROW),
+               dict(k_out=P + (1 << 20), ldko=256), dict(k_out=P + (1 << 20) + 512, ldko=512)]:
+        assert refused(**kw), kw
+    for kw in [{}, dict(q_out=P, ldqo=ROW), dict(q_out=P, ldqo=512, t=1), dict(k_out=P + 1024, ldko=ROW), dict(k_out=P + 1024, ldko=256, t=1), dict(q_out=P, ldqo=ROW, k_out=P + 1024, ldko=ROW),
+               dict(k_out=P + (2 << 20), ldko=256), dict(q_out=P + 2 * 9 * ROW, ldqo=512), dict(q_out=P - 2 * 9 * 512, ldqo=512),
+               dict(q=P, k=P + 1024, v=P + 1536, ld=2 * ROW, q_out=P + 2 * ROW, ldqo=2 * ROW)]:
+        assert not refused(**kw), kw
