@@ -811,6 +811,10 @@ int32_t dsuf_attn_decode(dsuf_ctx* ctx, void* stream, const dsuf_kv_cache* cache
     if (b == 0) return DSUF_OK;
     DSUF_REQUIRE(ctx, q && out && block_table && seq_lens && workspace && (q & 15) == 0 && (out & 15) == 0 && (block_table & 3) == 0 &&
                  (seq_lens & 3) == 0 && (lse & 3) == 0 && (workspace & 15) == 0, "attn_decode: null or misaligned pointer (q, out, workspace 16 bytes, indexes and lse 4)");
+    const long long width = (long long)q_heads * D, lse_bytes = 4ll * b * q_heads;
+    DSUF_REQUIRE(ctx, rows_in_place(out, ldo, q, ldq, b) || !rows_overlap(out, ldo, width, q, ldq, width, b), "attn_decode: out must be q itself, row for row, or share no memory with it");
+    DSUF_REQUIRE(ctx, !lse || (!block_meets_rows(lse, lse_bytes, q, ldq, width, b) && !block_meets_rows(lse, lse_bytes, out, ldo, width, b)),
+                 "attn_decode: lse must share no memory with q and out");
     DecodeArgs a;
     memset(&a, 0, sizeof(a));
     a.q = (const bf16*)q; a.out = (bf16*)out; a.lse = (float*)lse;

@@ -759,6 +759,10 @@ extern "C" int32_t dsuf_attn_prompt(dsuf_ctx* ctx, void* stream, uint64_t q, int
     const long long wq = (long long)q_heads * head_dim, wk = (long long)kv_heads * head_dim;
     DSUF_REQUIRE(ctx, !rows_overlap(out, ldo, wq, q, ldq, wq, t) && !rows_overlap(out, ldo, wq, k, ldk, wk, t) && !rows_overlap(out, ldo, wq, v, ldv, wk, t),
                  "attn_prompt: out must not share memory with q, k or v");
+    const long long lse_bytes = 4ll * t * q_heads;
+    DSUF_REQUIRE(ctx, !lse || (!block_meets_rows(lse, lse_bytes, q, ldq, wq, t) && !block_meets_rows(lse, lse_bytes, k, ldk, wk, t) &&
+                 !block_meets_rows(lse, lse_bytes, v, ldv, wk, t) && !block_meets_rows(lse, lse_bytes, out, ldo, wq, t)),
+                 "attn_prompt: lse must share no memory with q, k, v and out");
     DSUF_REQUIRE_DEVICE(ctx, "attn_prompt");
     PromptArgs a;
     memset(&a, 0, sizeof(a));

@@ -119,6 +119,12 @@ inline bool rows_overlap(uint64_t out, long long ldo, long long wo, uint64_t x, 
     return apart < w || apart + wo > ld;
 }
 
+// Whether `bytes` at `block` meet one of t rows of `w` bf16 columns at `x`.
+inline bool block_meets_rows(uint64_t block, long long bytes, uint64_t x, long long ld, long long w, long long t) {
+    const long long r = block < x + 2 * w ? 0 : (long long)(block - x - 2 * w) / (2 * ld) + 1;      // the first row that ends behind the block's begin
+    return r < t && x + 2 * ld * r < block + bytes;
+}
+
 // The same rows written in place: each element is read by the thread that writes it, or before it is written.
 inline bool rows_in_place(uint64_t out, long long ldo, uint64_t x, long long ld, long long t) { return out == x && (ldo == ld || t == 1); }
 

@@ -429,7 +429,8 @@ int32_t dsuf_kv_append(dsuf_ctx* ctx, void* stream, const dsuf_kv_cache* cache, 
 /* Attention of one new token per sequence over the cache: out[b][h] = sum_j softmax_j(scale * <q[b][h], K_j>) V_j over positions
  * j in [max(0, len - window), len) (window 0: all), kv head = h / (q_heads / kv_heads).  The new token's own key is in the cache
  * already (dsuf_kv_append); seq_lens i32 [b] counts it.  A sequence of length <= 0 gives zeros and lse -inf.
- * q / out bf16 [b][q_heads * head_dim] (out = q with ldo = ldq: in place); lse f32 [b][q_heads] = log of the sum of exp(scale * <q, k>), or 0.
+ * q / out bf16 [b][q_heads * head_dim] (out = q with ldo = ldq: in place; otherwise they share no memory); lse f32 [b][q_heads] = log of the sum of
+ * exp(scale * <q, k>), in memory of its own, or 0.
  * q_heads a multiple of kv_heads.  workspace: dsuf_attn_workspace_bytes(ctx), zeroed once by dsuf_attn_workspace_init; the kernel
  * leaves its counters zeroed.  Calls (and captured graphs) that share one workspace must be stream-ordered. */
 size_t dsuf_attn_workspace_bytes(dsuf_ctx* ctx);
@@ -440,7 +441,7 @@ int32_t dsuf_attn_decode(dsuf_ctx* ctx, void* stream, const dsuf_kv_cache* cache
 /* Causal attention over packed prompts: rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1 (i32 [n_seqs + 1], device, ascending, at most t)
  * of q, k, v, out are sequence i; row r of a sequence sees its rows max(0, r - window + 1) .. r (window 0: all up to r).
  * q / out bf16 [t][q_heads * head_dim], k / v bf16 [t][kv_heads * head_dim] (row strides ld*, so the parts of one merged projection can be
- * passed as they lie), lse f32 [t][q_heads] or 0.  out shares no memory with q, k or v (columns of its own in their rows are no sharing).  Rows that belong to no sequence are left as they were, and nothing of them is
+ * passed as they lie), lse f32 [t][q_heads] in memory of its own, or 0.  out shares no memory with q, k or v (columns of its own in their rows are no sharing).  Rows that belong to no sequence are left as they were, and nothing of them is
  * read into a result; an infinity or NaN inside a sequence reaches the rows that see it, no others.  q_heads a multiple of kv_heads, head_dim 64 or 128. */
 int32_t dsuf_attn_prompt(dsuf_ctx* ctx, void* stream, uint64_t q, int32_t ldq, uint64_t k, int32_t ldk, uint64_t v, int32_t ldv, int32_t t,
                          int32_t q_heads, int32_t kv_heads, int32_t head_dim, uint64_t cu_seqlens, int32_t n_seqs, float scale,

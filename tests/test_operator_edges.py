@@ -256,3 +256,25 @@ def test_append_refuses_outputs_in_its_inputs(pkg, cblock):
                dict(k_out=P + (2 << 20), ldko=256), dict(q_out=P + 2 * 9 * ROW, ldqo=512), dict(q_out=P - 2 * 9 * 512, ldqo=512),
                dict(q=P, k=P + 1024, v=P + 1536, ld=2 * ROW, q_out=P + 2 * ROW, ldqo=2 * ROW)]:
         assert not refused(**kw), kw
+
+
+def test_decode_refuses_outputs_in_its_inputs(pkg, cblock):
+    cache = pkg.KvCacheStruct(P >> 4, P >> 4, 0, 0, 2 * 16 * 128, 0, 4, 16, 2, 128)
+
+    def refused(b=9, q=P, ldq=512, out=P + (1 << 20), ldo=512, lse=0):
+        return shares(pkg, cblock, pkg.lib().dsuf_attn_decode(cblock, None, C.byref(cache), q, ldq, 4, b, P - 4096, 4, P - 4096, 0.1, 0, out, ldo, lse, P + (1 << 22)))
+    for kw in [dict(out=P + 16), dict(out=P + 1024), dict(out=P, ldo=520), dict(out=P - 1008), dict(out=P + 1008, b=1), dict(out=P, ldq=1024), dict(ldq=1024, ldo=1024, out=P + 1008),
+               dict(lse=P), dict(lse=P + 9 * 1024 - 4), dict(lse=P - 9 * 16 + 4), dict(lse=P + (1 << 20) + 1024), dict(lse=P + 1040, ldq=1024, ldo=1024, out=P + 1024)]:
+        assert refused(**kw), kw
+    for kw in [{}, dict(out=P), dict(out=P, b=1, ldo=520), dict(out=P + 9 * 1024), dict(out=P - 9 * 1024), dict(ldq=1024, ldo=1024, out=P + 1024), dict(lse=P + 9 * 1024),
+               dict(lse=P - 9 * 16), dict(lse=P + 1024, ldq=1024, b=1), dict(lse=P + 1024, ldq=1024)]:
+        assert not refused(**kw), kw
+
+
+def test_prompt_refuses_an_lse_in_its_inputs(pkg, cblock):
+    def refused(t=9, ld=ROW, out=P + (1 << 20), ldo=512, lse=0):
+        return shares(pkg, cblock, pkg.lib().dsuf_attn_prompt(cblock, None, P, ld, P + 1024, ld, P + 1536, ld, t, 4, 2, 128, P - 4096, 1, 0.1, 0, out, ldo, lse))
+    for kw in [dict(lse=P), dict(lse=P + 1024), dict(lse=P + 1536 + 4), dict(lse=P + 9 * 2 * ROW - 4), dict(lse=P - 9 * 16 + 4), dict(lse=P + (1 << 20)), dict(lse=P + (1 << 20) + 9 * 1024 - 4)]:
+        assert refused(**kw), kw
+    for kw in [{}, dict(lse=P + 9 * 2 * ROW), dict(lse=P - 9 * 16), dict(lse=P + (1 << 20) + 9 * 1024), dict(ld=2 * ROW, lse=P + 2 * ROW)]:
+        assert not refused(**kw), kw
