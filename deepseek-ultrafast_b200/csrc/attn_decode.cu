@@ -789,6 +789,7 @@ int32_t dsuf_attn_workspace_init(dsuf_ctx* ctx, void* stream, uint64_t workspace
     if (!ctx) return DSUF_E_BADARG;
     DSUF_REQUIRE(ctx, workspace && (workspace & 15) == 0 && bytes >= dsuf_attn_workspace_bytes(ctx), "attn_workspace_init: need %zu bytes, 16-byte aligned",
                  dsuf_attn_workspace_bytes(ctx));
+    DSUF_REQUIRE_DEVICE(ctx, "attn_workspace_init");
     cudaError_t e = cudaMemsetAsync((void*)workspace, 0, dsuf_attn_workspace_bytes(ctx), (cudaStream_t)stream);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "cudaMemsetAsync(attention workspace)");
     return DSUF_OK;

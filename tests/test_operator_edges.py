@@ -278,3 +278,13 @@ def test_prompt_refuses_an_lse_in_its_inputs(pkg, cblock):
         assert refused(**kw), kw
     for kw in [{}, dict(lse=P + 9 * 2 * ROW), dict(lse=P - 9 * 16), dict(lse=P + (1 << 20) + 9 * 1024), dict(ld=2 * ROW, lse=P + 2 * ROW)]:
         assert not refused(**kw), kw
+
+
+# ------------------------------------------------------------------ the workspace
+def test_workspace_init_refuses_another_current_device(pkg, cblock):
+    """The stand-in's device is never the current one.  (Its zeroed number of SMs asks for no bytes, so a memset that is let through does nothing.)"""
+    assert pkg.lib().dsuf_attn_workspace_bytes(cblock) == 0
+    assert pkg.lib().dsuf_attn_workspace_init(cblock, None, P, 0) != 0
+    text = C.create_string_buffer(512)
+    pkg.lib().dsuf_last_error(cblock, text, 512)
+    assert text.value.startswith(b"attn_workspace_init"), text.value
