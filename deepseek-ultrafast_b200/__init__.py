@@ -335,13 +335,15 @@ class Ctx:
         self.sm_count = lib().dsuf_sm_count(self.h)
 
     def new_attn_workspace(self):
-        """A workspace for attn_decode, ready for use: calls and captured graphs that may run at the same time need one each."""
+        """A workspace for attn_decode, ready for use on any stream: calls and captured graphs that may run at the same time need one each.  Not
+        under stream capture, which would only record its zeroing."""
         t = self.torch
+        if t.cuda.is_current_stream_capturing():
+            raise DsufError(-1, "new_attn_workspace: not while a stream is being captured")
         nbytes = lib().dsuf_attn_workspace_bytes(self.h)
         w = t.empty(nbytes, dtype=t.uint8, device=self.device)
         self.check(lib().dsuf_attn_workspace_init(self.h, self.stream(), w.data_ptr(), nbytes))
-        if not t.cuda.is_current_stream_capturing():
-            t.cuda.current_stream(self.index).synchronize()     # (its first user may be another stream)
+        t.cuda.current_stream(self.index).synchronize()     # (its first user may be another stream)
         return w
 
     def set_decode_path(self, tcgen05):

@@ -288,3 +288,14 @@ def test_workspace_init_refuses_another_current_device(pkg, cblock):
     text = C.create_string_buffer(512)
     pkg.lib().dsuf_last_error(cblock, text, 512)
     assert text.value.startswith(b"attn_workspace_init"), text.value
+
+
+def test_no_new_workspace_under_capture(pkg):
+    """Its zeroing would only be recorded, and a call before the graph's first replay would find arbitrary counters."""
+    done = []
+    t = types.SimpleNamespace(uint8=torch.uint8, empty=lambda *a, **k: done.append("empty") or torch.zeros(8, dtype=torch.uint8),
+                              cuda=types.SimpleNamespace(is_current_stream_capturing=lambda: True, current_stream=lambda d: None))
+    ctx = types.SimpleNamespace(torch=t, h=None, device=torch.device("cpu"), index=0, check=lambda rc: None, stream=lambda: None)
+    with pytest.raises(pkg.DsufError, match="captur"):
+        pkg.Ctx.new_attn_workspace(ctx)
+    assert not done
