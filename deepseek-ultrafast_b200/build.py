@@ -1,4 +1,4 @@
-"""In-tree build of libdsuf_qmm.so (nvcc, sm_100a only) and of the Python module dsuf_hostcall.so (g++).
+"""In-tree build of libdsuf_qmm.so (nvcc, sm_100a only) and, where torch can be imported, of the Python module dsuf_hostcall.so (g++).
 
 ``python deepseek-ultrafast_b200/build.py`` or ``build()`` from Python.  Objects are cached under
 ``csrc/build/`` and rebuilt when a source or header is newer.
@@ -12,6 +12,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libdsuf_qmm.so")
 HOSTCALL = os.path.join(HERE, "dsuf_hostcall.so")
+HOSTCALL_FOR = os.path.join(CSRC, "build", "hostcall.for")     # the torch and Python that the module was built for
 SOURCES = ["abi.cu", "quant.cu", "moe_aux.cu", "stream_launch.cu", "noalloc.cu", "ep_comm.cu", "peak_probe.cu", "lm_head.cu", "kv_cache.cu", "attn_decode.cu", "attn_prompt.cu", "sample.cu", "pack.cc", "loader.cc"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC",
@@ -38,12 +39,23 @@ def _compile(src, obj, log):
 
 def build_hostcall():
     """dsuf_hostcall.so: the Python entries that check tensors and call the library in native code (csrc/hostcall.cc), against the torch and Python
-    that run this."""
+    that run this.  None without torch, or with one that has no CUDA: the library itself needs neither."""
+    import importlib.util
     import sysconfig
+    if importlib.util.find_spec("torch") is None:
+        return None
     import torch
+    if torch.version.cuda is None:
+        return None
     src, header = os.path.join(CSRC, "hostcall.cc"), os.path.join(HERE, "..", "include", "dsuf_qmm.h")
+    made_for = f"torch {torch.__version__} in {os.path.dirname(torch.__file__)}, Python {sys.version}\n"
     if os.path.exists(HOSTCALL) and os.path.getmtime(HOSTCALL) >= max(os.path.getmtime(src), os.path.getmtime(header)):
-        return HOSTCALL
+        try:
+            with open(HOSTCALL_FOR) as f:
+                if f.read() == made_for:
+                    return HOSTCALL
+        except OSError:
+            pass
     root = os.path.dirname(torch.__file__)
     includes = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include")]
     cuda = os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")
@@ -54,6 +66,9 @@ def build_hostcall():
     if r.returncode != 0:
         raise RuntimeError("g++ failed on hostcall.cc:\n" + r.stderr)
     os.replace(HOSTCALL + ".tmp", HOSTCALL)
+    os.makedirs(os.path.dirname(HOSTCALL_FOR), exist_ok=True)
+    with open(HOSTCALL_FOR, "w") as f:
+        f.write(made_for)
     return HOSTCALL
 
 
