@@ -30,7 +30,7 @@
 // output share it); it is set 7 below the maximum so that p <= 2^15 and p's fp16 form keeps full precision down to 2^-21 of
 // the largest.  Scores, sums and outputs are fp32.  As operand of the second product p is rounded to fp16
 // (e4m3 cache), or split into two bf16 numbers (bf16 cache, whose values fix the operands' type): one alone would make the output's error 1.4 times
-// that of its own rounding, the second costs 1 % of the time.  e4m3 codes are widened exactly to fp16; the query is scaled by a power of two into fp16's range first.
+// that of its own rounding, the second costs 1 % of the time.  e4m3 codes are widened exactly to fp16; every query head is scaled by a power of two into fp16's range first.
 #include "internal.h"
 
 namespace dsuf {
@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(AD_THREADS, 2) attn_decode_kernel(const Decode
         const int frag = min((int)(segs << seg), at.nu - at.u);         // units
         // query operand: column n = head, k = 16 columns of the head per step
         uint32_t qf[KS][NT][2];
-        float q_unscale = 1.f;
+        float sl2[NT][2];        // log2(e) times the scale of the scores, of the heads 2 quad and 2 quad + 1
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int h = nt * 8 + row8;
@@ -443,12 +443,12 @@ __global__ void __launch_bounds__(AD_THREADS, 2) attn_decode_kernel(const Decode
             }
         }
         if constexpr (FP8) {
-            // largest finite magnitude of the block -> a power of two that brings it to about 2^14
-            uint32_t top = 0;
+            // a head's largest finite magnitude -> a power of two that brings it to about 2^14
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
+            for (int nt = 0; nt < NT; ++nt) {
+                uint32_t top = 0;
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -456,19 +456,23 @@ __global__ void __launch_bounds__(AD_THREADS, 2) attn_decode_kernel(const Decode
                             const uint32_t m = (qf[ks][nt][j] >> (16 * e)) & 0x7fffu;
                             if (m < 0x7f80u) top = max(top, m);
                         }
-            top = __reduce_max_sync(0xffffffffu, top);
-            const int shift = min(max(14 - ((int)(top >> 7) - 127), -120), 120);
-            const float up = __uint_as_float((uint32_t)(shift + 127) << 23);
-            q_unscale = __uint_as_float((uint32_t)(127 - shift) << 23);
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const int shift = min(max(14 - ((int)(top >> 7) - 127), -120), 120);
+                const float up = __uint_as_float((uint32_t)(shift + 127) << 23);
+                const float scale = a.scale_log2 * __uint_as_float((uint32_t)(127 - shift) << 23) * (a.k_scale ? __ldg(a.k_scale + kvh) : 1.f);
+                sl2[nt][0] = __shfl_sync(0xffffffffu, scale, quad * 8);
+                sl2[nt][1] = __shfl_sync(0xffffffffu, scale, quad * 8 + 4);
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
                         qf[ks][nt][j] = pack2<true>(__uint_as_float(qf[ks][nt][j] << 16) * up, __uint_as_float(qf[ks][nt][j] & 0xffff0000u) * up);
+            }
+        } else {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) sl2[nt][0] = sl2[nt][1] = a.scale_log2;
         }
-        const float sl2 = a.scale_log2 * q_unscale * (FP8 && a.k_scale ? __ldg(a.k_scale + kvh) : 1.f);
         float o[KS][NT][4], ref[NT][2], sum[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -530,16 +534,16 @@ __global__ void __launch_bounds__(AD_THREADS, 2) attn_decode_kernel(const Decode
                     const bool va = ta >= at.beg && ta < at.len, vb = tb >= at.beg && tb < at.len;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        st[nt][0] = va ? st[nt][0] * sl2 : -INFINITY;
-                        st[nt][1] = va ? st[nt][1] * sl2 : -INFINITY;
-                        st[nt][2] = vb ? st[nt][2] * sl2 : -INFINITY;
-                        st[nt][3] = vb ? st[nt][3] * sl2 : -INFINITY;
+                        st[nt][0] = va ? st[nt][0] * sl2[nt][0] : -INFINITY;
+                        st[nt][1] = va ? st[nt][1] * sl2[nt][1] : -INFINITY;
+                        st[nt][2] = vb ? st[nt][2] * sl2[nt][0] : -INFINITY;
+                        st[nt][3] = vb ? st[nt][3] * sl2[nt][1] : -INFINITY;
                     }
                 } else {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) st[nt][e] *= sl2;
+                        for (int e = 0; e < 4; ++e) st[nt][e] *= sl2[nt][e & 1];
                 }
                 bool over = false;
 #pragma unroll

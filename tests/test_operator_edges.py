@@ -299,3 +299,22 @@ def test_no_new_workspace_under_capture(pkg):
     with pytest.raises(pkg.DsufError, match="captur"):
         pkg.Ctx.new_attn_workspace(ctx)
     assert not done
+
+
+# ------------------------------------------------------------------ scores of very different sizes
+@gpu
+@pytest.mark.parametrize("d,hq,hkv,lens", [(128, 7, 1, [300, 40]), (64, 24, 2, [77, 900]), (128, 3, 1, [50] * 400)])
+def test_a_head_is_alone_with_its_scale(pkg, ectx, d, hq, hkv, lens):
+    """Over an e4m3 cache queries are brought into fp16's range: one head's size does not touch another's result."""
+    cache, q, table, n = A.decode_inputs(pkg, ectx, 41, lens, hq, hkv, d, 16, True)
+    q = q.reshape(len(lens), hq, d).clone()
+    q[:, 1] *= 2.0 ** 60
+    q[:, 2] *= 2.0 ** -60
+    out, lse = pkg.attn_decode(ectx, cache, q.reshape(len(lens), -1), table, n, return_lse=True)
+    torch.cuda.synchronize()
+    assert ectx.status().code == 0
+    want, wl, size = A.decode64(cache, q.reshape(len(lens), -1), table, lens, 0, d ** -0.5)
+    keep = [h for h in range(hq) if h != 1]         # (head 1: all weight on one key, but for ties within its scores' rounding)
+    pick = lambda x: x.reshape(len(lens), hq, d)[:, keep]   # noqa: E731
+    A.within(pick(out), pick(want), pick(size), terms=2 ** -8 + 2 ** -12)
+    assert ((lse.double() - wl)[:, keep].abs() <= 2 ** -12 + 2 ** -22 * wl[:, keep].abs()).all()
