@@ -749,7 +749,9 @@ extern "C" int32_t dsuf_attn_prompt(dsuf_ctx* ctx, void* stream, uint64_t q, int
     DSUF_REQUIRE(ctx, head_dim == 64 || head_dim == 128, "attn_prompt: head_dim (%d) must be 64 or 128", head_dim);
     DSUF_REQUIRE(ctx, kv_heads >= 1 && q_heads >= 1 && q_heads <= 4096 && q_heads % kv_heads == 0,
                  "attn_prompt: q_heads (%d) must be a multiple of kv_heads (%d), at most 4096", q_heads, kv_heads);
-    DSUF_REQUIRE(ctx, t >= 0 && t <= 0x7fff0000 && n_seqs >= 0, "attn_prompt: t must be in 0..2^31 - 65536 and n_seqs >= 0");
+    // (a CTA looks for its next pair 32 sequences and a level at a time; with 2^18 sequences that is at most 296 levels x 8192 steps of about 1000 cycles,
+    // as every other level has a pair, and stays inside the waits' limit of 4e9 cycles)
+    DSUF_REQUIRE(ctx, t >= 0 && t <= 0x7fff0000 && n_seqs >= 0 && n_seqs <= 1 << 18, "attn_prompt: t must be in 0..2^31 - 65536 and n_seqs in 0..2^18");
     DSUF_REQUIRE(ctx, ldq >= q_heads * head_dim && ldq % 8 == 0 && ldo >= q_heads * head_dim && ldo % 8 == 0 && ldk >= kv_heads * head_dim && ldk % 8 == 0 &&
                  ldv >= kv_heads * head_dim && ldv % 8 == 0, "attn_prompt: row strides must be multiples of 8 and hold all heads");
     DSUF_REQUIRE(ctx, window >= 0 && scale > 0.f && scale - scale == 0.f, "attn_prompt: window must be >= 0, scale positive and finite");

@@ -438,7 +438,7 @@ int32_t dsuf_attn_workspace_init(dsuf_ctx* ctx, void* stream, uint64_t workspace
 int32_t dsuf_attn_decode(dsuf_ctx* ctx, void* stream, const dsuf_kv_cache* cache, uint64_t q, int32_t ldq, int32_t q_heads, int32_t b,
                          uint64_t block_table, int32_t max_pages, uint64_t seq_lens, float scale, int32_t window, uint64_t out,
                          int32_t ldo, uint64_t lse, uint64_t workspace);
-/* Causal attention over packed prompts: rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1 (i32 [n_seqs + 1], device, ascending, at most t)
+/* Causal attention over packed prompts: rows cu_seqlens[i] .. cu_seqlens[i + 1] - 1 (i32 [n_seqs + 1], device, ascending, at most t; n_seqs <= 2^18)
  * of q, k, v, out are sequence i; row r of a sequence sees its rows max(0, r - window + 1) .. r (window 0: all up to r).
  * q / out bf16 [t][q_heads * head_dim], k / v bf16 [t][kv_heads * head_dim] (row strides ld*, so the parts of one merged projection can be
  * passed as they lie), lse f32 [t][q_heads] in memory of its own, or 0.  out shares no memory with q, k or v (columns of its own in their rows are no sharing).  Rows that belong to no sequence are left as they were, and nothing of them is

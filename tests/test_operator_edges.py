@@ -318,3 +318,19 @@ def test_a_head_is_alone_with_its_scale(pkg, ectx, d, hq, hkv, lens):
     pick = lambda x: x.reshape(len(lens), hq, d)[:, keep]   # noqa: E731
     A.within(pick(out), pick(want), pick(size), terms=2 ** -8 + 2 ** -12)
     assert ((lse.double() - wl)[:, keep].abs() <= 2 ** -12 + 2 ** -22 * wl[:, keep].abs()).all()
+
+
+# ------------------------------------------------------------------ sizes that the waits' limit would not cover
+def test_prompt_refuses_more_sequences_than_its_walk_is_made_for(pkg, cblock):
+    """A CTA looks for its next tiles in steps of 32 sequences and one level of lengths; at least every other level has a pair, and a CTA gets one of 148, so
+    it takes at most 296 n / 32 steps of about 1000 cycles, which other warps' waits of 4e9 cycles have to cover."""
+    limit = 1 << 18
+    assert 296 * limit / 32 * 1000 < 4e9
+
+    def call(n):
+        rc = pkg.lib().dsuf_attn_prompt(cblock, None, P, ROW, P + 1024, ROW, P + 1536, ROW, 9, 4, 2, 128, P - 4096, n, 0.1, 0, P + (1 << 20), 512, 0)
+        text = C.create_string_buffer(512)
+        pkg.lib().dsuf_last_error(cblock, text, 512)
+        assert rc != 0
+        return b"n_seqs" in text.value
+    assert call(limit + 1) and call(0x7fffffff) and not call(limit)
