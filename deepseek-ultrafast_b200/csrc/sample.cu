@@ -842,6 +842,15 @@ extern "C" int32_t dsuf_sample(dsuf_ctx* ctx, void* stream, uint64_t logits, int
     if (m == 0) return DSUF_OK;
     DSUF_REQUIRE(ctx, logits && u && ids_out && ((logits | u | ids_out | logprobs_out | temperature | top_k | top_p | min_p) & 3) == 0,
                  "sample: null or misaligned pointer");
+    const uint64_t bytes = 4ull * m;
+    auto meets = [&](uint64_t x, uint64_t y) { return x && y && x < y + bytes && y < x + bytes; };
+    bool apart = !meets(ids_out, logprobs_out);
+    for (uint64_t o : {ids_out, logprobs_out}) {
+        // (a row reads its settings before its result is written, so one of their columns may receive it)
+        for (uint64_t c : {temperature, top_k, top_p, min_p, u}) apart = apart && (o == c || !meets(o, c));
+        apart = apart && !(o && block_meets_rows(o, (long long)bytes, logits, 2 * ld, 2ll * n, m));      // (rows of n fp32: 2 n halves)
+    }
+    DSUF_REQUIRE(ctx, apart, "sample: ids and logprobs must share no memory with the logits, each other or (but for a whole column) the settings");
     DSUF_REQUIRE_DEVICE(ctx, "sample");
     SampleArgs a;
     memset(&a, 0, sizeof(a));

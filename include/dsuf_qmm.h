@@ -456,7 +456,8 @@ int32_t dsuf_attn_prompt(dsuf_ctx* ctx, void* stream, uint64_t q, int32_t ldq, u
  *   ids[row] = the lowest id i of C with weight(C, ids up to i) > u * weight(C), u in [0, 1).
  * temperature <= 0: the largest logit's lowest id.  NaN and -inf logits are never drawn; a row without any other gives -1.
  * temperature, top_p, min_p f32 [m], top_k i32 [m] (device), 0: 1, 1, 0 and 0 for every row; u f32 [m]; ids i32 [m];
- * logprobs f32 [m] or 0: log softmax(logits)[id] of the logits as they are (temperature 1, no limits).  Weights are 2^-40 fixed point and
+ * logprobs f32 [m] or 0: log softmax(logits)[id] of the logits as they are (temperature 1, no limits).  ids and logprobs share no
+ * memory with the logits or each other, and with a setting only as that whole column in place.  Weights are 2^-40 fixed point and
  * their sums exact, so equal inputs give equal tokens whatever the batch. */
 int32_t dsuf_sample(dsuf_ctx* ctx, void* stream, uint64_t logits, int64_t ld, int32_t m, int32_t n, uint64_t temperature, uint64_t top_k,
                     uint64_t top_p, uint64_t min_p, uint64_t u, uint64_t ids_out, uint64_t logprobs_out);

@@ -334,3 +334,16 @@ def test_prompt_refuses_more_sequences_than_its_walk_is_made_for(pkg, cblock):
         assert rc != 0
         return b"n_seqs" in text.value
     assert call(limit + 1) and call(0x7fffffff) and not call(limit)
+
+
+def test_sample_refuses_outputs_in_its_inputs(pkg, cblock):
+    """A setting's own column may receive the result (each row reads its settings first); nothing else may be shared."""
+    far = P + (1 << 22)
+
+    def refused(logits=P, ld=100, m=5, n=100, t=far, k=far + 64, p=far + 128, q=far + 192, u=far + 256, ids=far + 320, lp=far + 384):
+        return shares(pkg, cblock, pkg.lib().dsuf_sample(cblock, None, logits, ld, m, n, t, k, p, q, u, ids, lp))
+    for kw in [dict(ids=P), dict(lp=P + 4 * 499), dict(ids=P - 4), dict(ids=far + 68), dict(lp=far + 252), dict(lp=far + 320), dict(lp=far + 324), dict(lp=far + 4), dict(ids=far - 16),
+               dict(ids=P + 400, ld=101)]:
+        assert refused(**kw), kw
+    for kw in [{}, dict(ids=far + 64), dict(lp=far + 256), dict(lp=far), dict(lp=0), dict(t=0, k=0, p=0, q=0), dict(ids=P + 2000), dict(ids=P - 20), dict(ids=P + 400, ld=200), dict(ids=far + 44)]:
+        assert not refused(**kw), kw
