@@ -143,6 +143,7 @@ PyObject* kv_append(PyObject* const* a) {
     }
     uint64_t qp = 0, qo = 0, ko = 0;
     at::Tensor q_out;
+    if (given(a[11]) && !given(a[10])) refuse("kv_append: q_out without q");
     if (given(a[10])) {
         const at::Tensor& q = c.rows(a[10], "q", at::kBFloat16, n, -1, ldq);
         const int64_t w = q.size(1);

@@ -347,3 +347,10 @@ def test_sample_refuses_outputs_in_its_inputs(pkg, cblock):
         assert refused(**kw), kw
     for kw in [{}, dict(ids=far + 64), dict(lp=far + 256), dict(lp=far), dict(lp=0), dict(t=0, k=0, p=0, q=0), dict(ids=P + 2000), dict(ids=P - 20), dict(ids=P + 400, ld=200), dict(ids=far + 44)]:
         assert not refused(**kw), kw
+
+
+def test_append_refuses_a_place_for_queries_it_was_not_given(pkg, hctx):
+    cache = pkg.KvCache(hctx, z(4, 2, 16, 128), z(4, 2, 16, 128))
+    i = torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(pkg.DsufError, match="q_out"):
+        pkg.kv_append(hctx, cache, z(3, 256), z(3, 256), i, i.reshape(3, 1), q_out=z(3, 512))
