@@ -678,7 +678,7 @@ class KvCache:
 def kv_append(ctx, cache, k, v, pos, block_table, seq=None, rope=None, rope_half=False, q=None, q_out=None, k_out=None):
     """dsuf_kv_append: writes the tokens' keys (rotated) and values bf16 [t][kv_heads * head_dim] into the cache at positions
     ``pos`` i32 [t] of sequences ``seq`` i32 [t] (None: token i is sequence i), pages from ``block_table`` i32 [seqs][pages]; a
-    negative pos or seq is padding.  ``rope`` = (cos f32 [positions][rot/2], sin, off): columns [off, off + rot) of every head, in
+    negative pos or seq is padding (its rows of q_out and k_out are not written).  ``rope`` = (cos f32 [positions][rot/2], sin, off): columns [off, off + rot) of every head, in
     (even, odd) pairs or with ``rope_half`` in pairs rot/2 apart.  ``q`` bf16 [t][q_heads * head_dim]: rotated as well, into
     ``q_out`` (None: a new tensor; q itself: in place).  ``k_out``: receives the rotated keys as rows, for attn_prompt over these tokens (k
     itself: in place).  Returns q_out."""

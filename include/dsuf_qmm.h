@@ -401,7 +401,7 @@ int32_t dsuf_lm_head_bf16(dsuf_ctx* ctx, void* stream, uint64_t w, int32_t n, in
  *   k_scale/v_scale  f32 [kv_heads] on the device, E4M3 only; 0 = all ones
  * Device-side indexes are checked on the device: a page id outside [0, n_pages), a position outside the block table's row or
  * the rotation table, or a sequence outside [0, n_seqs) is never followed; it is reported as code 2 (inconsistent plan) by
- * dsuf_status_poll, and the token (append) or the 16 keys (attention) concerned are skipped. */
+ * dsuf_status_poll, and the token concerned is skipped (append), or the 16 keys concerned count as keys and values of zeros (attention). */
 enum { DSUF_KV_BF16 = 0, DSUF_KV_E4M3 = 1 };
 typedef struct {
     uint64_t k, v;
@@ -421,7 +421,7 @@ typedef struct {
  * the same tokens (k_out = k with ldko = ldk: in place).  Otherwise q_out and k_out share no memory with q, k, v or each other (columns of their own
  * in the same rows are no sharing).  k, v bf16 [t][kv_heads * head_dim] (row strides ldk, ldv), q / q_out bf16
  * [t][q_heads * head_dim]; pos i32 [t], seq i32 [t] (0: token i belongs to sequence i, t <= n_seqs).  A token with a negative
- * pos or seq is padding: nothing of it is written.  The (seq, pos) pairs of one call must be distinct, and distinct sequences must not
+ * pos or seq is padding: nothing of it is written, its rows of q_out and k_out stay as they were.  The (seq, pos) pairs of one call must be distinct, and distinct sequences must not
  * share the pages that are written: which of two writes to one slot lands is undefined. */
 int32_t dsuf_kv_append(dsuf_ctx* ctx, void* stream, const dsuf_kv_cache* cache, uint64_t k, int32_t ldk, uint64_t v, int32_t ldv, int32_t t,
                        uint64_t pos, uint64_t seq, uint64_t block_table, int32_t n_seqs, int32_t max_pages, const dsuf_rope* rope,
@@ -432,7 +432,8 @@ int32_t dsuf_kv_append(dsuf_ctx* ctx, void* stream, const dsuf_kv_cache* cache, 
  * q / out bf16 [b][q_heads * head_dim] (out = q with ldo = ldq: in place; otherwise they share no memory); lse f32 [b][q_heads] = log of the sum of
  * exp(scale * <q, k>), in memory of its own, or 0.
  * q_heads a multiple of kv_heads.  workspace: dsuf_attn_workspace_bytes(ctx), zeroed once by dsuf_attn_workspace_init; the kernel
- * leaves its counters zeroed.  Calls (and captured graphs) that share one workspace must be stream-ordered. */
+ * leaves its counters zeroed.  Calls (and captured graphs) that share one workspace must be stream-ordered.  Scores are fp32 and carry a factor
+ * log2(e): they have to stay below 2^127 in magnitude, here and in dsuf_attn_prompt. */
 size_t dsuf_attn_workspace_bytes(dsuf_ctx* ctx);
 int32_t dsuf_attn_workspace_init(dsuf_ctx* ctx, void* stream, uint64_t workspace, size_t bytes);
 int32_t dsuf_attn_decode(dsuf_ctx* ctx, void* stream, const dsuf_kv_cache* cache, uint64_t q, int32_t ldq, int32_t q_heads, int32_t b,
