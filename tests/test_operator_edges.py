@@ -354,3 +354,41 @@ def test_append_refuses_a_place_for_queries_it_was_not_given(pkg, hctx):
     i = torch.zeros(3, dtype=torch.int32)
     with pytest.raises(pkg.DsufError, match="q_out"):
         pkg.kv_append(hctx, cache, z(3, 256), z(3, 256), i, i.reshape(3, 1), q_out=z(3, 512))
+
+
+@gpu
+@pytest.mark.parametrize("scale", [1.0, 20.0])
+def test_large_scores_within_their_own_rounding(pkg, ectx, scale):
+    """Scores of thousands and tens of thousands that grow along the context.  A score is a sum of d products in fp32, in the tensor core at worst cut and not rounded
+    (2^-23 each time), times the scale and log2(e) (2^-22): it is off by at most E = (d + 2) 2^-23 scale sum |q k|.  So lse is off by E and its own rounding, a row's
+    weights by factors between exp(-2 E) and exp(2 E), and where all weights but the largest add up to r, the output by no more than 2 r exp(2 E)
+    of the largest value."""
+    g = A.gen(21)
+    d, n, hq = 128, 700, 2
+    q, k, v = A.bf16(g, n, hq * d), A.bf16(g, n, d), A.bf16(g, n, d)
+    k *= (1.0 + torch.arange(n, device=DEV)[:, None] * 0.2).to(torch.bfloat16)
+    cu = i32(0, n)
+    out, lse = pkg.attn_prompt(ectx, q, k, v, cu, scale=scale, return_lse=True)
+    cache = pkg.KvCache.empty(ectx, 44, 16, 1, d)
+    table = torch.arange(44, dtype=torch.int32, device=DEV).reshape(1, 44)
+    pkg.kv_append(ectx, cache, k, v, torch.arange(n, dtype=torch.int32, device=DEV), table, seq=torch.zeros(n, dtype=torch.int32, device=DEV))
+    lens = torch.arange(1, n + 1, dtype=torch.int32, device=DEV)
+    out1, lse1 = pkg.attn_decode(ectx, cache, q, table.repeat(n, 1), lens, scale=scale, return_lse=True)
+    torch.cuda.synchronize()
+    assert ectx.status().code == 0
+    want, wl, size = A.prompt64(q, k, v, [n], hq, 1, d, 0, scale)
+    q64, k64 = q.double().reshape(n, hq, d), k.double()
+    hidden = torch.ones(n, n, dtype=torch.bool, device=DEV).triu(1)
+    sharp = 0
+    for h in range(hq):
+        s = (q64[:, h] @ k64.T * scale).masked_fill(hidden, -math.inf)
+        e = ((q64[:, h].abs() @ k64.abs().T) * scale).masked_fill(hidden, 0).amax(1) * (d + 2) * 2 ** -23
+        top = s.amax(1, keepdim=True)
+        r = torch.exp(s - top).sum(1) - 1
+        off = torch.minimum(2 * r * torch.exp(2 * e), torch.full_like(r, 4.0)) * v.double().abs().amax()
+        sharp += (off < 2 ** -6).sum().item()
+        for o, l in ((out, lse), (out1, lse1)):
+            assert ((l[:, h].double() - wl[:, h]).abs() <= e + 2 ** -12 + 2 ** -22 * wl[:, h].abs()).all()
+            got, w, z = (x.reshape(n, hq, d)[:, h] for x in (o.double(), want, size))
+            assert ((got - w).abs() <= 2 ** -8 * w.abs() + (2 ** -8 + 2 ** -12) * z + off[:, None]).all()
+    assert sharp > n * hq / 2             # (most rows are compared closely)
