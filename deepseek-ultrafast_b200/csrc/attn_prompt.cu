@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
     extern __shared__ uint8_t smem_raw[];
     uint8_t* base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     uint8_t* ring = base + 2 * S::TILE;
-    __shared__ __align__(8) uint64_t q_full[2], q_empty[2], kv_full[S::STAGES], kv_empty[S::STAGES], s_full[2], p_full[2], o_full[2];
+    __shared__ __align__(8) uint64_t q_full[2], q_empty[2], kv_full[S::STAGES], kv_empty[S::STAGES], s_full[2], p_full[2], o_full[2], drained[2];
     __shared__ uint32_t s_tmem;
     __shared__ int s_odd[8];         // softmax warps that have met outputs which are not finite
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -414,6 +414,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
             mbar_init(&s_full[t], 1);
             mbar_init(&p_full[t], 4);
             mbar_init(&o_full[t], 1);
+            mbar_init(&drained[t], 1);
         }
         for (int s = 0; s < S::STAGES; ++s) {
             mbar_init(&kv_full[s], 1);
@@ -437,11 +438,12 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
             prefetch_tmap(&a.tm_v);
         }
         int st = 0;
-        uint32_t ph = 0, qn[2] = {0, 0};
+        uint32_t ph = 0, qn[2] = {0, 0}, copied = 0, qcopied[2] = {0, 0};
         long long n = 0;
         auto kv = [&](const PromptPair& p, const CUtensorMap* map, int j) {
             if (n >= S::STAGES && !dead && !mbar_wait(&kv_empty[st], ph ^ 1, a.status, KID_PROMPT, 1)) dead = true;
-            if (warp_elect()) {
+            if (warp_elect() && !dead) {        // (else nothing is copied any more, and what has been is awaited below)
+                ++copied;
                 mbar_expect_tx(&kv_full[st], S::TILE);
 #pragma unroll
                 for (int b = 0; b < S::BOXES; ++b)
@@ -460,7 +462,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
                 const PromptTile q = t ? p.t1 : p.t0;
                 if (q.hi == 0) continue;
                 if (qn[t] > 0 && !dead && !mbar_wait(&q_empty[t], (qn[t] - 1) & 1, a.status, KID_PROMPT, 2)) dead = true;
-                if (warp_elect()) {
+                if (warp_elect() && !dead) {
+                    ++qcopied[t];
                     mbar_expect_tx(&q_full[t], S::TILE);
 #pragma unroll
                     for (int b = 0; b < S::BOXES; ++b)
@@ -473,6 +476,14 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
                 if (j > p.jlo) kv(p, &a.tm_k, j);
                 kv(p, &a.tm_v, j);
             }
+        }
+        // no CTA ends with copies on their way: the last one into each stage, and of each tile's queries
+        copied = __reduce_add_sync(0xffffffffu, copied);
+        for (uint32_t s = 0; s < min(copied, (uint32_t)S::STAGES); ++s) mbar_wait(&kv_full[s], ((copied - 1 - s) / S::STAGES) & 1, a.status, KID_PROMPT, 8);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const uint32_t of = __reduce_add_sync(0xffffffffu, qcopied[t]);
+            if (of > 0) mbar_wait(&q_full[t], (of - 1) & 1, a.status, KID_PROMPT, 9);
         }
     } else if (warp >= 9) {
         // ---------------- tensor core issuer of tile t ----------------
@@ -590,6 +601,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1) attn_prompt_kernel(const __grid
             mine = then;
         }
         if (t == 0) take_turn();     // (the last turn that tile 1 has passed on)
+        // nor with products on their way, whose operands and results the CTA's memory holds
+        if (warp_elect()) tc_commit(&drained[t]);
+        __syncwarp();
+        mbar_wait(&drained[t], 0, a.status, KID_PROMPT, 10);
     } else {
         // ---------------- softmax: tile t, one row per thread ----------------
         const int t = warp >> 2;

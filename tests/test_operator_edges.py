@@ -392,3 +392,29 @@ def test_large_scores_within_their_own_rounding(pkg, ectx, scale):
             got, w, z = (x.reshape(n, hq, d)[:, h] for x in (o.double(), want, size))
             assert ((got - w).abs() <= 2 ** -8 * w.abs() + (2 ** -8 + 2 ** -12) * z + off[:, None]).all()
     assert sharp > n * hq / 2             # (most rows are compared closely)
+
+
+# ------------------------------------------------------------------ the prompt kernel's end
+def test_no_copies_or_products_outlive_the_prompt_kernel(pkg):
+    """After a wait that has run out a CTA still frees its memory: its text has waits for the copies and the products that it has issued on every way to the
+    end, and copies stop at the first such wait.  (The waits cannot run out in a test: nothing that could make them is reachable from outside.)"""
+    import re
+    with open(os.path.join(os.path.dirname(pkg.__file__), "csrc", "attn_prompt.cu")) as f:
+        text = re.sub(r"//[^\n]*", "", f.read())
+    body = text[text.index("attn_prompt_kernel(const"):]
+    body = body[:body.index("tmem_dealloc")]
+    producer = body[body.index("if (warp == 8) {", body.index("PromptWalk walk(a)")):body.index("else if (warp >= 9)")]
+    issuer = body[body.index("else if (warp >= 9)"):body.index("const uint32_t lanes")]
+    for part, issued, waits in ((producer, "tma_2d_nh", ("mbar_wait(&kv_full", "mbar_wait(&q_full")), (issuer, "pa_mma_ts", ("tc_commit(&drained", "mbar_wait(&drained"))):
+        for w in waits:
+            assert part.rindex(w) > part.rindex(issued), w
+    for m in re.finditer("tma_2d_nh", producer):
+        assert "warp_elect() && !dead" in producer[max(0, m.start() - 600):m.start()]
+    # the phase that the last of n copies into ring slot s completes, counted copy by copy
+    for stages in (4, 8):
+        for n in range(1, 40):
+            fills = [0] * stages
+            for i in range(n):
+                fills[i % stages] += 1
+            for s in range(min(n, stages)):
+                assert (n - 1 - s) // stages % 2 == (fills[s] - 1) % 2
