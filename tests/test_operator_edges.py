@@ -418,3 +418,18 @@ def test_no_copies_or_products_outlive_the_prompt_kernel(pkg):
                 fills[i % stages] += 1
             for s in range(min(n, stages)):
                 assert (n - 1 - s) // stages % 2 == (fills[s] - 1) % 2
+
+
+@gpu
+def test_prompts_of_nothing(pkg, ectx):
+    """Sequences without rows: nothing is written, and the next call finds everything in order."""
+    q = A.bf16(A.gen(5), 300, 128)
+    out, lse = torch.full_like(q, 3.0), torch.full((300, 1), 3.0, device=DEV)
+    for cu in (i32(0, 0), i32(0, 0, 0, 0), i32(300, 300), i32(7, 7, 7)):
+        pkg.attn_prompt(ectx, q, q, q, cu, out=out, lse=lse)
+        torch.cuda.synchronize()
+        assert (out == 3.0).all() and (lse == 3.0).all() and ectx.status().code == 0
+    pkg.attn_prompt(ectx, q, q, q, i32(0, 0, 300, 300), out=out, lse=lse)
+    want, wl, size = A.prompt64(q, q, q, [0, 300, 0], 1, 1, 128, 0, 128 ** -0.5)
+    A.within(out, want, size, terms=2 ** -8 + 2 ** -12)
+    assert ectx.status().code == 0
