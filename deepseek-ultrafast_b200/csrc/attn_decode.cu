@@ -2,8 +2,9 @@
 // sliding window, bf16 or e4m3 cache.
 //
 // out = sum_j exp(scale <q, k_j> - top) v_j / sum_j exp(scale <q, k_j> - top), one pass over the cache: HBM-bound, every
-// visible key and value is read once and serves all query heads of its group (64 contexts of up to 8192 tokens, 56 / 8 heads of 128: 188 us = 6.1 TB/s,
-// 0.93 of the measured copy bandwidth; one of 131071: 93.5 us, 0.88).
+// visible key and value is read once and serves all query heads of its group (64 contexts of up to 8192 tokens, 56 / 8 heads of 128: 191 us = 6.0 TB/s,
+// 0.92 of the measured copy bandwidth; one of 131071: 93 us, 0.88).  Groups of more than 16 heads read their keys once per 16 (32 contexts of 8192 over one kv head:
+// 16 heads 37 us, 32 heads 50, 64 heads 76).
 //
 // Work split.  A piece is (sequence, kv head, block of 8 NT query heads); its keys are cut into units of 4 warps x CH tokens
 // (CH tokens = 4 KB of keys), and all pieces' units, laid end to end, are dealt to the CTAs (two per SM) in equal contiguous
@@ -13,8 +14,8 @@
 // so the result does not depend on timing.  Where there are few units, segments of four of one piece are dealt instead of units (8 contexts
 // of 1000 tokens, 56 / 8 heads of 128: 12.8 us instead of 14.5; one of 16000, one kv head: 14.0 instead of 24.6).  Where every piece is short (four
 // units at most) and there is one for each CTA that the GPU holds, a warp takes whole pieces alone and writes them itself: no barrier and no other warp's part to add
-// (56 / 8 heads of 128; 512 contexts of 128 tokens: 56 us instead of 68; 256 of 1 to 256: 37 instead of 61; 64 of 40: 7.6 instead of 10; with half as many pieces
-// as CTAs it would lose: 32 of 100 tokens 9.6 instead of 7.6).
+// (56 / 8 heads of 128; 512 contexts of 128 tokens: 56 us instead of 68; 256 of 1 to 256: 37 instead of 61; 64 of 40: 7.6 instead of 10; with fewer pieces than
+// CTAs it would lose: 256 pieces of 100 tokens 9.6 instead of 7.6).
 //
 // Inside a CTA every warp runs alone: a private ring of three stages (4 KB keys + 4 KB values each, cp.async, zero-filled
 // outside the visible range so that stale values behind a sequence cannot reach the sums), no barrier until the end of a

@@ -16,12 +16,14 @@
 // issued before the last output is stored.  The two issuing warps take strict turns (P0 V, S0, P1 V, S1): issuing blocks while the tensor
 // core's short queue is full, so the barrier waits of one tile (100 cycles and more each, even when met) have to pass while the
 // other's products are issued; without turns the tiles fall into step, and both softmaxes share the exponential unit and then both wait.
-// (8192 tokens, 56 / 8 heads of 128: one issuing warp 867 us, two without turns 1022, two with turns 778; now 757 = 1270 TFLOP/s
-// of visible pairs, with the tensor pipe and the exponential unit each 54 % busy.)
+// (8192 tokens, 56 / 8 heads of 128: one issuing warp 867 us, two without turns 1022, two with turns 778; now 755 to 795 from one GPU to another,
+// 1270 TFLOP/s of visible pairs at best; in a capture of 4096 tokens the tensor pipe was 54 % and the exponential unit 55 % busy.)
 // Tensor memory (512 columns): S0 S1 (128 fp32 columns each; P_t overwrites the first 64 of S_t as packed bf16), O0 O1 (D each).
 // The reference point of a row is the largest of 16 or 32 scores of its first tile and only moves when a tile's weights add up to more than 2^24 (exact: the
 // sum and the output share the reference, and bf16's and fp32's precision does not depend on the magnitude), so usual tiles need no maximum at
-// all.  p is rounded once to bf16 as operand; sums, statistics and outputs are fp32.
+// all.  Sums, statistics and outputs are fp32.  p is rounded once to bf16 as operand: the outputs' error against 64 bits is then 0.0020 of their norm, where
+// that of their own rounding is 0.0016.  A second bf16 number for what the rounding leaves, as decode attention has it, would take 64 registers more
+// of a softmax thread that has none left, twice the stores of p and half as many products again (here the tensor core is as tight as anything).
 //
 // Pairs are ordered from the longest rows to the shortest, those of all sequences together, and dealt to the CTAs back and forth, which
 // leaves the CTAs within 1 or 2 % of one another (9 prompts of 900 to 2600 tokens: 332 us; sequence after sequence 8 % apart and 342; one of 2048 69 instead of 74).  Values behind a sequence's end inside its last tile belong to another sequence (or nobody) and are
@@ -54,7 +56,7 @@ struct PromptArgs {
     float* lse;
     int ldo, t, q_heads, kv_heads, group, n_seqs, window;
     const int* cu;
-    float scale, scale_log2;
+    float scale_log2;
     DevStatus* status;
 };
 
@@ -790,7 +792,6 @@ extern "C" int32_t dsuf_attn_prompt(dsuf_ctx* ctx, void* stream, uint64_t q, int
     a.out = (bf16*)out; a.lse = (float*)lse; a.ldo = ldo; a.t = t;
     a.q_heads = q_heads; a.kv_heads = kv_heads; a.group = q_heads / kv_heads; a.n_seqs = n_seqs; a.window = window;
     a.cu = (const int*)cu_seqlens;
-    a.scale = scale;
     a.scale_log2 = scale * 1.4426950408889634f;
     a.q = (const bf16*)q; a.k = (const bf16*)k; a.v = (const bf16*)v;
     a.ldq = ldq; a.ldk = ldk; a.ldv = ldv;
