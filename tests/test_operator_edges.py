@@ -433,3 +433,19 @@ def test_prompts_of_nothing(pkg, ectx):
     want, wl, size = A.prompt64(q, q, q, [0, 300, 0], 1, 1, 128, 0, 128 ** -0.5)
     A.within(out, want, size, terms=2 ** -8 + 2 ** -12)
     assert ectx.status().code == 0
+
+
+@gpu
+@pytest.mark.parametrize("m,n", [(1, 129280), (64, 5000), (300, 70)])
+@pytest.mark.parametrize("settings", [dict(), dict(top_k=20, top_p=0.9), dict(top_p=0.7), dict(temperature=0.0), dict(min_p=0.05)])
+def test_results_in_the_columns_of_settings(pkg, ectx, m, n, settings):
+    """Tokens may replace top_k, and log-probabilities the uniform numbers, row for row."""
+    g = A.gen(m + n)
+    x, u = torch.empty(m, n, device=DEV).normal_(0, 2, generator=g), torch.rand(m, generator=g, device=DEV)
+    x[m // 2] = -math.inf
+    kw = {k: torch.full((m,), v, dtype=torch.int32 if k == "top_k" else torch.float32, device=DEV) for k, v in settings.items()}
+    kw.setdefault("top_k", torch.zeros(m, dtype=torch.int32, device=DEV))
+    ids, lp = pkg.sample(ectx, x, u, return_logprobs=True, **kw)
+    got, got_lp = pkg.sample(ectx, x, u, ids=kw["top_k"], logprobs=u, return_logprobs=True, **kw)
+    assert got is kw["top_k"] and got_lp is u
+    assert torch.equal(got, ids) and torch.equal(got_lp, lp)
